@@ -10,7 +10,7 @@ uint8 [pages][nkv][1152]): 16 tokens x 128 dims of codes n + 8 (n in -8..7),
 then bf16 scales [token][4], one per 32 dims; the value is n * scale.
 K codes: dim 32 j + 8 w + i of a token at byte token*64 + w*16 + j*4 + i/2.
 V codes: dim 32 j + 4 g + i of token 8 a + 2 w + b at byte
-(4 g + w)*32 + (2 a + b)*8 + 2 j + i/2.  Even i: the low half of the byte.
+a*512 + (4 g + w)*16 + b*8 + 2 j + i/2.  Even i: the low half of the byte.
 """
 import random
 
@@ -277,9 +277,9 @@ def _k_values(cache):
 
 
 def _v_values(cache):
-    c = _halves(cache[..., :CODES].unflatten(-1, (8, 4, 2, 2, 4, 2)))      # g, w, a, b, j, i/2, i%2
+    c = _halves(cache[..., :CODES].unflatten(-1, (2, 8, 4, 2, 4, 2)))      # a, g, w, b, j, i/2, i%2
     n = c.dim() - 7
-    c = c.permute(*range(n), n + 2, n + 1, n + 3, n + 4, n, n + 5, n + 6)  # a, w, b, j, g, i/2, i%2
+    c = c.permute(*range(n), n, n + 2, n + 3, n + 4, n + 1, n + 5, n + 6)  # a, w, b, j, g, i/2, i%2
     return _values(c.flatten(-4).flatten(-4, -2), _scales(cache))
 
 
@@ -316,7 +316,7 @@ def _plain_write(s):
     page, t = s["table"][s["row_seq"].long(), pos // PAGE].long(), pos % PAGE
     (kc, ks), (vc, vs) = _quantise(k), _quantise(v)
     s["k_cache"][..., :CODES].unflatten(-1, (PAGE, 64))[page, :, t] = _k_bytes(kc)
-    s["v_cache"][..., :CODES].unflatten(-1, (8, 4, 4, 8))[page, :, :, t % 8 // 2, t // 8 * 2 + t % 2] = _v_bytes(vc)
+    s["v_cache"][..., :CODES].unflatten(-1, (2, 8, 4, 2, 8))[page, :, t // 8, :, t % 8 // 2, t % 2] = _v_bytes(vc)
     _scales(s["k_cache"])[page, :, t] = ks
     _scales(s["v_cache"])[page, :, t] = vs
     # read the rows back out of the pages
@@ -434,7 +434,7 @@ def _read64(cache, which, table, n):
     if which == "k":
         byte, i = t * 64 + d % 32 // 8 * 16 + d // 32 * 4 + d % 8 // 2, d % 2
     else:
-        byte, i = (4 * (d % 32 // 4) + t % 8 // 2) * 32 + (2 * (t // 8) + t % 2) * 8 + 2 * (d // 32) + d % 4 // 2, d % 2
+        byte, i = t // 8 * 512 + (4 * (d % 32 // 4) + t % 8 // 2) * 16 + t % 2 * 8 + 2 * (d // 32) + d % 4 // 2, d % 2
     code = (page[:, :, byte].long() >> (4 * i)) & 15
     at = CODES + 2 * (4 * t + d // 32)
     bits = page[:, :, at].long() | (page[:, :, at + 1].long() << 8)
