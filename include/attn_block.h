@@ -99,6 +99,23 @@ moe_status_t attn_paged_rows(const void* q_bf16, const void* k_cache, const void
                              size_t workspace_bytes, void* out_bf16, void* out_q, float* out_s, int out_ld,
                              int* error_word, cwStream_t stream);
 
+/* Causal attention over whole prompts given as packed rows, no pages: rows
+ * [cu_seqlens[s], cu_seqlens[s + 1]) (device int32 [num_seqs + 1], ascending,
+ * within 0..T) are the tokens of sequence s, and
+ *   out[t][h] = sum_j softmax_j(q[t][h] . k[j][h / G] * scale) v[j][h / G],
+ * j from the sequence's first row to t, G = nq / nkv at most 16.  q bf16
+ * [T][nq][128] and k, v bf16 rows of nkv heads; consecutive rows lie q_stride,
+ * k_stride, v_stride elements apart (multiples of 8, so v may stay inside the
+ * qkv projection's rows); 16-byte aligned.  out_bf16 [T][nq][128], out_q and
+ * out_s as in attn_decode_paged.  Rows in no sequence are left as they were.
+ * From the first bound that is out of order or outside 0..T on, sequences are
+ * skipped (*error_word = 5).  A NaN or infinity in k or v reaches the rows that attend
+ * it and no others. */
+moe_status_t attn_prompt_packed(const void* q_bf16, long long q_stride, const void* k_bf16, long long k_stride,
+                                const void* v_bf16, long long v_stride, const int32_t* cu_seqlens, int num_seqs, int T,
+                                int nq, int nkv, int head_dim, float scale, void* out_bf16, void* out_q, float* out_s,
+                                int out_ld, int* error_word, cwStream_t stream);
+
 /* out[t][i] = bf16(residual[t][i] + sum_{r < tp} partial_r[t][i]), the ranks
  * summed in fp32 in order 0..tp-1 so every rank gets the same bits.
  * partials_dev: device array of tp pointers (this GPU's buffers, or peer

@@ -1,0 +1,207 @@
+"""attn_prompt_packed on the GPU against a plain 64-bit statement, within the
+bound that bf16 weights and outputs leave (kv_ref.attend)."""
+import numpy as np
+import pytest
+import torch
+
+import kv_ref as R
+from time_b200 import attn as A
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+
+
+def f64(t):
+    return t.double().cpu().numpy()
+
+
+def rows(rng, *shape):
+    return torch.from_numpy(rng.standard_normal(shape).astype(np.float32)).to(torch.bfloat16)
+
+
+def cu_of(lens, gpu, first=0):
+    return torch.tensor(np.concatenate([[first], first + np.cumsum(lens)]), dtype=torch.int32, device=gpu)
+
+
+def check(out, q, k, v, lens, scale, first=0):
+    at = first
+    for n in lens:
+        s = slice(at, at + n)
+        ref, tol = R.attend(f64(q[s]), f64(k[s]), f64(v[s]), np.arange(1, n + 1), scale)
+        got = f64(out[s])
+        assert (np.abs(got - ref) <= tol).all(), (n, np.max(np.abs(got - ref) / tol))
+        at += n
+
+
+@pytest.mark.parametrize("nq,nkv,lens", [
+    (12, 1, [1]), (12, 1, [1, 2, 3, 1]), (12, 1, [21, 22, 43, 64, 65]), (4, 4, [130, 1, 127, 128, 129]),
+    (1, 1, [300]), (16, 1, [100, 33]), (7, 1, [300, 5]), (6, 2, [257, 256, 255]), (96, 8, [150, 3, 40]),
+    (8, 8, [513]), (12, 1, [700, 10]), (2, 1, [1100]), (12, 1, [5] * 100)])
+def test_packed_prompts(gpu, nq, nkv, lens):
+    rng = np.random.default_rng(nq * 1000 + len(lens))
+    T = sum(lens)
+    q, k, v = rows(rng, T, nq, D).to(gpu), rows(rng, T, nkv, D).to(gpu), rows(rng, T, nkv, D).to(gpu)
+    err = torch.zeros(1, dtype=torch.int32, device=gpu)
+    out, _, _ = A.prompt_packed(q, k, v, cu_of(lens, gpu), D ** -0.5, error_word=err)
+    assert int(err) == 0
+    check(out, q, k, v, lens, D ** -0.5)
+
+
+@pytest.mark.parametrize("scale,mag", [(1.0, 4.0), (0.02, 1.0), (3.0, 0.01)])
+def test_sharp_and_flat_softmax(gpu, scale, mag):
+    """Weights concentrated on one key (the running maximum moves often) and spread evenly."""
+    rng = np.random.default_rng(1)
+    n = 600
+    q, k, v = (rows(rng, n, 2, D) * mag).to(gpu), (rows(rng, n, 1, D) * mag).to(gpu), rows(rng, n, 1, D).to(gpu)
+    k *= torch.linspace(0.2, 2, n, device=gpu)[:, None, None]        # later keys score higher
+    out, _, _ = A.prompt_packed(q, k, v, cu_of([n], gpu), scale)
+    check(out, q, k, v, [n], scale)
+
+
+def test_strides_empty_sequences_and_rows_outside(gpu):
+    """q, k and v inside the projection's rows, sequences of length 0, rows before the first and behind the last."""
+    rng = np.random.default_rng(2)
+    nq, nkv, T = 6, 2, 60
+    qkv = rows(rng, T, (nq + 2 * nkv) * D).to(gpu).unflatten(1, (nq + 2 * nkv, D))
+    q, k, v = qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:]
+    cu = torch.tensor([3, 3, 20, 20, 50, 50], dtype=torch.int32, device=gpu)
+    out = torch.full((T, nq, D), 7.0, dtype=torch.bfloat16, device=gpu)
+    A.prompt_packed(q, k, v, cu, 0.1, out=out)
+    check(out, q, k, v, [17, 30], 0.1, first=3)
+    assert (out[:3] == 7).all() and (out[50:] == 7).all()
+
+
+def test_from_a_bad_bound_on_sequences_are_skipped(gpu):
+    rng = np.random.default_rng(3)
+    q, k, v = rows(rng, 40, 2, D).to(gpu), rows(rng, 40, 1, D).to(gpu), rows(rng, 40, 1, D).to(gpu)
+    for cu, good in [([0, 30, 20, 40], [(0, 30)]), ([-1, 10, 20], []), ([0, 10, 41], [(0, 10)])]:
+        out = torch.full((40, 2, D), 7.0, dtype=torch.bfloat16, device=gpu)
+        err = torch.zeros(1, dtype=torch.int32, device=gpu)
+        A.prompt_packed(q, k, v, torch.tensor(cu, dtype=torch.int32, device=gpu), 0.1, out=out, error_word=err)
+        assert int(err) == 5
+        for a, b in good:
+            check(out[a:b], q[a:b], k[a:b], v[a:b], [b - a], 0.1)
+        untouched = [t for t in range(40) if not any(x <= t < y for x, y in good)]
+        assert (out[untouched] == 7).all()
+
+
+@pytest.mark.parametrize("nq,nkv", [(12, 1), (4, 4)])
+def test_nan_and_infinity_reach_only_the_rows_that_attend_them(gpu, nq, nkv):
+    rng = np.random.default_rng(4)
+    lens = [90, 300]
+    T = sum(lens)
+    q, k, v = rows(rng, T, nq, D), rows(rng, T, nkv, D), rows(rng, T, nkv, D)
+    clean = A.prompt_packed(q.to(gpu), k.to(gpu), v.to(gpu), cu_of(lens, gpu), 0.1)[0]
+    bad_v = v.clone()
+    bad_v[40, 0, 3] = float("inf")
+    bad_v[60, 0, 3] = float("-inf")
+    bad_v[41, 0, 9] = float("nan")
+    bad_v[89, 0] = float("nan")                            # last row of the first sequence
+    bad_v[90 + 135, 0, 5] = float("inf")
+    out = A.prompt_packed(q.to(gpu), k.to(gpu), bad_v.to(gpu), cu_of(lens, gpu), 0.1)[0]
+    G = nq // nkv
+    want = clean.clone()
+    want[40:60, :G, 3] = float("inf")
+    want[60:90, :G, 3] = float("nan")
+    want[41:90, :G, 9] = float("nan")
+    want[89, :G] = float("nan")
+    want[90 + 135:, :G, 5] = float("inf")
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(torch.isinf(out), torch.isinf(want))
+    fine = torch.isfinite(want)
+    assert torch.equal(out[fine], clean[fine]) and (out[40:60, :G, 3] > 0).all()
+    # keys: a NaN score makes the rows from there on NaN, those before keep their bits
+    bad_k = k.clone()
+    bad_k[90 + 140, 0, 0] = float("nan")
+    out = A.prompt_packed(q.to(gpu), bad_k.to(gpu), v.to(gpu), cu_of(lens, gpu), 0.1)[0]
+    assert torch.isnan(out[90 + 140:, :G]).all() and torch.equal(out[:90 + 140], clean[:90 + 140])
+    assert torch.equal(out[:, G:], clean[:, G:])
+    # and a NaN query its own row and head
+    bad_q = q.clone()
+    bad_q[17, nq - 1, 100] = float("nan")
+    out = A.prompt_packed(bad_q.to(gpu), k.to(gpu), v.to(gpu), cu_of(lens, gpu), 0.1)[0]
+    assert torch.isnan(out[17, nq - 1]).all()
+    out[17, nq - 1] = clean[17, nq - 1]
+    assert torch.equal(out, clean)
+
+
+def test_minus_infinite_scores(gpu):
+    """-inf scores weigh 0 as long as a row attends any other; a row of nothing else is 0 / 0."""
+    n = 200
+    q = torch.zeros(n, 1, D, dtype=torch.bfloat16, device=gpu)
+    k, v = torch.zeros_like(q), rows(np.random.default_rng(5), n, 1, D).to(gpu)
+    q[..., 0] = -3e38
+    k[:150, :, 0] = 64.0                                   # times the scale: below the fp32 range
+    out = f64(A.prompt_packed(q, k, v, cu_of([n], gpu), 4.0)[0])
+    assert np.isnan(out[:150]).all()
+    vf = f64(v)
+    for t in (150, 151, 199):
+        ref, size = vf[150:t + 1, 0].mean(axis=0), np.abs(vf[150:t + 1, 0]).mean(axis=0)
+        assert (np.abs(out[t, 0] - ref) <= 2.0 ** -8 * 1.01 * (np.abs(ref) + size) + 1e-6).all()
+
+
+def test_quantised_rows(gpu):
+    rng = np.random.default_rng(6)
+    lens, nq = [33, 100], 12
+    T = sum(lens)
+    q, k, v = rows(rng, T, nq, D).to(gpu), rows(rng, T, 1, D).to(gpu), rows(rng, T, 1, D).to(gpu)
+    v[5] = 0
+    v[0] = 0
+    out, oq, os_ = A.prompt_packed(q, k, v, cu_of(lens, gpu), 0.1, quant=True)
+    got = f64(out)
+    e4m3 = oq.view(torch.float8_e4m3fn).double().cpu().numpy().reshape(T, nq, D)
+    sc = os_.double().cpu().numpy()[:, :T].T[..., None]
+    # half an e4m3 step (2^-4, or 2^-10 below the smallest normal) of the fp32 row, which the bf16 row is 2^-8 from
+    amax = np.abs(got).max(axis=-1, keepdims=True) * (1 + 2.0 ** -7)
+    assert (np.abs(e4m3 * sc - got) <= (2.0 ** -4 + 2.0 ** -7) * np.abs(got) + amax / 448 * 2.0 ** -10 * 1.01).all()
+    assert not oq[0].any() and not os_[:, 0].any()
+    assert torch.equal(out, A.prompt_packed(q, k, v, cu_of(lens, gpu), 0.1)[0])
+
+
+def test_rows_do_not_depend_on_the_packing(gpu):
+    rng = np.random.default_rng(7)
+    lens, nq, nkv = [130, 7, 400], 12, 2
+    T = sum(lens)
+    q, k, v = rows(rng, T, nq, D).to(gpu), rows(rng, T, nkv, D).to(gpu), rows(rng, T, nkv, D).to(gpu)
+    out = A.prompt_packed(q, k, v, cu_of(lens, gpu), 0.1)[0]
+    at = 0
+    for n in lens:
+        one = A.prompt_packed(q[at:at + n].contiguous(), k[at:at + n], v[at:at + n], cu_of([n], gpu), 0.1)[0]
+        assert torch.equal(one, out[at:at + n])
+        at += n
+
+
+def test_stream_and_graph(gpu):
+    rng = np.random.default_rng(8)
+    q, k, v = rows(rng, 90, 4, D).to(gpu), rows(rng, 90, 2, D).to(gpu), rows(rng, 90, 2, D).to(gpu)
+    cu = cu_of([30, 60], gpu)
+    want = A.prompt_packed(q, k, v, cu, 0.1)[0].clone()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    got = A.prompt_packed(q, k, v, cu, 0.1, stream=s)[0]
+    s.synchronize()
+    assert torch.equal(got, want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = A.prompt_packed(q, k, v, cu, 0.1)[0]
+    cu.copy_(torch.tensor([0, 50, 90]))
+    g.replay()
+    assert torch.equal(o, A.prompt_packed(q, k, v, cu, 0.1)[0])
+    check(o, q, k, v, [50, 40], 0.1)
+
+
+def test_agrees_with_the_paged_prefill(gpu):
+    """The same prompt through bf16 pages and the paged prefill kernel: both within their bound of the same values."""
+    rng = np.random.default_rng(9)
+    n, nq, nkv = 150, 12, 1
+    q, k, v = rows(rng, n, nq, D).to(gpu), rows(rng, n, nkv, D).to(gpu), rows(rng, n, nkv, D).to(gpu)
+    out = A.prompt_packed(q, k, v, cu_of([n], gpu), 0.1)[0]
+    pages = -(-n // 16)
+    kc = torch.zeros(pages, 16, nkv, D, dtype=torch.bfloat16, device=gpu)
+    vc = torch.zeros_like(kc)
+    kc.view(-1, nkv, D)[:n], vc.view(-1, nkv, D)[:n] = k, v
+    pt = torch.arange(pages, dtype=torch.int32, device=gpu)[None].contiguous()
+    paged = A.paged_rows(q, kc, vc, pt, torch.zeros(n, dtype=torch.int32, device=gpu),
+                         torch.arange(1, n + 1, dtype=torch.int32, device=gpu), nq, nkv, 0.1, prefill_rows=n)[0]
+    ref, tol = R.attend(f64(q), f64(k), f64(v), np.arange(1, n + 1), 0.1)
+    assert (np.abs(f64(out) - ref) <= tol).all() and (np.abs(f64(paged) - ref) <= tol).all()

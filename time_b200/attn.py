@@ -1,7 +1,8 @@
 """ctypes front-end of the decode-attention entry points of libkernels.so
 (include/attn_block.h): partial RoPE + bf16 page write, split-context paged
-flash decode (with the e4m3 1x128 output the o_proj GEMM reads), and the
-fixed-order tensor-parallel sum of o_proj partials.
+flash decode (with the e4m3 1x128 output the o_proj GEMM reads), attention over
+whole packed prompts, and the fixed-order tensor-parallel sum of o_proj
+partials.
 
 The reference runs this path through launch_rope / launch_update_kv_cache /
 launch_paged_attention_decode (csrc/kernels.h, fp32, src/terra/engine.t:1269-1310);
@@ -9,8 +10,9 @@ those stay exported unchanged as drop-ins.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
-from ctypes import c_float, c_int, c_size_t, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_size_t, c_void_p
 
 import numpy as np
 
@@ -49,6 +51,9 @@ def lib():
                      c_int, c_void_p, c_void_p]
         k.attn_decode_paged_rows.argtypes = rows_args
         k.attn_paged_rows.argtypes = rows_args[:10] + [c_int] + rows_args[10:]
+        k.attn_prompt_packed.argtypes = [c_void_p, c_longlong, c_void_p, c_longlong, c_void_p, c_longlong, c_void_p,
+                                         c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p,
+                                         c_int, c_void_p, c_void_p]
         k.attn_tp_reduce_residual.argtypes = [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p]
         k.attn_block_create.argtypes = [ctypes.POINTER(BlockConfig), ctypes.POINTER(BlockWeights),
                                         ctypes.POINTER(c_void_p)]
@@ -152,6 +157,73 @@ def paged_rows(q, k_cache, v_cache, page_table, row_seq, seq_lens, nq: int, nkv:
     else:
         M.check("attn_paged_rows", k.attn_paged_rows(*head, prefill_rows, *tail))
     return out, out_q, out_s
+
+
+@contextlib.contextmanager
+def on_stream(t, stream=None):
+    """The handle of `stream` (None: the current one) with torch's allocations on it.  The tensor `t` must lie on the
+    current device: a launch goes to that one."""
+    import torch
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {t.device}, current device {torch.cuda.current_device()}")
+    if stream is None:
+        yield torch.cuda.current_stream().cuda_stream
+    else:
+        with torch.cuda.stream(stream):
+            yield stream.cuda_stream
+
+
+def check_i32(**tensors):
+    """Index tensors (or None): contiguous int32."""
+    for name, t in tensors.items():
+        if t is not None and (str(t.dtype) != "torch.int32" or not t.is_contiguous()):
+            raise ValueError(f"{name} is a contiguous int32 tensor")
+
+
+def check_rows(name, t, dtype, width):
+    if t.dim() != 2 or t.dtype != dtype or t.shape[1] != width or not t.is_contiguous():
+        raise ValueError(f"{name} is a contiguous {dtype} tensor [rows][{width}]")
+
+
+def check_heads(name, t, dtype):
+    """Rows of 128-dim heads, contiguous inside a row."""
+    if t.dim() != 3 or t.dtype != dtype or t.shape[2] != HEAD_DIM or t.stride(2) != 1 or \
+            (t.shape[1] > 1 and t.stride(1) != HEAD_DIM):
+        raise ValueError(f"{name} is a {dtype} tensor [rows][heads][{HEAD_DIM}], contiguous inside a row")
+
+
+def prompt_packed(q, k, v, cu_seqlens, scale: float, quant: bool = False, out=None, error_word=None, stream=None):
+    """attn_prompt_packed: causal attention over packed prompts, sequence s in rows [cu_seqlens[s], cu_seqlens[s + 1]).
+    q bf16 [T][nq][128], k and v [T][nkv][128]; rows may lie apart (v as a slice of the qkv projection's rows).
+    Rows in no sequence keep what `out` holds.  Returns (out bf16 [T][nq][128], out_q e4m3 [T][nq * 128] or None, out_s
+    [nq][ld] or None)."""
+    import torch
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        check_heads(name, t, torch.bfloat16)
+    check_i32(cu_seqlens=cu_seqlens)
+    T, nq = q.shape[:2]
+    nkv = k.shape[1]
+    if k.shape[0] != T or v.shape != k.shape:
+        raise ValueError("q, k and v have the same rows, k and v the same heads")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
+        raise ValueError("out is a contiguous tensor like q")
+    with on_stream(q, stream) as s:
+        out = torch.empty(T, nq, HEAD_DIM, dtype=q.dtype, device=q.device) if out is None else out
+        out_q = out_s = None
+        ld = (T + 3) // 4 * 4
+        if quant:
+            out_q = torch.empty(T, nq * HEAD_DIM, dtype=torch.uint8, device=q.device)
+            out_s = torch.empty(nq, ld, dtype=torch.float32, device=q.device)
+        M.check("attn_prompt_packed", lib().attn_prompt_packed(
+            q.data_ptr(), _row_stride(q), k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v),
+            cu_seqlens.data_ptr(), max(cu_seqlens.numel() - 1, 0), T, nq, nkv, HEAD_DIM, scale, out.data_ptr(),
+            M.ptr(out_q), M.ptr(out_s), ld, M.ptr(error_word), s))
+    return out, out_q, out_s
+
+
+def _row_stride(t) -> int:
+    """Elements between rows; a single row's stride does not matter."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * HEAD_DIM
 
 
 def tp_reduce_residual(partials, residual, stream=None):

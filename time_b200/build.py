@@ -8,8 +8,9 @@ Outputs (time_b200/lib/):
     libncclwrap.so    csrc/nccl_wrappers.cu                       (reference libncclwrap)
     libcublaswrap.so  csrc/cublas_wrappers.cu + csrc/moe_gemm.cu  (reference libcublaswrap + grouped GEMM)
     libkernels.so     csrc/kernels.cu + csrc/moe_prep.cu + csrc/moe_ep.cu + csrc/moe_layer.cu
-                      + csrc/attn.cu + csrc/attn_block.cu + csrc/gemm_small.cu + csrc/st_loader.cpp
-                      (reference libkernels + the MoE layer, the attention block and the
+                      + csrc/attn.cu + csrc/attn_prompt.cu + csrc/attn_kv4.cu + csrc/kv_pages.cu
+                      + csrc/attn_block.cu + csrc/gemm_small.cu + csrc/st_loader.cpp
+                      (reference libkernels + the MoE layer, attention and its caches, the
                       checkpoint loader; links the two above)
     engine.so         csrc/engine.cpp + csrc/engine_kernels.cu
                       (reference engine.so: the serving engine; links libkernels)
@@ -41,8 +42,8 @@ LIBS = {
     "libcudawrap.so": (["cuda_wrappers.cu"], ["-lcudart"], []),
     "libncclwrap.so": (["nccl_wrappers.cu"], ["-lcudart", "-lnccl"], []),
     "libcublaswrap.so": (["cublas_wrappers.cu", "moe_gemm.cu"], ["-lcudart", "-lcublas", "-lcublasLt"], []),
-    "libkernels.so": (["kernels.cu", "moe_prep.cu", "moe_ep.cu", "moe_layer.cu", "attn.cu", "attn_block.cu", "gemm_small.cu",
-                       "st_loader.cpp"], ["-lcudart"], ["libcublaswrap.so", "libncclwrap.so"]),
+    "libkernels.so": (["kernels.cu", "moe_prep.cu", "moe_ep.cu", "moe_layer.cu", "attn.cu", "attn_prompt.cu",
+                       "attn_kv4.cu", "kv_pages.cu", "attn_block.cu", "gemm_small.cu", "st_loader.cpp"], ["-lcudart"], ["libcublaswrap.so", "libncclwrap.so"]),
     "engine.so": (["engine.cpp", "engine_kernels.cu"], ["-lcudart", "-lcublas"],
                   ["libkernels.so", "libcublaswrap.so", "libncclwrap.so"]),
 }

@@ -29,33 +29,18 @@
 #include <cstdint>
 
 #include "attn_block.h"
+#include "attn_common.cuh"
 #include "sm100.cuh"
 
 namespace {
 
 using namespace tb;
 
-constexpr int kD = 128;            // head_dim (the kernels are specialised)
-constexpr int kPage = 16;          // tokens per KV page
 constexpr int kRowPad = kD + 8;    // bf16 elements per shared row (272 B: conflict-free ldmatrix)
 constexpr int kGPad = 16;          // query rows of one GQA group, padded to the MMA M
 constexpr int kWarps = 4;
 constexpr int kNst = 3;            // pages in flight per warp
-constexpr float kLog2e = 1.4426950408889634f;
-
-inline moe_status_t launch_status() {
-    return cudaGetLastError() == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
-}
-
 // ---------------------------------------------------------------- RoPE + page write
-
-// Page-table row of row b: row_seq[b] when the rows are tokens of several
-// sequences (prefill chunks, slot-indexed batches), else b; -1 when outside
-// [0, num_seqs).
-__device__ __forceinline__ int seq_of_row(const int32_t* row_seq, int b, int num_seqs) {
-    const int s = row_seq ? row_seq[b] : b;
-    return (s >= 0 && s < num_seqs) ? s : -1;
-}
 
 // One 64-thread block per (token, head): heads 0..nq-1 are queries, the next
 // nkv keys (both rotated on their first `rot` dims, pairs i, i + rot/2), the
@@ -105,28 +90,6 @@ rope_kv_write_kernel(const __nv_bfloat16* __restrict__ qkv, int nq, int nkv, int
             dst[i] = src[i];
         }
     }
-}
-
-// ---------------------------------------------------------------- mma.sync helpers
-
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
-}
-// D = A (16x16 bf16, row) * B (16x8 bf16, col) + D, fp32 accumulate
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
-                 "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
 }
 
 // ---------------------------------------------------------------- split decode
@@ -670,8 +633,6 @@ tp_reduce_kernel(const __nv_bfloat16* const* __restrict__ parts, int tp, const _
     for (int j = 0; j < 8; ++j) ob[j] = __float2bfloat16_rn(acc[j] + s[j]);
     *reinterpret_cast<uint4*>(out + i8) = ov;
 }
-
-inline bool a16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
 
 }  // namespace
 

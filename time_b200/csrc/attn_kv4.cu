@@ -1,0 +1,594 @@
+// attn_kv4.cu -- the 4-bit KV cache (include/kv_cache.h): partial RoPE with the
+// quantising page write, rows read back, and split-context decode attention.
+//
+// A value is n * s with n a 4-bit integer and s a bf16 number of four
+// significant bits, one per 32 dims.  Decode turns a code into it with one
+// lop3 and one bf16x2 fma: the code's nibble under the exponent of 128 is the
+// bf16 number 128 + (n + 8), and (136 + n) * s - 136 * s is exact -- 136 * s is
+// 17 * s with at most eight significant bits, n * s has at most eight -- so the
+// tensor cores see exactly the values held and nothing is rounded on the way.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+
+#include "attn_common.cuh"
+#include "kv_cache.h"
+#include "sm100.cuh"
+
+namespace {
+
+using namespace tb;
+
+constexpr int kGroups = kD / 32;                     // scales per token and head
+constexpr int kCodes = kPage * kD / 2;               // code bytes of one page and head
+constexpr int kPage4 = kCodes + kPage * kGroups * 2; // 1152
+constexpr int kGPad = 16;                            // query rows of one GQA group, padded to the MMA M
+
+// Byte offsets inside one (page, head) tile; see kv_cache.h.
+__host__ __device__ constexpr int k_code_byte(int t, int d) {
+    return t * 64 + (d % 32) / 8 * 16 + d / 32 * 4 + d % 8 / 2;
+}
+__host__ __device__ constexpr int v_code_byte(int t, int d) {
+    return t / 8 * 512 + (4 * (d % 32 / 4) + t % 8 / 2) * 16 + t % 2 * 8 + d / 32 * 2 + d % 4 / 2;
+}
+
+// ---------------------------------------------------------------- write
+
+constexpr int kWriteWarps = 8;
+
+// Scale of a group whose largest |x| has the bits `amax`, and 0 for a group
+// that is stored as NaN.
+__device__ __forceinline__ float group_scale(uint32_t amax) {
+    if (amax >= ((127u + 120u) << 23)) return 0.0f;
+    const uint32_t b = __float_as_uint(__fdiv_rn(__uint_as_float(amax), 7.5f));
+    return fmaxf(__uint_as_float((b + 0x000FFFFFu) & ~0x000FFFFFu), 1.17549435e-38f);
+}
+
+// One block per (row, share of the heads), one warp per head; lane l holds dims
+// 4l .. 4l+3, so a group of 32 dims is eight lanes.  The kernel is bound by the
+// rows in and the q rows out.
+__global__ void __launch_bounds__(kWriteWarps * 32)
+kv4_rope_write_kernel(const __nv_bfloat16* __restrict__ qkv, int nq, int nkv, int rot,
+                      const float* __restrict__ inv_freq, const int32_t* __restrict__ positions,
+                      const int32_t* __restrict__ row_seq, int num_seqs, const int32_t* __restrict__ page_table,
+                      int max_pages, int num_cache_pages, __nv_bfloat16* __restrict__ q_out,
+                      __nv_bfloat16* __restrict__ k_out, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
+                      int32_t* __restrict__ seq_lens_out, int* __restrict__ error_word) {
+    __shared__ float cs_s[kD / 2], sn_s[kD / 2];
+    const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool first = blockIdx.y == 0 && threadIdx.x == 0;
+    const int pos = positions[b];
+    const int seq = seq_of_row(row_seq, b, num_seqs);
+    if (first && seq_lens_out) seq_lens_out[b] = (pos >= 0 && seq >= 0) ? pos + 1 : 0;
+    if (seq < 0) {
+        if (first && error_word) atomicExch(error_word, 7);
+        return;
+    }
+    if (pos < 0 || pos / kPage >= max_pages) {
+        if (first && error_word) atomicExch(error_word, 4);
+        return;
+    }
+    const int phys = page_table[static_cast<size_t>(seq) * max_pages + pos / kPage];
+    if (phys < 0 || phys >= num_cache_pages) {
+        if (first && error_word) atomicExch(error_word, 6);
+        return;
+    }
+    const int half = rot / 2;
+    for (int i = threadIdx.x; i < half; i += blockDim.x) {
+        // the angle is the fp32 product, as in the bf16 page write
+        sincosf(static_cast<float>(pos) * inv_freq[i], &sn_s[i], &cs_s[i]);
+    }
+    __syncthreads();
+    const int t = pos % kPage;
+    const int heads = nq + 2 * nkv;
+    for (int h = blockIdx.y * kWriteWarps + warp; h < heads; h += gridDim.y * kWriteWarps) {
+        const __nv_bfloat16* src = qkv + (static_cast<size_t>(b) * heads + h) * kD;
+        const uint2 own = *reinterpret_cast<const uint2*>(src + 4 * lane);
+        const __nv_bfloat16* ob = reinterpret_cast<const __nv_bfloat16*>(&own);
+        __nv_bfloat16 x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int d = 4 * lane + e;
+            x[e] = ob[e];
+            if (h < nq + nkv && d < rot) {
+                const bool lo = d < half;
+                const int i = lo ? d : d - half;
+                const float a = __bfloat162float(lo ? ob[e] : src[i]);
+                const float c = __bfloat162float(lo ? src[i + half] : ob[e]);
+                // products rounded before the sum: one result whatever the compiler contracts
+                x[e] = __float2bfloat16_rn(lo ? __fsub_rn(__fmul_rn(a, cs_s[i]), __fmul_rn(c, sn_s[i]))
+                                              : __fadd_rn(__fmul_rn(a, sn_s[i]), __fmul_rn(c, cs_s[i])));
+            }
+        }
+        const uint2 xv = *reinterpret_cast<const uint2*>(x);
+        if (h < nq) {
+            *reinterpret_cast<uint2*>(q_out + (static_cast<size_t>(b) * nq + h) * kD + 4 * lane) = xv;
+            continue;
+        }
+        const bool is_k = h < nq + nkv;
+        const int kvh = is_k ? h - nq : h - nq - nkv;
+        if (is_k && k_out) *reinterpret_cast<uint2*>(k_out + (static_cast<size_t>(b) * nkv + kvh) * kD + 4 * lane) = xv;
+        uint32_t amax = 0;   // as bits: a NaN is above every number
+#pragma unroll
+        for (int e = 0; e < 4; ++e) amax = max(amax, __float_as_uint(__bfloat162float(x[e])) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        const float s = group_scale(amax);
+        uint32_t codes = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float n = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(__bfloat162float(x[e]), s)), -8.0f), 7.0f) : 0.0f;
+            codes |= static_cast<uint32_t>(static_cast<int>(n) + 8) << (4 * e);
+        }
+        uint8_t* page = (is_k ? k_cache : v_cache) + (static_cast<size_t>(phys) * nkv + kvh) * kPage4;
+        *reinterpret_cast<uint16_t*>(page + (is_k ? k_code_byte(t, 4 * lane) : v_code_byte(t, 4 * lane))) =
+            static_cast<uint16_t>(codes);
+        if ((lane & 7) == 0)
+            *reinterpret_cast<uint16_t*>(page + kCodes + (t * kGroups + lane / 8) * 2) =
+                s > 0.0f ? static_cast<uint16_t>(__float_as_uint(s) >> 16) : static_cast<uint16_t>(0x7FC0);   // s is a bf16 number
+    }
+}
+
+// ---------------------------------------------------------------- read
+
+constexpr int kReadWarps = 8;
+
+// One warp per (row, kv head, K or V).
+__global__ void __launch_bounds__(kReadWarps * 32)
+kv4_read_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, int num_cache_pages,
+                const int32_t* __restrict__ positions, const int32_t* __restrict__ row_seq, int num_seqs,
+                const int32_t* __restrict__ page_table, int max_pages, int B, int nkv,
+                __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ error_word) {
+    const long long w = static_cast<long long>(blockIdx.x) * kReadWarps + (threadIdx.x >> 5);
+    if (w >= 2ll * B * nkv) return;
+    const int lane = threadIdx.x & 31;
+    const bool is_k = w % 2 == 0;
+    const int kvh = static_cast<int>(w / 2 % nkv), b = static_cast<int>(w / 2 / nkv);
+    __nv_bfloat16* out = is_k ? k_out : v_out;
+    if (!out) return;
+    const int pos = positions[b];
+    const int seq = seq_of_row(row_seq, b, num_seqs);
+    int phys = -1, err = 0;
+    if (seq < 0) err = 7;
+    else if (pos < 0 || pos / kPage >= max_pages) err = 4;
+    else {
+        phys = page_table[static_cast<size_t>(seq) * max_pages + pos / kPage];
+        if (phys < 0 || phys >= num_cache_pages) err = 6;
+    }
+    if (err && lane == 0 && error_word) atomicExch(error_word, err);
+    __nv_bfloat16 x[4];
+    if (err) {
+        for (int e = 0; e < 4; ++e) x[e] = __float2bfloat16_rn(0.0f);
+    } else {
+        const int t = pos % kPage;
+        const uint8_t* page = (is_k ? k_cache : v_cache) + (static_cast<size_t>(phys) * nkv + kvh) * kPage4;
+        const uint32_t codes = *reinterpret_cast<const uint16_t*>(page + (is_k ? k_code_byte(t, 4 * lane) : v_code_byte(t, 4 * lane)));
+        const float s = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(page + kCodes + (t * kGroups + lane / 8) * 2));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            x[e] = __float2bfloat16_rn(static_cast<float>(static_cast<int>((codes >> (4 * e)) & 15u) - 8) * s);
+    }
+    *reinterpret_cast<uint2*>(out + (static_cast<size_t>(b) * nkv + kvh) * kD + 4 * lane) = *reinterpret_cast<const uint2*>(x);
+}
+
+// ---------------------------------------------------------------- decode
+
+constexpr int kWarps = 4;
+constexpr int kNst = 4;                                   // pages in flight per warp
+constexpr int kStage = 2 * kPage4;                        // K and V tile of one page
+constexpr int kMaxSplitPages = 512;                       // split_tokens <= 8192
+constexpr int kMergePad = kD + 4;
+constexpr size_t kRingBytes = static_cast<size_t>(kWarps) * kNst * kStage;
+constexpr size_t kDecodeSmem = kRingBytes + kMaxSplitPages * 4;
+// the warp merge reuses the rings: per warp 16 x 128 fp32 and 16 (m, l)
+static_assert(static_cast<size_t>(kWarps) * kGPad * (kMergePad + 2) * 4 <= kRingBytes, "merge scratch fits the rings");
+
+struct Kv4Params {
+    const __nv_bfloat16* q;
+    const uint8_t* k_cache;
+    const uint8_t* v_cache;
+    const int32_t* page_table;
+    const int32_t* row_seq;
+    const int32_t* seq_lens;
+    float* part_o;                 // [B * nkv][max_splits][G][128]
+    float* part_ml;                // [B * nkv][max_splits][G][2]
+    int* error_word;
+    int nq, nkv, G, max_pages, num_cache_pages, split_tokens, max_splits, num_seqs;
+    float scale_log2;
+};
+
+__device__ __forceinline__ int clamp_len(int len, int max_pages, int split_tokens, int max_splits) {
+    const long long cap = min(static_cast<long long>(max_pages) * kPage, static_cast<long long>(max_splits) * split_tokens);
+    return len < 0 ? 0 : (len > cap ? static_cast<int>(cap) : len);
+}
+
+__device__ __forceinline__ uint32_t bf2_fma(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+    return d;
+}
+__device__ __forceinline__ uint32_t bf2_mul(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+constexpr uint32_t kMinus136 = 0xC308C308u;   // bf16x2
+
+// The codes at nibble i of both halves of w as the bf16 pair 136 + n.
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {
+    return ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+}
+
+__global__ void __launch_bounds__(kWarps * 32, 3)
+kv4_decode_kernel(const Kv4Params p) {
+    extern __shared__ __align__(128) uint8_t sm[];
+    const int split = blockIdx.x;
+    const int bk = blockIdx.y;
+    const int b = bk / p.nkv, kvh = bk % p.nkv;
+    const int seq = seq_of_row(p.row_seq, b, p.num_seqs);
+    if (seq < 0) {
+        if (split == 0 && threadIdx.x == 0 && kvh == 0 && p.error_word) atomicExch(p.error_word, 7);
+        return;
+    }
+    const int len_in = p.seq_lens[b];
+    const int len = clamp_len(len_in, p.max_pages, p.split_tokens, p.max_splits);
+    if (len < len_in && split == 0 && threadIdx.x == 0 && kvh == 0 && p.error_word) atomicExch(p.error_word, 5);
+    const int t0 = split * p.split_tokens;
+    if (t0 >= len) return;
+    const int t1 = min(t0 + p.split_tokens, len);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, tq = lane & 3;
+
+    uint8_t* ring = sm + static_cast<size_t>(warp) * kNst * kStage;
+    int* pid_s = reinterpret_cast<int*>(sm + kRingBytes);
+    const int page0 = t0 / kPage;
+    const int npages = (t1 - 1) / kPage - page0 + 1;
+    {
+        const int32_t* ptb = p.page_table + static_cast<size_t>(seq) * p.max_pages + page0;
+        for (int i = threadIdx.x; i < npages; i += blockDim.x) {
+            const int phys = ptb[i];
+            const bool ok = phys >= 0 && phys < p.num_cache_pages;
+            if (!ok && p.error_word) atomicExch(p.error_word, 6);
+            pid_s[i] = ok ? phys : -1;
+        }
+    }
+    // Query fragments: MMA k-step 2j + u takes dims 32 j + 8 tq + {2u, 2u + 4, 2u + 1, 2u + 5} at this lane's
+    // four contraction indices, the order the K codes unpack in.
+    uint32_t qa[kD / 16][4];
+    {
+        const __nv_bfloat16* q0 = p.q + (static_cast<size_t>(b) * p.nq + kvh * p.G) * kD;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = g + 8 * h;
+#pragma unroll
+            for (int j = 0; j < kGroups; ++j) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (r < p.G) v = *reinterpret_cast<const uint4*>(q0 + static_cast<size_t>(r) * kD + 32 * j + 8 * tq);
+                // v: dims 0 1 | 2 3 | 4 5 | 6 7
+                qa[2 * j][h] = __byte_perm(v.x, v.z, 0x5410);          // 0, 4
+                qa[2 * j][2 + h] = __byte_perm(v.x, v.z, 0x7632);      // 1, 5
+                qa[2 * j + 1][h] = __byte_perm(v.y, v.w, 0x5410);      // 2, 6
+                qa[2 * j + 1][2 + h] = __byte_perm(v.y, v.w, 0x7632);  // 3, 7
+            }
+        }
+    }
+    __syncthreads();
+
+    const int my_pages = npages > warp ? (npages - warp + kWarps - 1) / kWarps : 0;
+    auto load_page = [&](int i, int stage) {
+        int phys = pid_s[warp + i * kWarps];
+        const uint32_t nbytes = phys >= 0 ? 16u : 0u;     // a bad page reads as zero scales: zeros
+        phys = phys >= 0 ? phys : 0;
+        const size_t off = (static_cast<size_t>(phys) * p.nkv + kvh) * kPage4;
+        uint8_t* dst = ring + stage * kStage;
+        for (int c = lane; c < kStage / 16; c += 32) {
+            const uint8_t* src = c < kPage4 / 16 ? p.k_cache + off + c * 16 : p.v_cache + off + (c * 16 - kPage4);
+            cp_async16(dst + c * 16, src, nbytes);
+        }
+    };
+
+    float o[kD / 8][4];
+#pragma unroll
+    for (int i = 0; i < kD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+    float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.0f, 0.0f};
+
+#pragma unroll
+    for (int s = 0; s < kNst - 1; ++s) {
+        if (s < my_pages) load_page(s, s);
+        cp_async_commit();
+    }
+    for (int i = 0; i < my_pages; ++i) {
+        cp_async_wait<kNst - 2>();
+        __syncwarp();
+        if (i + kNst - 1 < my_pages) load_page(i + kNst - 1, (i + kNst - 1) % kNst);
+        cp_async_commit();
+        const uint8_t* kt = ring + (i % kNst) * kStage;
+        const uint8_t* vt = kt + kPage4;
+        const int tok = (page0 + warp + i * kWarps) * kPage;
+        const int valid = t1 - tok;                        // tokens of this page inside the split, at least 1
+        // S = Q K^T, two tiles of eight tokens
+        float sv[2][4];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint4 cw = *reinterpret_cast<const uint4*>(kt + (g + 8 * n) * 64 + tq * 16);
+            const uint2 sw = *reinterpret_cast<const uint2*>(kt + kCodes + (g + 8 * n) * 8);
+            const uint32_t w[4] = {cw.x, cw.y, cw.z, cw.w};
+#pragma unroll
+            for (int j = 0; j < kGroups; ++j) {
+                const uint32_t s2 = __byte_perm(j < 2 ? sw.x : sw.y, 0, (j & 1) ? 0x3232 : 0x1010);
+                const uint32_t c2 = bf2_mul(s2, kMinus136);
+                uint32_t v[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[u] = bf2_fma(code_pair(w[j], u), s2, c2);
+                mma_bf16(s, qa[2 * j], v[0], v[1]);
+                mma_bf16(s, qa[2 * j + 1], v[2], v[3]);
+            }
+            sv[0][2 * n] = s[0]; sv[0][2 * n + 1] = s[1];
+            sv[1][2 * n] = s[2]; sv[1][2 * n + 1] = s[3];
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int t = 2 * tq + (j & 1) + 8 * (j >> 1);
+                sv[h][j] = t < valid ? sv[h][j] * p.scale_log2 : -INFINITY;
+            }
+        float alpha[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float mx = fmaxf(fmaxf(sv[h][0], sv[h][1]), fmaxf(sv[h][2], sv[h][3]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float mn = fmaxf(m_r[h], mx);
+            const float ms = mn == -INFINITY ? 0.0f : mn;   // every score -inf so far: weights 0, not NaN
+            alpha[h] = exp2f(m_r[h] - ms);
+            m_r[h] = mn;
+            float rs = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                sv[h][j] = exp2f(sv[h][j] - ms);
+                rs += sv[h][j];
+            }
+            l_r[h] = l_r[h] * alpha[h] + rs;
+        }
+        if (alpha[0] != 1.0f || alpha[1] != 1.0f) {
+#pragma unroll
+            for (int nd = 0; nd < kD / 8; ++nd) {
+                o[nd][0] *= alpha[0]; o[nd][1] *= alpha[0];
+                o[nd][2] *= alpha[1]; o[nd][3] *= alpha[1];
+            }
+        }
+        // O += P V.  P is rounded to bf16, as the bf16 pages' decode rounds it (2^-9 of each weight).
+        uint32_t pa[4];
+        pa[0] = pack_bf16(sv[0][0], sv[0][1]);
+        pa[1] = pack_bf16(sv[1][0], sv[1][1]);
+        pa[2] = pack_bf16(sv[0][2], sv[0][3]);
+        pa[3] = pack_bf16(sv[1][2], sv[1][3]);
+        // codes and scales of tokens 2 tq, 2 tq + 1 (half a = 0) and 8 more (a = 1)
+        uint4 vc[2], vs[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            vc[a] = *reinterpret_cast<const uint4*>(vt + a * 512 + lane * 16);
+            vs[a] = *reinterpret_cast<const uint4*>(vt + kCodes + (8 * a + 2 * tq) * 8);
+            // a slot past the end may hold anything: weight 0 times value 0
+            if (8 * a + 2 * tq >= valid) vs[a].x = vs[a].y = 0;
+            if (8 * a + 2 * tq + 1 >= valid) vs[a].z = vs[a].w = 0;
+        }
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j) {
+            uint32_t w[2], s2[2], c2[2];
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const uint32_t sel = (j & 1) ? 0x7632 : 0x5410;
+                w[a] = __byte_perm(j < 2 ? vc[a].x : vc[a].y, j < 2 ? vc[a].z : vc[a].w, sel);
+                s2[a] = __byte_perm(j < 2 ? vs[a].x : vs[a].y, j < 2 ? vs[a].z : vs[a].w, sel);
+                c2[a] = bf2_mul(s2[a], kMinus136);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                mma_bf16(o[4 * j + u], pa, bf2_fma(code_pair(w[0], u), s2[0], c2[0]),
+                         bf2_fma(code_pair(w[1], u), s2[1], c2[1]));
+        }
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l_r[h] += __shfl_xor_sync(0xffffffffu, l_r[h], 1);
+        l_r[h] += __shfl_xor_sync(0xffffffffu, l_r[h], 2);
+    }
+    __syncthreads();   // every warp is done with its ring: reuse as merge scratch
+    float* mo = reinterpret_cast<float*>(sm);                       // [warp][16][kMergePad]
+    float* mml = mo + kWarps * kGPad * kMergePad;                   // [warp][16][2]
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = g + 8 * h;
+        float* ow = mo + (warp * kGPad + r) * kMergePad;
+        // output tile 4 j + u, column c is dim 32 j + 4 c + u
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                *reinterpret_cast<float4*>(ow + 32 * j + 8 * tq + 4 * e) =
+                    make_float4(o[4 * j][2 * h + e], o[4 * j + 1][2 * h + e], o[4 * j + 2][2 * h + e], o[4 * j + 3][2 * h + e]);
+        if (tq == 0) {
+            mml[(warp * kGPad + r) * 2 + 0] = m_r[h];
+            mml[(warp * kGPad + r) * 2 + 1] = l_r[h];
+        }
+    }
+    __syncthreads();
+    const size_t base = (static_cast<size_t>(bk) * p.max_splits + split) * p.G;
+    for (int r = 0; r < p.G; ++r) {
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, mml[(w * kGPad + r) * 2]);
+        float L = 0.0f, acc = 0.0f;
+        const int d = threadIdx.x;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float mw = mml[(w * kGPad + r) * 2];
+            const float lw = mml[(w * kGPad + r) * 2 + 1];
+            const float f = (mw == -INFINITY) ? 1.0f : exp2f(mw - M);   // no weight yet: l and o are 0 or NaN
+            L += lw * f;
+            acc += mo[(w * kGPad + r) * kMergePad + d] * f;
+        }
+        p.part_o[(base + r) * kD + d] = acc;
+        if (d == 0) {
+            p.part_ml[(base + r) * 2 + 0] = M;
+            p.part_ml[(base + r) * 2 + 1] = L;
+        }
+    }
+}
+
+// One block (128 threads = head_dim) per (row, query head): merges the splits.
+__global__ void __launch_bounds__(kD)
+kv4_merge_kernel(const Kv4Params p, __nv_bfloat16* __restrict__ out, uint8_t* __restrict__ out_q,
+                 float* __restrict__ out_s, int out_ld) {
+    const int b = blockIdx.x / p.nq, h = blockIdx.x % p.nq;
+    const int kvh = h / p.G, r = h % p.G;
+    const int d = threadIdx.x;
+    const int len = seq_of_row(p.row_seq, b, p.num_seqs) < 0
+                        ? 0 : clamp_len(p.seq_lens[b], p.max_pages, p.split_tokens, p.max_splits);
+    const int ns = (len + p.split_tokens - 1) / p.split_tokens;
+    const size_t base = (static_cast<size_t>(b) * p.nkv + kvh) * p.max_splits * p.G + r;
+    float M = -INFINITY;
+    for (int s = 0; s < ns; ++s) M = fmaxf(M, p.part_ml[(base + static_cast<size_t>(s) * p.G) * 2]);
+    float L = 0.0f, acc = 0.0f;
+    for (int s = 0; s < ns; ++s) {
+        const size_t i = base + static_cast<size_t>(s) * p.G;
+        const float ms = p.part_ml[i * 2];
+        const float f = ms == -INFINITY ? 1.0f : exp2f(ms - M);
+        L += p.part_ml[i * 2 + 1] * f;
+        acc += p.part_o[i * kD + d] * f;
+    }
+    const float v = ns > 0 ? acc / L : 0.0f;
+    out[(static_cast<size_t>(b) * p.nq + h) * kD + d] = __float2bfloat16_rn(v);
+    if (out_q) {
+        __shared__ float red[kD / 32];
+        float a = fabsf(v);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        if ((d & 31) == 0) red[d >> 5] = a;
+        __syncthreads();
+        const float amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        uint8_t qv = 0;
+        if (amax > 0.0f) qv = static_cast<uint8_t>(cvt_e4m3x2(v * (448.0f / amax), 0.0f) & 0xFFu);
+        out_q[(static_cast<size_t>(b) * p.nq + h) * kD + d] = qv;
+        if (d == 0) out_s[static_cast<size_t>(h) * out_ld + b] = amax > 0.0f ? amax / 448.0f : 0.0f;
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t attn_kv4_page_bytes(int nkv) { return nkv > 0 ? static_cast<size_t>(nkv) * kPage4 : 0; }
+
+moe_status_t attn_kv4_rope_write_rows(const void* qkv_bf16, int B, int nq, int nkv, int head_dim, int rot,
+                                      const float* inv_freq, const int32_t* positions, const int32_t* row_seq,
+                                      int num_seqs, const int32_t* page_table, int max_pages, int page_size,
+                                      int num_cache_pages, void* q_out_bf16, void* k_out_bf16, void* k_cache,
+                                      void* v_cache, int32_t* seq_lens_out, int* error_word, cwStream_t stream) {
+    if (B < 0 || nq <= 0 || nkv <= 0 || nq % nkv || head_dim != kD || page_size != kPage) return MOE_ERR_INVALID_ARGUMENT;
+    if (num_cache_pages <= 0 || num_seqs <= 0) return MOE_ERR_INVALID_ARGUMENT;
+    if (rot < 0 || rot > kD || rot % 2 || max_pages <= 0) return MOE_ERR_INVALID_ARGUMENT;
+    if (B == 0) return MOE_OK;
+    if (!qkv_bf16 || (rot > 0 && !inv_freq) || !positions || !page_table || !q_out_bf16 || !k_cache || !v_cache)
+        return MOE_ERR_INVALID_ARGUMENT;
+    if (!a16(qkv_bf16) || !a16(q_out_bf16) || !a16(k_out_bf16) || !a16(k_cache) || !a16(v_cache))
+        return MOE_ERR_INVALID_ARGUMENT;
+    const int groups = (nq + 2 * nkv + kWriteWarps - 1) / kWriteWarps;
+    kv4_rope_write_kernel<<<dim3(B, groups < 65535 ? groups : 65535), kWriteWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const __nv_bfloat16*>(qkv_bf16), nq, nkv, rot, inv_freq, positions, row_seq, num_seqs, page_table,
+        max_pages, num_cache_pages, static_cast<__nv_bfloat16*>(q_out_bf16), static_cast<__nv_bfloat16*>(k_out_bf16),
+        static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(v_cache), seq_lens_out, error_word);
+    return launch_status();
+}
+
+moe_status_t attn_kv4_read_rows(const void* k_cache, const void* v_cache, int num_cache_pages,
+                                const int32_t* positions, const int32_t* row_seq, int num_seqs,
+                                const int32_t* page_table, int max_pages, int page_size, int B, int nkv, int head_dim,
+                                void* k_out_bf16, void* v_out_bf16, int* error_word, cwStream_t stream) {
+    if (B < 0 || nkv <= 0 || head_dim != kD || page_size != kPage || num_cache_pages <= 0 || num_seqs <= 0 ||
+        max_pages <= 0)
+        return MOE_ERR_INVALID_ARGUMENT;
+    if (B == 0 || (!k_out_bf16 && !v_out_bf16)) return MOE_OK;
+    if (!positions || !page_table || (k_out_bf16 && !k_cache) || (v_out_bf16 && !v_cache)) return MOE_ERR_INVALID_ARGUMENT;
+    if (!a16(k_cache) || !a16(v_cache) || !a16(k_out_bf16) || !a16(v_out_bf16)) return MOE_ERR_INVALID_ARGUMENT;
+    const long long blocks = (2ll * B * nkv + kReadWarps - 1) / kReadWarps;
+    if (blocks > 0x7FFFFFFF) return MOE_ERR_UNSUPPORTED;
+    kv4_read_kernel<<<static_cast<int>(blocks), kReadWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const uint8_t*>(k_cache), static_cast<const uint8_t*>(v_cache), num_cache_pages, positions, row_seq,
+        num_seqs, page_table, max_pages, B, nkv, static_cast<__nv_bfloat16*>(k_out_bf16),
+        static_cast<__nv_bfloat16*>(v_out_bf16), error_word);
+    return launch_status();
+}
+
+int attn_kv4_split_tokens(int B, int nkv, int max_context) {
+    if (B <= 0 || nkv <= 0 || max_context <= 0) return kPage;
+    // about two waves of three CTAs per SM at half the longest context, at least a page per warp
+    const long long rows = static_cast<long long>(B) * nkv;
+    const long long want = (2 * 444 + rows - 1) / rows;
+    long long split = (max_context / 2 + want - 1) / want;
+    split = (split + kPage - 1) / kPage * kPage;
+    const long long low = kWarps * kPage, high = kMaxSplitPages * kPage;
+    return static_cast<int>(split < low ? low : split > high ? high : split);
+}
+
+size_t attn_kv4_decode_workspace_bytes(int B, int nq, int max_splits) {
+    if (B <= 0 || nq <= 0 || max_splits <= 0) return 0;
+    return static_cast<size_t>(B) * nq * max_splits * (kD + 2) * sizeof(float);
+}
+
+moe_status_t attn_kv4_decode_rows(const void* q_bf16, const void* k_cache, const void* v_cache, int num_cache_pages,
+                                  const int32_t* page_table, int max_pages, const int32_t* row_seq, int num_seqs,
+                                  const int32_t* seq_lens, int B, int nq, int nkv, int head_dim, int page_size,
+                                  float scale, int split_tokens, int max_splits, void* workspace,
+                                  size_t workspace_bytes, void* out_bf16, void* out_q, float* out_s, int out_ld,
+                                  int* error_word, cwStream_t stream) {
+    if (B < 0 || num_seqs <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || nq / nkv > kGPad || head_dim != kD ||
+        page_size != kPage)
+        return MOE_ERR_INVALID_ARGUMENT;
+    if (split_tokens <= 0 || split_tokens % kPage || split_tokens > kMaxSplitPages * kPage || max_splits <= 0 ||
+        max_pages <= 0 || num_cache_pages <= 0)
+        return MOE_ERR_INVALID_ARGUMENT;
+    if (static_cast<long long>(B) * nkv > 65535 || static_cast<long long>(B) * nq > 0x7FFFFFFF) return MOE_ERR_UNSUPPORTED;
+    if (B == 0) return MOE_OK;
+    if (!q_bf16 || !k_cache || !v_cache || !page_table || !seq_lens || !workspace || !out_bf16)
+        return MOE_ERR_INVALID_ARGUMENT;
+    if (!a16(q_bf16) || !a16(k_cache) || !a16(v_cache) || !a16(workspace)) return MOE_ERR_INVALID_ARGUMENT;
+    if (out_q && (!out_s || out_ld < B)) return MOE_ERR_INVALID_ARGUMENT;
+    if (workspace_bytes < attn_kv4_decode_workspace_bytes(B, nq, max_splits)) return MOE_ERR_WORKSPACE;
+    static bool attr[kMaxDevices] = {};
+    if (smem_optin_once(kv4_decode_kernel, static_cast<int>(kDecodeSmem), attr) != cudaSuccess) return MOE_ERR_CUDA;
+    Kv4Params p;
+    p.q = static_cast<const __nv_bfloat16*>(q_bf16);
+    p.k_cache = static_cast<const uint8_t*>(k_cache);
+    p.v_cache = static_cast<const uint8_t*>(v_cache);
+    p.page_table = page_table;
+    p.row_seq = row_seq;
+    p.seq_lens = seq_lens;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = p.part_o + static_cast<size_t>(B) * nq * max_splits * kD;
+    p.error_word = error_word;
+    p.nq = nq;
+    p.nkv = nkv;
+    p.G = nq / nkv;
+    p.max_pages = max_pages;
+    p.num_cache_pages = num_cache_pages;
+    p.split_tokens = split_tokens;
+    p.max_splits = max_splits;
+    p.num_seqs = num_seqs;
+    p.scale_log2 = scale * kLog2e;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    kv4_decode_kernel<<<dim3(max_splits, B * nkv), kWarps * 32, kDecodeSmem, st>>>(p);
+    moe_status_t s = launch_status();
+    if (s != MOE_OK) return s;
+    kv4_merge_kernel<<<B * nq, kD, 0, st>>>(p, static_cast<__nv_bfloat16*>(out_bf16), static_cast<uint8_t*>(out_q), out_s,
+                                           out_ld);
+    return launch_status();
+}
+
+}  // extern "C"

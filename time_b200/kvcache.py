@@ -1,0 +1,211 @@
+"""ctypes front-end of include/kv_cache.h: the 4-bit KV cache (RoPE and
+quantising page write, rows read back, split decode attention) and the page
+operators (fork, free and extend rows; compact a pool).
+
+The 4-bit caches stand beside the bf16 pages of :mod:`time_b200.attn` and take
+the same page tables; the page operators work on the pages of either, all
+layers' K and V in one tensor ``[caches][pages][...]``.  A sequence of ``len``
+tokens owns the first ``ceil(len / 16)`` entries of its page-table row and a
+page in no row is free, so a request is freed by leaving its row out of the
+next fork.
+"""
+from __future__ import annotations
+
+from ctypes import c_float, c_int, c_size_t, c_void_p
+
+from . import attn as A
+from . import moe as M
+
+HEAD_DIM, PAGE, GROUP = A.HEAD_DIM, A.PAGE, 32
+CODE_BYTES = PAGE * HEAD_DIM // 2
+PAGE4_BYTES = CODE_BYTES + PAGE * (HEAD_DIM // GROUP) * 2      # one page of one kv head
+
+_bound = False
+
+
+def lib():
+    global _bound
+    k = M.libs()["libkernels.so"]
+    if not _bound:
+        k.attn_kv4_page_bytes.argtypes = [c_int]
+        k.attn_kv4_page_bytes.restype = c_size_t
+        k.attn_kv4_rope_write_rows.argtypes = [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
+                                               c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p,
+                                               c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+        k.attn_kv4_read_rows.argtypes = [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int,
+                                         c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]
+        k.attn_kv4_split_tokens.argtypes = [c_int, c_int, c_int]
+        k.attn_kv4_decode_workspace_bytes.argtypes = [c_int, c_int, c_int]
+        k.attn_kv4_decode_workspace_bytes.restype = c_size_t
+        k.attn_kv4_decode_rows.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int,
+                                           c_void_p, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int,
+                                           c_void_p, c_size_t, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p]
+        k.kv_pages_workspace_bytes.argtypes = [c_int, c_int]
+        k.kv_pages_workspace_bytes.restype = c_size_t
+        k.kv_pages_fork.argtypes = [c_void_p, c_size_t, c_int, c_int, c_size_t, c_int, c_void_p, c_int, c_void_p,
+                                    c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p,
+                                    c_void_p]
+        k.kv_pages_compact.argtypes = [c_void_p, c_size_t, c_int, c_int, c_size_t, c_int, c_void_p, c_int, c_void_p,
+                                       c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]
+        _bound = True
+    return k
+
+
+def kv4_cache(num_pages: int, nkv: int, device):
+    """An empty 4-bit K or V cache, uint8 [pages][nkv][1152]."""
+    import torch
+    return torch.zeros(num_pages, nkv, PAGE4_BYTES, dtype=torch.uint8, device=device)
+
+
+def _check_kv4(k_cache, v_cache):
+    for c in (k_cache, v_cache):
+        if c.dim() != 3 or c.shape[2] != PAGE4_BYTES or c.element_size() != 1 or not c.is_contiguous():
+            raise ValueError(f"a 4-bit cache is a contiguous uint8 tensor [pages][nkv][{PAGE4_BYTES}]")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache differ in shape")
+    return k_cache.shape[0], k_cache.shape[1]
+
+
+def kv4_rope_write(qkv, positions, row_seq, page_table, k_cache, v_cache, nq: int, rot: int, inv_freq,
+                   keys: bool = False, seq_lens_out=None, error_word=None, stream=None):
+    """attn_kv4_rope_write_rows: qkv bf16 [B][(nq + 2 nkv) * 128] -> (rotated q bf16 [B][nq][128], with `keys` the
+    rotated keys bf16 [B][nkv][128] before quantisation, else None); k and v into their page slots.  row_seq None:
+    row b uses page-table row b."""
+    import torch
+    pages, nkv = _check_kv4(k_cache, v_cache)
+    A.check_rows("qkv", qkv, torch.bfloat16, (nq + 2 * nkv) * HEAD_DIM)
+    A.check_i32(positions=positions, row_seq=row_seq, page_table=page_table, seq_lens_out=seq_lens_out)
+    B = qkv.shape[0]
+    if positions.numel() != B or (B if row_seq is None else row_seq.numel()) != B:
+        raise ValueError("positions and row_seq have one entry per row")
+    if inv_freq is not None and inv_freq.numel() < rot // 2:
+        raise ValueError("inv_freq has rot / 2 entries")
+    if row_seq is None and page_table.shape[0] < B:
+        raise ValueError("the page table has a row per row of qkv when row_seq is None")
+    with A.on_stream(qkv, stream) as s:
+        q = torch.empty(B, nq, HEAD_DIM, dtype=torch.bfloat16, device=qkv.device)
+        k = torch.empty(B, nkv, HEAD_DIM, dtype=torch.bfloat16, device=qkv.device) if keys else None
+        M.check("attn_kv4_rope_write_rows", lib().attn_kv4_rope_write_rows(
+            M.ptr(qkv), B, nq, nkv, HEAD_DIM, rot, M.ptr(inv_freq), M.ptr(positions), M.ptr(row_seq),
+            page_table.shape[0], M.ptr(page_table), page_table.shape[1], PAGE, pages, M.ptr(q), M.ptr(k),
+            M.ptr(k_cache), M.ptr(v_cache), M.ptr(seq_lens_out), M.ptr(error_word), s))
+    return q, k
+
+
+def kv4_read_rows(k_cache, v_cache, positions, row_seq, page_table, error_word=None, stream=None):
+    """attn_kv4_read_rows: the tokens at `positions` of page-table rows `row_seq` as the bf16 values the cache holds:
+    (k, v), each [B][nkv][128]."""
+    import torch
+    pages, nkv = _check_kv4(k_cache, v_cache)
+    A.check_i32(positions=positions, row_seq=row_seq, page_table=page_table)
+    B = positions.numel()
+    if (B if row_seq is None else row_seq.numel()) != B or (row_seq is None and page_table.shape[0] < B):
+        raise ValueError("row_seq has one entry per position")
+    with A.on_stream(k_cache, stream) as s:
+        k = torch.empty(B, nkv, HEAD_DIM, dtype=torch.bfloat16, device=k_cache.device)
+        v = torch.empty_like(k)
+        M.check("attn_kv4_read_rows", lib().attn_kv4_read_rows(
+            M.ptr(k_cache), M.ptr(v_cache), pages, M.ptr(positions), M.ptr(row_seq), page_table.shape[0],
+            M.ptr(page_table), page_table.shape[1], PAGE, B, nkv, HEAD_DIM, M.ptr(k), M.ptr(v), M.ptr(error_word), s))
+    return k, v
+
+
+def kv4_decode(q, k_cache, v_cache, page_table, seq_lens, scale: float, row_seq=None, split_tokens: int | None = None,
+               max_splits: int | None = None, quant: bool = False, workspace=None, error_word=None, stream=None):
+    """attn_kv4_decode_rows: attention of q bf16 [B][nq][128] over the first seq_lens[b] tokens of page-table row
+    row_seq[b] (None: b).  split_tokens None: the split that fills the GPU.  Returns (out bf16 [B][nq][128], out_q e4m3
+    [B][nq * 128] or None, out_s [nq][ld] or None)."""
+    import torch
+    pages, nkv = _check_kv4(k_cache, v_cache)
+    A.check_heads("q", q, torch.bfloat16)
+    A.check_i32(page_table=page_table, seq_lens=seq_lens, row_seq=row_seq)
+    if not q.is_contiguous():
+        raise ValueError("q is contiguous")
+    B, nq = q.shape[:2]
+    if seq_lens.numel() != B or (B if row_seq is None else row_seq.numel()) != B:
+        raise ValueError("seq_lens and row_seq have one entry per row of q")
+    if row_seq is None and page_table.shape[0] < B:
+        raise ValueError("the page table has a row per row of q when row_seq is None")
+    num_seqs, max_pages = page_table.shape
+    k = lib()
+    if split_tokens is None:
+        split_tokens = k.attn_kv4_split_tokens(B, nkv, max_pages * PAGE)
+    if max_splits is None:
+        max_splits = -(-max_pages * PAGE // split_tokens)
+    with A.on_stream(q, stream) as s:
+        if workspace is None:
+            workspace = torch.empty(max(k.attn_kv4_decode_workspace_bytes(B, nq, max_splits), 16), dtype=torch.uint8,
+                                    device=q.device)
+        out = torch.empty_like(q)
+        out_q = out_s = None
+        ld = (B + 3) // 4 * 4
+        if quant:
+            out_q = torch.empty(B, nq * HEAD_DIM, dtype=torch.uint8, device=q.device)
+            out_s = torch.empty(nq, ld, dtype=torch.float32, device=q.device)
+        M.check("attn_kv4_decode_rows", k.attn_kv4_decode_rows(
+            M.ptr(q), M.ptr(k_cache), M.ptr(v_cache), pages, M.ptr(page_table), max_pages, M.ptr(row_seq), num_seqs,
+            M.ptr(seq_lens), B, nq, nkv, HEAD_DIM, PAGE, scale, split_tokens, max_splits, M.ptr(workspace),
+            workspace.numel() * workspace.element_size(), M.ptr(out), M.ptr(out_q), M.ptr(out_s), ld,
+            M.ptr(error_word), s))
+    return out, out_q, out_s
+
+
+# ---------------------------------------------------------------- pages
+
+def _cache_args(caches):
+    """(pointer, bytes between caches, caches, pages, bytes of a page) of a tensor [caches][pages][...]."""
+    if caches.dim() < 3 or not caches[0].is_contiguous():
+        raise ValueError("caches is a tensor [caches][pages][...] with every cache contiguous")
+    e = caches.element_size()
+    return M.ptr(caches), caches.stride(0) * e, caches.shape[0], caches.shape[1], caches.stride(1) * e
+
+
+def _check_table(table, lens):
+    if table.dim() != 2 or lens.numel() != table.shape[0]:
+        raise ValueError("lens has one entry per page-table row")
+
+
+def fork_pages(caches, table, lens, parents, reserve=None, workspace=None, error_word=None, stream=None):
+    """kv_pages_fork: row i of the result is row parents[i] (-1: empty) with room for reserve[i] more tokens; full
+    pages are shared, a page in part filled is copied for all appending rows but one.  Returns (table, lens) int32,
+    new tensors."""
+    import torch
+    A.check_i32(table=table, lens=lens, parents=parents, reserve=reserve)
+    _check_table(table, lens)
+    if reserve is not None and reserve.numel() != parents.numel():
+        raise ValueError("reserve has one entry per parent")
+    ptr, stride, n, pages, page_bytes = _cache_args(caches)
+    rows, k = parents.numel(), lib()
+    with A.on_stream(caches, stream) as s:
+        if workspace is None:
+            workspace = torch.empty(k.kv_pages_workspace_bytes(pages, rows), dtype=torch.uint8, device=caches.device)
+        out = torch.empty(rows, table.shape[1], dtype=torch.int32, device=caches.device)
+        lens_out = torch.empty(rows, dtype=torch.int32, device=caches.device)
+        M.check("kv_pages_fork", k.kv_pages_fork(
+            ptr, stride, n, pages, page_bytes, PAGE, M.ptr(table), table.shape[1], M.ptr(lens), table.shape[0],
+            M.ptr(parents), M.ptr(reserve), rows, M.ptr(out), M.ptr(lens_out), M.ptr(workspace),
+            workspace.numel() * workspace.element_size(), M.ptr(error_word), s))
+    return out, lens_out
+
+
+def compact_pages(caches, table, lens, out=None, workspace=None, error_word=None, stream=None):
+    """kv_pages_compact: moves the pages in use to the lowest ids.  Returns (table, pages in use int32 [1]); `out` may
+    be `table` itself."""
+    import torch
+    A.check_i32(table=table, lens=lens, out=out)
+    _check_table(table, lens)
+    if out is not None and out.shape != table.shape:
+        raise ValueError("out has the page table's shape")
+    ptr, stride, n, pages, page_bytes = _cache_args(caches)
+    k = lib()
+    with A.on_stream(caches, stream) as s:
+        if workspace is None:
+            workspace = torch.empty(k.kv_pages_workspace_bytes(pages, table.shape[0]), dtype=torch.uint8,
+                                    device=caches.device)
+        out = torch.empty_like(table) if out is None else out
+        used = torch.empty(1, dtype=torch.int32, device=caches.device)
+        M.check("kv_pages_compact", k.kv_pages_compact(
+            ptr, stride, n, pages, page_bytes, PAGE, M.ptr(table), table.shape[1], M.ptr(lens), table.shape[0],
+            M.ptr(out), M.ptr(used), M.ptr(workspace), workspace.numel() * workspace.element_size(),
+            M.ptr(error_word), s))
+    return out, used
