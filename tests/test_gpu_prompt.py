@@ -205,3 +205,32 @@ def test_agrees_with_the_paged_prefill(gpu):
                          torch.arange(1, n + 1, dtype=torch.int32, device=gpu), nq, nkv, 0.1, prefill_rows=n)[0]
     ref, tol = R.attend(f64(q), f64(k), f64(v), np.arange(1, n + 1), 0.1)
     assert (np.abs(f64(out) - ref) <= tol).all() and (np.abs(f64(paged) - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+def test_scales_of_any_sign(gpu, scale):
+    rng = np.random.default_rng(10)
+    n = 300
+    q, k, v = rows(rng, n, 6, D).to(gpu), rows(rng, n, 2, D).to(gpu), rows(rng, n, 2, D).to(gpu)
+    out, _, _ = A.prompt_packed(q, k, v, cu_of([n], gpu), scale)
+    ref, tol = R.attend(f64(-q if scale < 0 else q), f64(k), f64(v), np.arange(1, n + 1), abs(scale))
+    assert (np.abs(f64(out) - ref) <= tol).all()
+
+
+def test_many_uneven_prompts(gpu):
+    """More tiles than SMs, one M tile and two, one step and several: what a CTA carries from tile to tile."""
+    rng = np.random.default_rng(11)
+    nq, nkv = 32, 8
+    lens = [int(x) for x in np.exp(rng.uniform(0, np.log(700), 70))]
+    T = sum(lens)
+    q, k, v = rows(rng, T, nq, D).to(gpu), rows(rng, T, nkv, D).to(gpu), rows(rng, T, nkv, D).to(gpu)
+    for _ in range(3):
+        out, _, _ = A.prompt_packed(q, k, v, cu_of(lens, gpu), 0.1)
+    at = 0
+    for n in lens:
+        if n < 200 or n == max(lens):
+            s = slice(at, at + n)
+            ref, tol = R.attend(f64(q[s]), f64(k[s]), f64(v[s]), np.arange(1, n + 1), 0.1)
+            assert (np.abs(f64(out[s]) - ref) <= tol).all()
+        at += n
+    assert torch.equal(out, A.prompt_packed(q, k, v, cu_of(lens, gpu), 0.1)[0])
