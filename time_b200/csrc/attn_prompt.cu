@@ -131,12 +131,14 @@ __device__ __forceinline__ bool zero_nonfinite(uint4& v) {
 // V arrive by TMA in a ring of 128-key stages that runs on into the next tile,
 // as do Q and its first scores, under the last tile's epilogue.  The running
 // maximum is left behind by up to 2^8 before the output is rescaled, so a
-// rescale is rare and the softmax threads do it themselves: the scores' arrival
-// means that the product before is done.
+// rescale is rare and the softmax threads do it themselves.  Scores come in
+// steps of 64 keys into two buffers per tile, so the tensor core is a step ahead
+// of the softmax: TMEM holds 2 x 2 x 64 columns of scores and 2 x 128 of output.
 
 constexpr int kSms = 148;
 constexpr int kRows = 256;
-constexpr int kKeys = 128;
+constexpr int kKeys = 128;                              // of a ring stage
+constexpr int kStep = 64;                               // of a softmax step
 constexpr int kStages = 5;                            // K and V tiles in flight, 32 KB each
 constexpr int kThreads = 384;                         // 2 softmax warpgroups; a warp each for MMA, K and V loads, Q loads, V cleaning
 constexpr uint32_t kHalf = kKeys * 128;               // 64 dims of a 128-row tile: rows of 128 bytes, swizzled
@@ -151,14 +153,16 @@ struct TileWork {
     int first;                                          // row of the sequence's first token
     int pos0;                                           // position of the tile's first rows
     int rows, mt;                                       // rows, M tiles in use
-    int steps, first_masked;                            // from that step on there are positions that not every row attends
+    int steps, first_masked;                            // steps of 64 keys; from that one on there are positions that
+                                                        // not every row attends
     int last;                                           // keys of the last step, up to a multiple of 16
     int dirty;                                          // V values zeroed behind pos0
 };
 
 struct Bars {
     uint64_t full[kStages], empty[kStages];         // ring of K0 V0 K1 V1 ...
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[2][2], p_full[2][2];                // [M tile][score buffer]
+    uint64_t pv_done[2], o_full[2];
     uint64_t tile_full[2], tile_empty[2], q_full, q_empty, go, clean, drain;
 };
 
@@ -206,15 +210,18 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     __shared__ uint32_t tmem_s;
     __shared__ int abort_s;
     volatile int* abort_flag = &abort_s;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform for the compiler
     if (warp == 9 && lane == 0) {
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&bars.full[i], 1);
             mbar_init(&bars.empty[i], 1);
         }
         for (int t = 0; t < 2; ++t) {
-            mbar_init(&bars.s_full[t], 1);
-            mbar_init(&bars.p_full[t], 128);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&bars.s_full[t][b], 1);
+                mbar_init(&bars.p_full[t][b], 128);
+            }
+            mbar_init(&bars.pv_done[t], 1);
             mbar_init(&bars.o_full[t], 2);
             mbar_init(&bars.tile_full[t], 1);
             mbar_init(&bars.tile_empty[t], kTileReaders);
@@ -254,7 +261,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 const int kvh = static_cast<int>(c % p.nkv);
                 if (lane == 0) {
                     ok = wait(&bars.tile_empty[n & 1], ((n >> 1) & 1) ^ 1);
-                    int steps = 0;
+                    int loads = 0;
                     if (ok) {
                         TileWork w;
                         w.some = t.some;
@@ -264,16 +271,17 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                         w.rows = min(tile_pos, t.len - w.pos0) * p.G;
                         w.mt = w.rows > 128 ? 2 : 1;
                         const int pos1 = min(w.pos0 + tile_pos, t.len) - 1;
-                        steps = w.steps = t.some ? pos1 / kKeys + 1 : 0;
-                        w.last = (pos1 % kKeys + 16) / 16 * 16;
-                        w.first_masked = (w.pos0 + 1) / kKeys;
+                        w.steps = t.some ? pos1 / kStep + 1 : 0;
+                        loads = (w.steps + 1) / 2 * 2;
+                        w.last = (pos1 % kStep + 16) / 16 * 16;
+                        w.first_masked = (w.pos0 + 1) / kStep;
                         w.dirty = 0;
                         tile_s[n & 1] = w;
                         mbar_arrive(&bars.tile_full[n & 1]);
                     }
                     if (ok) {
                         const int x = kvh * kD;
-                        for (int j = 0; j < 2 * steps; ++j, ++item) {
+                        for (int j = 0; j < loads; ++j, ++item) {
                             const int st = item % kStages;
                             if (!(ok = wait(&bars.empty[st], ((item / kStages) & 1) ^ 1))) break;
                             uint8_t* dst = kv_s + st * kTileBytes;
@@ -289,68 +297,91 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 }
                 ok = __shfl_sync(0xffffffffu, ok, 0) && t.some;
             }
-        } else if (warp == 8 && lane == 0) {
-            // ---- MMA issue
+        } else if (warp == 8) {
+            // ---- MMA issue, by the whole warp
+            const bool el = lane == 0;
+            auto uni = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };       // uniform for the compiler as well
+            auto all = [&](bool x) { return __all_sync(0xffffffffu, x); };
             const uint32_t negate = p.flip_q ? 1u << 13 : 0u;      // of A
             constexpr uint32_t id_o = idesc_bf16_f32(128, kD, true);
-            int item = 0, masked = 0;                   // ring items and masked steps so far
-            int p_n[2] = {0, 0};                        // steps of each M tile so far
-            auto wait_item = [&](int i) { return wait(&bars.full[i % kStages], (i / kStages) & 1); };
-            auto scores = [&](int t, int i, int keys) { // S_t = Q_t K^T, K in ring item i
-                const uint32_t id_s = idesc_bf16_f32(128, keys, false) | negate;
-                const uint32_t q = smem_u32(q_s + t * kHalf), k = smem_u32(kv_s + i % kStages * kTileBytes);
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    const uint32_t dims = (ks & 3) * 32;
-                    umma_f16(tmem + t * 128, umma_desc_sw128(q + (ks >> 2) * 2 * kHalf + dims),
-                             umma_desc_sw128(k + (ks >> 2) * kHalf + dims), id_s, ks > 0);
-                }
-                umma_commit(&bars.s_full[t]);
+            const uint32_t tm = uni(tmem);
+            const uint32_t q_lo = desc_lo_k(smem_u32(q_s)), k_lo = desc_lo_k(smem_u32(kv_s)), v_lo = desc_lo_mn(smem_u32(kv_s), kHalf);
+            int item = 0, stage = 0;                    // ring items so far, and their stage
+            uint32_t p_phase = 0;                       // of p_full[t][b], bit 2 t + b
+            int masked = 0;
+            auto stage_of = [&](int ahead) { return (stage + ahead) % kStages; };
+            auto wait_item = [&](int ahead) {
+                return all(wait(&bars.full[stage_of(ahead)], ((item + ahead) / kStages) & 1));
             };
             bool ok = true;
             for (int n = 0; ok; ++n) {
-                if (!(ok = wait(&bars.tile_full[n & 1], (n >> 1) & 1))) break;
-                const TileWork w = tile_s[n & 1];
-                if (!w.some) break;
-                if (!(ok = wait(&bars.q_full, n & 1) && wait_item(item))) break;
-                tc_fence_after();
-                for (int t = 0; t < w.mt; ++t) scores(t, item, w.steps == 1 ? w.last : kKeys);
-                if (w.steps == 1) umma_commit(&bars.q_empty);
-                umma_commit(&bars.empty[item % kStages]);
-                for (int i = 0; i < w.steps && ok; ++i) {
-                    const int vi = item + 1, ki = item + 2;
-                    if (!(ok = wait_item(vi))) break;
-                    const bool clean = i >= w.first_masked;
-                    if (clean) mbar_arrive(&bars.go);
-                    for (int t = 0; t < w.mt && ok; ++t) {
-                        if (!(ok = wait(&bars.p_full[t], p_n[t]++ & 1))) break;
-                        if (t == 0 && clean && !(ok = wait(&bars.clean, masked++ & 1))) break;
-                        tc_fence_after();
-                        const uint32_t v = smem_u32(kv_s + vi % kStages * kTileBytes);
-                        const int ksteps = i + 1 == w.steps ? w.last / 16 : 8;
+                if (!(ok = all(wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
+                const TileWork& slot = tile_s[n & 1];
+                if (!uni(slot.some)) break;
+                const int steps = uni(slot.steps), mt = uni(slot.mt), last = uni(slot.last), first_masked = uni(slot.first_masked);
+                int k_at = 0;                           // K item of the scores issued next, from the tile's first
+                // S_t of step j into buffer j % 2; what the last M tile's scores are the last to read is free after them
+                auto scores = [&](int t, int j) {
+                    const int st = stage_of(k_at);
+                    const uint32_t id_s = idesc_bf16_f32(128, j + 1 == steps ? last : kStep, false) | negate;
+                    const uint32_t q = q_lo + t * (kHalf >> 4), k = k_lo + st * (kTileBytes >> 4) + (j & 1) * (kStep * 128 >> 4);
+                    const uint32_t d = tm + t * 128 + (j & 1) * kStep;
 #pragma unroll
-                        for (int ks = 0; ks < 8; ++ks)  // 16 keys: 16 rows of 128 bytes
-                            if (ks < ksteps)
-                                umma_f16_ta(tmem + 256 + t * 128, tmem + t * 128 + ks * 8,
-                                            umma_desc_mn_sw128(v + ks * 2048, kHalf), id_o, i > 0 || ks > 0);
-                        if (i == w.steps - 1) {
-                            mbar_arrive(&bars.o_full[t]);   // the cleaner's word on the tile goes with it
-                            umma_commit(&bars.o_full[t]);
-                        }
-                        if (t == w.mt - 1) umma_commit(&bars.empty[vi % kStages]);
-                        if (i + 1 < w.steps) {
-                            if (t == 0 && !(ok = wait_item(ki))) break;
-                            scores(t, ki, i + 2 == w.steps ? w.last : kKeys);
-                            if (t == w.mt - 1 && i + 2 == w.steps) umma_commit(&bars.q_empty);
-                            if (t == w.mt - 1) umma_commit(&bars.empty[ki % kStages]);
-                        }
+                    for (int ks = 0; ks < 8; ++ks)
+                        umma_f16_warp(d, q + (ks >> 2) * (2 * kHalf >> 4) + (ks & 3) * 2, k + (ks >> 2) * (kHalf >> 4) + (ks & 3) * 2,
+                                      id_s, ks > 0);
+                    umma_commit_warp(&bars.s_full[t][j & 1]);
+                    if (t == mt - 1 && ((j & 1) || j + 1 == steps)) {
+                        umma_commit_warp(&bars.empty[st]);
+                        k_at += 2;
+                        if (j + 1 == steps) umma_commit_warp(&bars.q_empty);
                     }
-                    item += 2;
+                };
+                if (!(ok = all(wait(&bars.q_full, n & 1)) && wait_item(0))) break;
+                tc_fence_after();
+                for (int j = 0; j < 2 && j < steps; ++j)
+                    for (int t = 0; t < mt; ++t) scores(t, j);
+                if (!(ok = wait_item(1))) break;
+                bool ready = false;                     // what a test for the next weights gave, under the MMAs before
+                for (int j = 0; j < steps && ok; ++j) {
+                    const int st = stage_of(j / 2 * 2 + 1);
+                    const bool clean = j >= first_masked;
+                    if (clean && el) mbar_arrive(&bars.go);
+                    const uint32_t v = v_lo + st * (kTileBytes >> 4) + (j & 1) * (kStep * 128 >> 4);
+                    const int ksteps = j + 1 == steps ? last / 16 : kStep / 16;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (t >= mt || !ok) break;
+                        const int bit = 2 * t + (j & 1);
+                        if (!all(ready) && !(ok = all(wait(&bars.p_full[t][j & 1], (p_phase >> bit) & 1)))) break;
+                        p_phase ^= 1u << bit;
+                        if (t == 0 && clean && !(ok = all(wait(&bars.clean, masked++ & 1)))) break;
+                        tc_fence_after();
+                        const uint32_t pa = tm + t * 128 + (j & 1) * kStep;
+#pragma unroll
+                        for (int ks = 0; ks < kStep / 16; ++ks)     // 16 keys: 16 rows of 128 bytes
+                            if (ks < ksteps)
+                                umma_f16_ta_warp(tm + 256 + t * 128, pa + ks * 8, v + ks * (2048 >> 4), id_o, j > 0 || ks > 0);
+                        umma_commit_warp(&bars.pv_done[t]);
+                        if (j + 1 == steps) {
+                            if (el) mbar_arrive(&bars.o_full[t]);   // the cleaner's word on the tile goes with it
+                            umma_commit_warp(&bars.o_full[t]);
+                        }
+                        if (t == mt - 1 && ((j & 1) || j + 1 == steps)) umma_commit_warp(&bars.empty[st]);
+                        // K of step j + 2, and V for its product
+                        if (t == 0 && !(j & 1) && j + 2 < steps && !(ok = wait_item(k_at) && wait_item(k_at + 1))) break;
+                        const int nt = t + 1 < mt ? t + 1 : 0, nb = (t + 1 < mt ? j : j + 1) & 1;
+                        ready = mbar_test(&bars.p_full[nt][nb], (p_phase >> (2 * nt + nb)) & 1);
+                        if (j + 2 < steps) scores(t, j + 2);
+                    }
                 }
-                mbar_arrive(&bars.tile_empty[n & 1]);
+                const int used = (steps + 1) / 2 * 2;
+                item += used;
+                stage = (stage + used) % kStages;
+                if (el) mbar_arrive(&bars.tile_empty[n & 1]);
             }
             if (!ok) {
-                umma_commit(&bars.drain);
+                umma_commit_warp(&bars.drain);
                 mbar_drain(&bars.drain, 0);
             }
         } else if (warp == 10 && lane == 0) {
@@ -378,12 +409,12 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 const TileWork w = tile_s[n & 1];
                 if (!w.some) break;
                 for (int i = w.first_masked; i < w.steps && ok; ++i) {
-                    const int vi = item + 2 * i + 1;
+                    const int vi = item + i / 2 * 2 + 1;
                     ok = wait(&bars.go, masked++ & 1) && wait(&bars.full[vi % kStages], (vi / kStages) & 1);
                     if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                    uint8_t* v = kv_s + vi % kStages * kTileBytes;
-                    const int j0 = max(w.pos0 + 1 - i * kKeys, 0);       // first such row of the tile
-                    const int j1 = i + 1 == w.steps ? w.last : kKeys;
+                    uint8_t* v = kv_s + vi % kStages * kTileBytes + (i & 1) * (kStep * 128);
+                    const int j0 = max(w.pos0 + 1 - i * kStep, 0);       // first such row of the step
+                    const int j1 = i + 1 == w.steps ? w.last : kStep;
                     bool dirty = false;
 #pragma unroll 8
                     for (int c = lane; c < (j1 - j0) * 16; c += 32) {
@@ -398,7 +429,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     mbar_arrive(&bars.clean);
                 }
-                item += 2 * w.steps;
+                item += (w.steps + 1) / 2 * 2;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars.tile_empty[n & 1]);
             }
@@ -410,7 +441,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         const uint32_t ts = tmem + (static_cast<uint32_t>(warp & 3) << 21) + t * 128;   // this warp's 32 lanes
         const uint32_t to = ts + 256;
         const float sl2 = p.scale_log2;
-        int s_n = 0, o_n = 0;                           // steps and tiles of this M tile so far
+        uint32_t s_phase = 0;                           // of s_full[t][b], bit b
+        int pv_n = 0, o_n = 0;                          // steps and tiles of this M tile so far
         bool ok = true;
         for (int n = 0; ok; ++n) {
             if (!(ok = __all_sync(0xffffffffu, wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
@@ -420,28 +452,31 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 const int at = group_div(min(i_row, w.rows - 1), g_inv);
                 const int pos = w.pos0 + at;
                 float m = -INFINITY, l = 0.0f;
-                for (int i = 0; i < w.steps; ++i) {
-                    if (!(ok = __all_sync(0xffffffffu, wait(&bars.s_full[t], s_n++ & 1)))) break;
+                for (int j = 0; j < w.steps; ++j, ++pv_n) {
+                    const uint32_t sb = ts + (j & 1) * kStep;
+                    if (!(ok = __all_sync(0xffffffffu, wait(&bars.s_full[t][j & 1], (s_phase >> (j & 1)) & 1)))) break;
+                    s_phase ^= 1u << (j & 1);
                     tc_fence_after();
-                    uint32_t s[4][32];
+                    uint32_t s[2][32];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s[c]);
+                    for (int c = 0; c < 2; ++c) tmem_ld32(sb + 32 * c, s[c]);
                     tmem_wait_ld();
-                    if (i >= w.first_masked) {
-                        const int lim = pos - i * kKeys;
+                    if (j >= w.first_masked) {
+                        const int lim = pos - j * kStep;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
+                        for (int c = 0; c < 2; ++c)
 #pragma unroll
                             for (int e = 0; e < 32; ++e)
                                 if (32 * c + e > lim) s[c][e] = 0xFF800000u;
                     }
                     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
+                    for (int e = 0; e < 32; e += 2)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][e]));
+                        for (int c = 0; c < 4; ++c)
+                            mx[c] = fmaxf(mx[c], __uint_as_float(s[c >> 1][e + (c & 1)]));
                     const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    if (i == 0) {
+                    if (j == 0) {
                         m = mt;
                     } else {
                         const bool need = (mt - m) * sl2 > 8.0f;
@@ -449,6 +484,9 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                             const float f = need ? ex2((m - mt) * sl2) : 1.0f;
                             l *= f;
                             if (need) m = mt;
+                            // the product of the step before has to be in
+                            if (!(ok = __all_sync(0xffffffffu, wait(&bars.pv_done[t], (pv_n - 1) & 1)))) break;
+                            tc_fence_after();
 #pragma unroll
                             for (int c = 0; c < 4; ++c) {
                                 uint32_t o[32];
@@ -463,7 +501,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     const float nm = m == -INFINITY ? 0.0f : -m * sl2;     // nothing but -inf so far: weights 0, not NaN
                     float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < 2; ++c) {
                         uint32_t wt[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
@@ -474,13 +512,13 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                             sum[e & 1] = fadd2(sum[e & 1], x);
                             wt[e] = pack_bf16(x.x, x.y);    // the weights' rounding, 2^-8 at most; the sum has them whole
                         }
-                        tmem_st16(ts + 16 * c, wt);
+                        tmem_st16(sb + 16 * c, wt);
                     }
                     sum[0] = fadd2(sum[0], sum[1]);
                     l += sum[0].x + sum[0].y;
                     tmem_wait_st();
                     tc_fence_before();
-                    mbar_arrive(&bars.p_full[t]);
+                    mbar_arrive(&bars.p_full[t][j & 1]);
                 }
                 if (ok) ok = __all_sync(0xffffffffu, wait(&bars.o_full[t], o_n++ & 1));
                 if (!ok) break;
