@@ -123,29 +123,36 @@ __device__ __forceinline__ bool zero_nonfinite(uint4& v) {
 
 // ---------------------------------------------------------------- kernel
 //
-// A CTA per SM takes tiles of 256 rows, two M = 128 tiles with a softmax
-// warpgroup each, one thread per row.  While one tile's softmax runs on its
-// scores, the tensor core works on the other's: S = Q K^T into TMEM, read as
-// fp32, written back over itself as the bf16 weights P, which the second MMA
-// takes from TMEM as its A operand with V (MN-major) from shared memory.  K and
-// V arrive by TMA in a ring of 128-key stages that runs on into the next tile,
-// as do Q and its first scores, under the last tile's epilogue.  The running
-// maximum is left behind by up to 2^8 before the output is rescaled, so a
-// rescale is rare and the softmax threads do it themselves.  Scores come in
-// steps of 64 keys into two buffers per tile, so the tensor core is a step ahead
-// of the softmax: TMEM holds 2 x 2 x 64 columns of scores and 2 x 128 of output.
+// A CTA per SM takes tiles of 256 rows, two M = 128 tiles of 128 rows each:
+//
+//   warps 0-3, 4-7   softmax of M tile 0 and 1, one thread per row
+//   warps 8-11       epilogue: output rows from TMEM to memory
+//   warps 12, 13     MMA issue for M tile 0 and 1
+//   warp 14          tiles, Q, and the ring of K and V stages, by TMA
+//   warp 15          V of masked positions
+//
+// S = Q K^T of 64 keys goes to one of two TMEM buffers per M tile, is read as
+// fp32 and written back over itself as the bf16 weights P, which the second MMA
+// takes from TMEM as its A operand with V (MN-major) from shared memory; the
+// scores of the next step are computed meanwhile.  TMEM holds 2 x 2 x 64 columns
+// of scores and 2 x 128 of output.  The running maximum is left behind by up to
+// 2^8 before the output is rescaled, so a rescale is rare and the softmax threads
+// do it themselves.  An M tile's MMAs have a warp of their own, so that what one
+// spends between MMAs (barriers, descriptors) is covered by the other's.  The
+// next tile's loads, scores and softmax run under a tile's epilogue.
 
 constexpr int kSms = 148;
 constexpr int kRows = 256;
 constexpr int kKeys = 128;                              // of a ring stage
 constexpr int kStep = 64;                               // of a softmax step
-constexpr int kStages = 5;                            // K and V tiles in flight, 32 KB each
-constexpr int kThreads = 384;                         // 2 softmax warpgroups; a warp each for MMA, K and V loads, Q loads, V cleaning
-constexpr uint32_t kHalf = kKeys * 128;               // 64 dims of a 128-row tile: rows of 128 bytes, swizzled
+constexpr int kFmaPairs = 2;                            // pairs of eight whose exponentials go to the FMA pipe
+constexpr int kStages = 4;                              // K and V tiles in flight, 32 KB each
+constexpr int kThreads = 512;
+constexpr uint32_t kHalf = kKeys * 128;                 // 64 dims of a 128-row tile: rows of 128 bytes, swizzled
 constexpr uint32_t kTileBytes = 2 * kHalf;
 constexpr size_t kSmem = 2 * kTileBytes + kStages * kTileBytes + 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
-constexpr int kTileReaders = 8 + 1 + 2;                 // softmax warps, MMA, Q loads, V cleaning
+constexpr int kTileReaders = 8 + 4 + 2 + 1;             // softmax, epilogue, MMA warps and the cleaner
 
 // A tile as the load warp hands it to the others.
 struct TileWork {
@@ -159,15 +166,15 @@ struct TileWork {
     int dirty;                                          // V values zeroed behind pos0
 };
 
-struct Bars {
-    uint64_t full[kStages], empty[kStages];         // ring of K0 V0 K1 V1 ...
-    uint64_t s_full[2][2], p_full[2][2];                // [M tile][score buffer]
-    uint64_t pv_done[2], o_full[2];
-    uint64_t tile_full[2], tile_empty[2], q_full, q_empty, go, clean, drain;
-};
-
 // x / G for x < 4096, G <= 16
 __device__ __forceinline__ int group_div(int x, uint32_t g_inv) { return static_cast<int>(static_cast<uint32_t>(x) * g_inv >> 16); }
+
+struct Bars {
+    uint64_t full[kStages], empty[kStages];             // ring of K0 V0 K1 V1 ...
+    uint64_t s_full[2][2], p_full[2][2];                // [M tile][score buffer]
+    uint64_t pv_done[2], o_full[2], o_free[2];
+    uint64_t tile_full[2], tile_empty[2], q_full, q_empty, go, clean, drain[2];
+};
 
 // Bounded wait that reads the clock and the abort flag every 256 tries only: a
 // read of the global timer takes longer than most of the waits here.
@@ -192,29 +199,96 @@ __device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
     while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 < kWaitNs) {}
 }
 
+// 32 bytes to a 32-byte aligned address.
+__device__ __forceinline__ void st_global_32(void* dst, const uint32_t* r) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 :: "l"(dst), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+
 __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
     uint64_t ar = *reinterpret_cast<uint64_t*>(&a), br = *reinterpret_cast<uint64_t*>(&b), d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(ar), "l"(br));
     return *reinterpret_cast<float2*>(&d);
 }
 
+// 2^x for x up to 127 on the FMA pipe, which the softmax leaves idle while the
+// MUFU is its limit: x = n + f with n the nearest integer, a polynomial for 2^f
+// on [-1/2, 1/2] (least largest relative error with P(0) = 1: 2.8e-6), n added
+// to the exponent.  x below -127 gives 0.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+    constexpr float kMagic = 12582912.0f;               // 1.5 * 2^23: the sum's low bits are n
+    x.x = fmaxf(x.x, -127.0f);
+    x.y = fmaxf(x.y, -127.0f);
+    const float2 t = fadd2(x, make_float2(kMagic, kMagic));
+    const float2 n = fadd2(t, make_float2(-kMagic, -kMagic));
+    const float2 f = ffma2(n, make_float2(-1.0f, -1.0f), x);
+    float2 r = ffma2(f, make_float2(0.009582852944731712f, 0.009582852944731712f), make_float2(0.055906426161527634f, 0.055906426161527634f));
+    r = ffma2(f, r, make_float2(0.24024099111557007f, 0.24024099111557007f));
+    r = ffma2(f, r, make_float2(0.6931241750717163f, 0.6931241750717163f));
+    r = ffma2(f, r, make_float2(1.0f, 1.0f));
+    return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23)));
+}
+
+// The largest of three, NaN if any is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Epilogue of a row of a tile with NaN or infinite values in V that not every
+// row attends: they were zeroed for the MMA, so a row that attends them adds
+// them here (a positive weight times one of them is the same again).
+__device__ __noinline__ void epilogue_dirty(const PromptParams& p, uint32_t to, float inv, long long first, int pos0, int pos,
+                                            int kvh, int head, bool store) {
+    const __nv_bfloat16* vrow = p.v + first * p.v_stride + kvh * kD;
+    const long long out_row = (first + pos) * p.nq + head;
+    float amax = 0.0f;
+    for (int pass = 0; pass < (p.out_q ? 2 : 1); ++pass) {
+        const float qi = amax > 0.0f ? 448.0f / amax : 0.0f;
+        for (int c = 0; c < 8; ++c) {
+            uint32_t o[16];
+            tmem_ld16(to + 16 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float x = __uint_as_float(o[e]) * inv;
+                for (int j = pos0 + 1; j <= pos; ++j) {
+                    const float y = __bfloat162float(vrow[j * p.v_stride + 16 * c + e]);
+                    if (!isfinite(y)) x += y;
+                }
+                if (pass == 0) {
+                    amax = fmaxf(amax, fabsf(x));
+                    if (store) p.out[out_row * kD + 16 * c + e] = __float2bfloat16_rn(x);
+                } else if (store) {
+                    p.out_q[out_row * kD + 16 * c + e] = amax > 0.0f ? static_cast<uint8_t>(cvt_e4m3x2(x * qi, 0.0f)) : 0;
+                }
+            }
+        }
+    }
+    if (p.out_q && store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
 prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                 const __grid_constant__ CUtensorMap vmap) {
+              const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ uint8_t sm_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* q_s = sm;                                  // [2 halves][256 rows][128 B]
     uint8_t* kv_s = sm + 2 * kTileBytes;                // [stages][2 halves][128][128 B]
     __shared__ Bars bars;
     __shared__ TileWork tile_s[2];
+    __shared__ float l_s[kRows];                        // row sums
     __shared__ uint32_t tmem_s;
     __shared__ int abort_s;
     volatile int* abort_flag = &abort_s;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform for the compiler
-    if (warp == 9 && lane == 0) {
+    if (warp == 15 && lane == 0) {
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&bars.full[i], 1);
-            mbar_init(&bars.empty[i], 1);
+            mbar_init(&bars.empty[i], 2);
         }
         for (int t = 0; t < 2; ++t) {
             for (int b = 0; b < 2; ++b) {
@@ -223,245 +297,60 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             }
             mbar_init(&bars.pv_done[t], 1);
             mbar_init(&bars.o_full[t], 2);
+            mbar_init(&bars.o_free[t], 128);
             mbar_init(&bars.tile_full[t], 1);
             mbar_init(&bars.tile_empty[t], kTileReaders);
+            mbar_init(&bars.drain[t], 1);
         }
         mbar_init(&bars.q_full, 1);
-        mbar_init(&bars.q_empty, 1);
-        mbar_init(&bars.go, 1);
+        mbar_init(&bars.q_empty, 2);
+        mbar_init(&bars.go, 2);
         mbar_init(&bars.clean, 32);
-        mbar_init(&bars.drain, 1);
         abort_s = 0;
         fence_mbar_init();
         prefetch_tmap(&qmap);
         prefetch_tmap(&kmap);
         prefetch_tmap(&vmap);
-    } else if (warp == 8) {
+    } else if (warp == 12) {
         tmem_alloc(&tmem_s, 512);
         tc_fence_before();
     }
+    const uint32_t g_inv = (65536u + p.G - 1) / p.G;
+    const int tile_pos = kRows / p.G;                   // positions of a tile
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_s;
-    const uint32_t g_inv = (65536u + p.G - 1) / p.G;
-    const int tile_pos = kRows / p.G;                 // positions of a tile
     auto wait = [&](uint64_t* bar, uint32_t parity) { return wait_phase(bar, parity, abort_flag); };
+    auto all = [&](bool x) { return __all_sync(0xffffffffu, x); };
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        if (warp == 9) {
-            // ---- tiles and loads: K and V of step 0, 1, ... of every tile
-            const TileOrder order(p, tile_pos, blockIdx.x == 0);
-            int item = 0;
-            bool ok = true;
-            for (int n = 0; ok; ++n) {
-                // every other round backwards: a CTA's tiles even out
-                const unsigned int c = n * gridDim.x + ((n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-                const Tile t = order.find(c / p.nkv);
-                const int kvh = static_cast<int>(c % p.nkv);
-                if (lane == 0) {
-                    ok = wait(&bars.tile_empty[n & 1], ((n >> 1) & 1) ^ 1);
-                    int loads = 0;
-                    if (ok) {
-                        TileWork w;
-                        w.some = t.some;
-                        w.kvh = kvh;
-                        w.first = t.first;
-                        w.pos0 = t.index * tile_pos;
-                        w.rows = min(tile_pos, t.len - w.pos0) * p.G;
-                        w.mt = w.rows > 128 ? 2 : 1;
-                        const int pos1 = min(w.pos0 + tile_pos, t.len) - 1;
-                        w.steps = t.some ? pos1 / kStep + 1 : 0;
-                        loads = (w.steps + 1) / 2 * 2;
-                        w.last = (pos1 % kStep + 16) / 16 * 16;
-                        w.first_masked = (w.pos0 + 1) / kStep;
-                        w.dirty = 0;
-                        tile_s[n & 1] = w;
-                        mbar_arrive(&bars.tile_full[n & 1]);
-                    }
-                    if (ok) {
-                        const int x = kvh * kD;
-                        for (int j = 0; j < loads; ++j, ++item) {
-                            const int st = item % kStages;
-                            if (!(ok = wait(&bars.empty[st], ((item / kStages) & 1) ^ 1))) break;
-                            uint8_t* dst = kv_s + st * kTileBytes;
-                            const int y = t.first + j / 2 * kKeys;
-                            mbar_arrive_expect_tx(&bars.full[st], kTileBytes);
-                            const CUtensorMap* map = (j & 1) ? &vmap : &kmap;
-                            tma_load_2d(map, &bars.full[st], dst, x, y);
-                            tma_load_2d(map, &bars.full[st], dst + kHalf, x + 64, y);
-                        }
-                    }
-                    if (!ok)   // loads in flight land before the block leaves
-                        for (int i = max(item - kStages, 0); i < item; ++i) mbar_drain(&bars.full[i % kStages], (i / kStages) & 1);
-                }
-                ok = __shfl_sync(0xffffffffu, ok, 0) && t.some;
-            }
-        } else if (warp == 8) {
-            // ---- MMA issue, by the whole warp
-            const bool el = lane == 0;
-            auto uni = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };       // uniform for the compiler as well
-            auto all = [&](bool x) { return __all_sync(0xffffffffu, x); };
-            const uint32_t negate = p.flip_q ? 1u << 13 : 0u;      // of A
-            constexpr uint32_t id_o = idesc_bf16_f32(128, kD, true);
-            const uint32_t tm = uni(tmem);
-            const uint32_t q_lo = desc_lo_k(smem_u32(q_s)), k_lo = desc_lo_k(smem_u32(kv_s)), v_lo = desc_lo_mn(smem_u32(kv_s), kHalf);
-            int item = 0, stage = 0;                    // ring items so far, and their stage
-            uint32_t p_phase = 0;                       // of p_full[t][b], bit 2 t + b
-            int masked = 0;
-            auto stage_of = [&](int ahead) { return (stage + ahead) % kStages; };
-            auto wait_item = [&](int ahead) {
-                return all(wait(&bars.full[stage_of(ahead)], ((item + ahead) / kStages) & 1));
-            };
-            bool ok = true;
-            for (int n = 0; ok; ++n) {
-                if (!(ok = all(wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
-                const TileWork& slot = tile_s[n & 1];
-                if (!uni(slot.some)) break;
-                const int steps = uni(slot.steps), mt = uni(slot.mt), last = uni(slot.last), first_masked = uni(slot.first_masked);
-                int k_at = 0;                           // K item of the scores issued next, from the tile's first
-                // S_t of step j into buffer j % 2; what the last M tile's scores are the last to read is free after them
-                auto scores = [&](int t, int j) {
-                    const int st = stage_of(k_at);
-                    const uint32_t id_s = idesc_bf16_f32(128, j + 1 == steps ? last : kStep, false) | negate;
-                    const uint32_t q = q_lo + t * (kHalf >> 4), k = k_lo + st * (kTileBytes >> 4) + (j & 1) * (kStep * 128 >> 4);
-                    const uint32_t d = tm + t * 128 + (j & 1) * kStep;
-#pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)
-                        umma_f16_warp(d, q + (ks >> 2) * (2 * kHalf >> 4) + (ks & 3) * 2, k + (ks >> 2) * (kHalf >> 4) + (ks & 3) * 2,
-                                      id_s, ks > 0);
-                    umma_commit_warp(&bars.s_full[t][j & 1]);
-                    if (t == mt - 1 && ((j & 1) || j + 1 == steps)) {
-                        umma_commit_warp(&bars.empty[st]);
-                        k_at += 2;
-                        if (j + 1 == steps) umma_commit_warp(&bars.q_empty);
-                    }
-                };
-                if (!(ok = all(wait(&bars.q_full, n & 1)) && wait_item(0))) break;
-                tc_fence_after();
-                for (int j = 0; j < 2 && j < steps; ++j)
-                    for (int t = 0; t < mt; ++t) scores(t, j);
-                if (!(ok = wait_item(1))) break;
-                bool ready = false;                     // what a test for the next weights gave, under the MMAs before
-                for (int j = 0; j < steps && ok; ++j) {
-                    const int st = stage_of(j / 2 * 2 + 1);
-                    const bool clean = j >= first_masked;
-                    if (clean && el) mbar_arrive(&bars.go);
-                    const uint32_t v = v_lo + st * (kTileBytes >> 4) + (j & 1) * (kStep * 128 >> 4);
-                    const int ksteps = j + 1 == steps ? last / 16 : kStep / 16;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        if (t >= mt || !ok) break;
-                        const int bit = 2 * t + (j & 1);
-                        if (!all(ready) && !(ok = all(wait(&bars.p_full[t][j & 1], (p_phase >> bit) & 1)))) break;
-                        p_phase ^= 1u << bit;
-                        if (t == 0 && clean && !(ok = all(wait(&bars.clean, masked++ & 1)))) break;
-                        tc_fence_after();
-                        const uint32_t pa = tm + t * 128 + (j & 1) * kStep;
-#pragma unroll
-                        for (int ks = 0; ks < kStep / 16; ++ks)     // 16 keys: 16 rows of 128 bytes
-                            if (ks < ksteps)
-                                umma_f16_ta_warp(tm + 256 + t * 128, pa + ks * 8, v + ks * (2048 >> 4), id_o, j > 0 || ks > 0);
-                        umma_commit_warp(&bars.pv_done[t]);
-                        if (j + 1 == steps) {
-                            if (el) mbar_arrive(&bars.o_full[t]);   // the cleaner's word on the tile goes with it
-                            umma_commit_warp(&bars.o_full[t]);
-                        }
-                        if (t == mt - 1 && ((j & 1) || j + 1 == steps)) umma_commit_warp(&bars.empty[st]);
-                        // K of step j + 2, and V for its product
-                        if (t == 0 && !(j & 1) && j + 2 < steps && !(ok = wait_item(k_at) && wait_item(k_at + 1))) break;
-                        const int nt = t + 1 < mt ? t + 1 : 0, nb = (t + 1 < mt ? j : j + 1) & 1;
-                        ready = mbar_test(&bars.p_full[nt][nb], (p_phase >> (2 * nt + nb)) & 1);
-                        if (j + 2 < steps) scores(t, j + 2);
-                    }
-                }
-                const int used = (steps + 1) / 2 * 2;
-                item += used;
-                stage = (stage + used) % kStages;
-                if (el) mbar_arrive(&bars.tile_empty[n & 1]);
-            }
-            if (!ok) {
-                umma_commit_warp(&bars.drain);
-                mbar_drain(&bars.drain, 0);
-            }
-        } else if (warp == 10 && lane == 0) {
-            // ---- Q: the heads of the group at tile_pos positions, [half][rows][128 B]
-            bool ok = true;
-            int loads = 0;
-            for (int n = 0; ok; ++n) {
-                if (!(ok = wait(&bars.tile_full[n & 1], (n >> 1) & 1))) break;
-                const TileWork w = tile_s[n & 1];
-                if (!w.some) break;
-                if (!(ok = wait(&bars.q_empty, (n & 1) ^ 1))) break;
-                mbar_arrive_expect_tx(&bars.q_full, tile_pos * p.G * 256);
-                tma_load_3d(&qmap, &bars.q_full, q_s, 0, w.kvh * p.G, w.first + w.pos0);
-                tma_load_3d(&qmap, &bars.q_full, q_s + 2 * kHalf, 64, w.kvh * p.G, w.first + w.pos0);
-                mbar_arrive(&bars.tile_empty[n & 1]);
-                ++loads;
-            }
-            if (!ok && loads) mbar_drain(&bars.q_full, (loads - 1) & 1);
-        } else if (warp == 11) {
-            // ---- a weight of 0 must meet a finite value: V of positions that not every row attends
-            int masked = 0, item = 0;
-            bool ok = true;
-            for (int n = 0; ok; ++n) {
-                if (!(ok = __all_sync(0xffffffffu, wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
-                const TileWork w = tile_s[n & 1];
-                if (!w.some) break;
-                for (int i = w.first_masked; i < w.steps && ok; ++i) {
-                    const int vi = item + i / 2 * 2 + 1;
-                    ok = wait(&bars.go, masked++ & 1) && wait(&bars.full[vi % kStages], (vi / kStages) & 1);
-                    if (!(ok = __all_sync(0xffffffffu, ok))) break;
-                    uint8_t* v = kv_s + vi % kStages * kTileBytes + (i & 1) * (kStep * 128);
-                    const int j0 = max(w.pos0 + 1 - i * kStep, 0);       // first such row of the step
-                    const int j1 = i + 1 == w.steps ? w.last : kStep;
-                    bool dirty = false;
-#pragma unroll 8
-                    for (int c = lane; c < (j1 - j0) * 16; c += 32) {
-                        uint4* at = reinterpret_cast<uint4*>(v + (c & 1) * kHalf + (j0 + (c >> 4)) * 128 + ((c >> 1) & 7) * 16);
-                        uint4 x = *at;
-                        if (zero_nonfinite(x)) {
-                            *at = x;
-                            dirty = true;
-                        }
-                    }
-                    if (dirty) tile_s[n & 1].dirty = 1;
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    mbar_arrive(&bars.clean);
-                }
-                item += (w.steps + 1) / 2 * 2;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars.tile_empty[n & 1]);
-            }
-        }
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    if (warp < 8) {
+        // ---- softmax
         const int t = warp >> 2;
         const int i_row = threadIdx.x;
         const uint32_t ts = tmem + (static_cast<uint32_t>(warp & 3) << 21) + t * 128;   // this warp's 32 lanes
         const uint32_t to = ts + 256;
         const float sl2 = p.scale_log2;
         uint32_t s_phase = 0;                           // of s_full[t][b], bit b
-        int pv_n = 0, o_n = 0;                          // steps and tiles of this M tile so far
+        int pv_n = 0, tiles = 0;                        // steps and tiles of this M tile so far
         bool ok = true;
         for (int n = 0; ok; ++n) {
-            if (!(ok = __all_sync(0xffffffffu, wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
-            const TileWork w = tile_s[n & 1];
+            if (!(ok = all(wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
+            const TileWork& w = tile_s[n & 1];
             if (!w.some) break;
             if (t < w.mt) {
-                const int at = group_div(min(i_row, w.rows - 1), g_inv);
-                const int pos = w.pos0 + at;
+                const int steps = w.steps, first_masked = w.first_masked;
+                const int pos = w.pos0 + group_div(min(i_row, w.rows - 1), g_inv);
                 float m = -INFINITY, l = 0.0f;
-                for (int j = 0; j < w.steps; ++j, ++pv_n) {
+                for (int j = 0; j < steps; ++j, ++pv_n) {
                     const uint32_t sb = ts + (j & 1) * kStep;
-                    if (!(ok = __all_sync(0xffffffffu, wait(&bars.s_full[t][j & 1], (s_phase >> (j & 1)) & 1)))) break;
+                    if (!(ok = all(wait(&bars.s_full[t][j & 1], (s_phase >> (j & 1)) & 1)))) break;
                     s_phase ^= 1u << (j & 1);
                     tc_fence_after();
                     uint32_t s[2][32];
 #pragma unroll
                     for (int c = 0; c < 2; ++c) tmem_ld32(sb + 32 * c, s[c]);
                     tmem_wait_ld();
-                    if (j >= w.first_masked) {
+                    if (j >= first_masked) {
                         const int lim = pos - j * kStep;
 #pragma unroll
                         for (int c = 0; c < 2; ++c)
@@ -469,32 +358,33 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                             for (int e = 0; e < 32; ++e)
                                 if (32 * c + e > lim) s[c][e] = 0xFF800000u;
                     }
-                    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    // a NaN score makes the maximum NaN, and with it the row
+                    float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                     for (int e = 0; e < 32; e += 2)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c)
-                            mx[c] = fmaxf(mx[c], __uint_as_float(s[c >> 1][e + (c & 1)]));
-                    const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                        for (int c = 0; c < 2; ++c)
+                            mx[c] = max3_nan(mx[c], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
+                    const float mt = max3_nan(mx[0], mx[1], -INFINITY);
                     if (j == 0) {
                         m = mt;
                     } else {
-                        const bool need = (mt - m) * sl2 > 8.0f;
+                        const bool need = !((mt - m) * sl2 <= 8.0f) && mt != m;
                         if (__any_sync(0xffffffffu, need)) {
                             const float f = need ? ex2((m - mt) * sl2) : 1.0f;
                             l *= f;
                             if (need) m = mt;
                             // the product of the step before has to be in
-                            if (!(ok = __all_sync(0xffffffffu, wait(&bars.pv_done[t], (pv_n - 1) & 1)))) break;
+                            if (!(ok = all(wait(&bars.pv_done[t], (pv_n - 1) & 1)))) break;
                             tc_fence_after();
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                uint32_t o[32];
-                                tmem_ld32(to + 32 * c, o);
+#pragma unroll 1
+                            for (int c = 0; c < 8; ++c) {
+                                uint32_t o[16];
+                                tmem_ld16(to + 16 * c, o);
                                 tmem_wait_ld();
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                                tmem_st32(to + 32 * c, o);
+                                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                tmem_st16(to + 16 * c, o);
                             }
                         }
                     }
@@ -507,8 +397,12 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                         for (int e = 0; e < 16; ++e) {
                             float2 x = ffma2(make_float2(__uint_as_float(s[c][2 * e]), __uint_as_float(s[c][2 * e + 1])),
                                              make_float2(sl2, sl2), make_float2(nm, nm));
-                            x.x = ex2(x.x);
-                            x.y = ex2(x.y);
+                            if (e % 8 < kFmaPairs) {
+                                x = ex2_fma(x);
+                            } else {
+                                x.x = ex2(x.x);
+                                x.y = ex2(x.y);
+                            }
                             sum[e & 1] = fadd2(sum[e & 1], x);
                             wt[e] = pack_bf16(x.x, x.y);    // the weights' rounding, 2^-8 at most; the sum has them whole
                         }
@@ -516,55 +410,66 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     }
                     sum[0] = fadd2(sum[0], sum[1]);
                     l += sum[0].x + sum[0].y;
+                    if (j + 1 == steps) {               // goes to the epilogue with the last weights
+                        if (tiles && !(ok = all(wait(&bars.o_free[t], (tiles - 1) & 1)))) break;   // it has the last tile's
+                        l_s[i_row] = l;
+                    }
                     tmem_wait_st();
                     tc_fence_before();
                     mbar_arrive(&bars.p_full[t][j & 1]);
                 }
-                if (ok) ok = __all_sync(0xffffffffu, wait(&bars.o_full[t], o_n++ & 1));
-                if (!ok) break;
+                ++tiles;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.tile_empty[n & 1]);
+        }
+    } else if (warp < 12) {
+        // ---- epilogue
+        int tiles[2] = {0, 0};
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+            if (!(ok = all(wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
+            const TileWork& w = tile_s[n & 1];
+            if (!w.some) break;
+            const int rows = w.rows, pos0 = w.pos0, kvh = w.kvh;
+            const long long first = w.first;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (t >= w.mt || !ok) break;
+                const int i_row = t * 128 + (threadIdx.x & 127);
+                const uint32_t to = tmem + (static_cast<uint32_t>(warp & 3) << 21) + 256 + t * 128;
+                if (!(ok = all(wait(&bars.o_full[t], tiles[t]++ & 1)))) break;
                 tc_fence_after();
-                const bool dirty = *static_cast<volatile int*>(&tile_s[n & 1].dirty) != 0;
-                const float inv = 1.0f / l;
-                const long long row = w.first + pos;
-                const int head = w.kvh * p.G + min(i_row, w.rows - 1) - at * p.G;
-                __nv_bfloat16* orow = p.out + (row * p.nq + head) * kD;
-                const __nv_bfloat16* vrow = p.v + static_cast<long long>(w.first) * p.v_stride + w.kvh * kD;
-                const bool store = i_row < w.rows;
+                const float inv = 1.0f / l_s[i_row];
+                const bool dirty = *static_cast<volatile const int*>(&w.dirty) != 0;
+                const int at = group_div(min(i_row, rows - 1), g_inv);
+                const int pos = pos0 + at;
+                const int head = kvh * p.G + min(i_row, rows - 1) - at * p.G;
+                const bool store = i_row < rows;
+                const long long out_row = (first + pos) * p.nq + head;
+                if (dirty) {
+                    epilogue_dirty(p, to, inv, first, pos0, pos, kvh, head, store);
+                    tc_fence_before();
+                    mbar_arrive(&bars.o_free[t]);
+                    continue;
+                }
                 auto columns = [&](int c, float (&x)[32]) {     // 32 dims of the row
                     uint32_t o[32];
                     tmem_ld32(to + 32 * c, o);
                     tmem_wait_ld();
 #pragma unroll
                     for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(o[e]) * inv;
-                    if (dirty)                          // the values zeroed above, for the rows that attend them
-                        for (int j = w.pos0 + 1; j <= pos; ++j) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const float y = __bfloat162float(vrow[j * p.v_stride + 32 * c + e]);
-                                if (!isfinite(y)) x[e] += y;
-                            }
-                        }
                 };
-                float amax = 0.0f;
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    float x[32];
-                    columns(c, x);
-                    uint32_t wt[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        amax = fmaxf(amax, fmaxf(fabsf(x[2 * e]), fabsf(x[2 * e + 1])));
-                        wt[e] = pack_bf16(x[2 * e], x[2 * e + 1]);
-                    }
-                    if (store)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            *reinterpret_cast<uint4*>(orow + 32 * c + 8 * e) =
-                                make_uint4(wt[4 * e], wt[4 * e + 1], wt[4 * e + 2], wt[4 * e + 3]);
-                }
                 if (p.out_q) {
+                    float amax = 0.0f;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        float x[32];
+                        columns(c, x);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) amax = fmaxf(amax, fabsf(x[e]));
+                    }
                     const float qi = amax > 0.0f ? 448.0f / amax : 0.0f;
-                    uint8_t* qrow = p.out_q + (row * p.nq + head) * kD;
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         float x[32];
@@ -575,22 +480,227 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                             wt[e] = amax > 0.0f ? cvt_e4m3x2(x[4 * e] * qi, x[4 * e + 1] * qi) |
                                                       static_cast<uint32_t>(cvt_e4m3x2(x[4 * e + 2] * qi, x[4 * e + 3] * qi)) << 16
                                                 : 0u;
-                        if (store)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                *reinterpret_cast<uint4*>(qrow + 32 * c + 16 * e) =
-                                    make_uint4(wt[4 * e], wt[4 * e + 1], wt[4 * e + 2], wt[4 * e + 3]);
+                        if (store) st_global_32(p.out_q + out_row * kD + 32 * c, wt);
                     }
-                    if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + row] = amax > 0.0f ? amax / 448.0f : 0.0f;
+                    if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
+                }
+                uint32_t wt[4][16];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float x[32];
+                    columns(c, x);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) wt[c][e] = pack_bf16(x[2 * e], x[2 * e + 1]);
                 }
                 tc_fence_before();
+                mbar_arrive(&bars.o_free[t]);           // the next tile may write its output
+                if (store)                              // whole 32-byte sectors
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) st_global_32(p.out + out_row * kD + 32 * c + 16 * e, wt[c] + 8 * e);
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.tile_empty[n & 1]);
+        }
+    } else if (warp < 14) {
+        // ---- MMA issue, by a whole warp for M tile t
+        const int t = warp - 12;
+        const bool el = lane == 0;
+        auto uni = [](int x) { return __shfl_sync(0xffffffffu, x, 0); };       // uniform for the compiler as well
+        const uint32_t negate = p.flip_q ? 1u << 13 : 0u;      // of A
+        constexpr uint32_t id_o = idesc_bf16_f32(128, kD, true);
+        const uint32_t tm = uni(tmem) + t * 128;
+        const uint32_t q_lo = desc_lo_k(smem_u32(q_s)) + t * (kHalf >> 4);
+        const uint32_t k_lo = desc_lo_k(smem_u32(kv_s)), v_lo = desc_lo_mn(smem_u32(kv_s), kHalf);
+        int item = 0, stage = 0;                        // ring items of the tiles before, and their stage
+        int tiles = 0, masked = 0;                      // tiles of this M tile, masked steps of all tiles
+        uint32_t p_phase = 0;                           // of p_full[t][b], bit b
+        auto stage_of = [&](int ahead) { return (stage + ahead) % kStages; };
+        auto wait_item = [&](int ahead) { return all(wait(&bars.full[stage_of(ahead)], ((item + ahead) / kStages) & 1)); };
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+            if (!(ok = all(wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
+            const TileWork& slot = tile_s[n & 1];
+            if (!uni(slot.some)) break;
+            const int steps = uni(slot.steps), last = uni(slot.last), first_masked = uni(slot.first_masked);
+            const bool active = t < uni(slot.mt);
+            if (!active) {
+                // the other M tile has it alone: this warp only keeps the counts of the barriers that both arrive on
+                for (int i = 0; i < (steps + 1) / 2 * 2 && ok; ++i) {
+                    if (!(ok = wait_item(i))) break;
+                    if (el) mbar_arrive(&bars.empty[stage_of(i)]);
+                    for (int j = i - 1; (i & 1) && j <= i && ok; ++j)      // the steps of V item i
+                        if (j < steps && j >= first_masked) {
+                            if (el) mbar_arrive(&bars.go);
+                            ok = all(wait(&bars.clean, masked++ & 1));
+                        }
+                }
+                if (ok && !(ok = all(wait(&bars.q_full, n & 1)))) break;
+                if (el) mbar_arrive(&bars.q_empty);
+            } else {
+                int k_at = 0;                           // K item of the scores issued next, from the tile's first
+                auto scores = [&](int j) {              // S of step j into buffer j % 2
+                    const int st = stage_of(k_at);
+                    const uint32_t id_s = idesc_bf16_f32(128, j + 1 == steps ? last : kStep, false) | negate;
+                    const uint32_t k = k_lo + st * (kTileBytes >> 4) + (j & 1) * (kStep * 128 >> 4);
+                    const uint32_t d = tm + (j & 1) * kStep;
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks)
+                        umma_f16_warp(d, q_lo + (ks >> 2) * (2 * kHalf >> 4) + (ks & 3) * 2,
+                                      k + (ks >> 2) * (kHalf >> 4) + (ks & 3) * 2, id_s, ks > 0);
+                    umma_commit_warp(&bars.s_full[t][j & 1]);
+                    if ((j & 1) || j + 1 == steps) {
+                        umma_commit_warp(&bars.empty[st]);
+                        k_at += 2;
+                        if (j + 1 == steps) umma_commit_warp(&bars.q_empty);
+                    }
+                };
+                if (!(ok = all(wait(&bars.q_full, n & 1)) && wait_item(0))) break;
+                tc_fence_after();
+                scores(0);
+                if (steps > 1) scores(1);
+                if (!(ok = wait_item(1) && all(wait(&bars.o_free[t], (tiles++ & 1) ^ 1)))) break;
+                bool ready = false;                     // what a test for the next weights gave, under the MMAs before
+                for (int j = 0; j < steps; ++j) {
+                    const int st = stage_of(j / 2 * 2 + 1);
+                    const bool clean = j >= first_masked;
+                    if (clean && el) mbar_arrive(&bars.go);
+                    if (!all(ready) && !(ok = all(wait(&bars.p_full[t][j & 1], (p_phase >> (j & 1)) & 1)))) break;
+                    p_phase ^= 1u << (j & 1);
+                    if (clean && !(ok = all(wait(&bars.clean, masked++ & 1)))) break;
+                    tc_fence_after();
+                    const uint32_t v = v_lo + st * (kTileBytes >> 4) + (j & 1) * (kStep * 128 >> 4);
+                    const uint32_t pa = tm + (j & 1) * kStep;
+                    const int ksteps = j + 1 == steps ? last / 16 : kStep / 16;
+#pragma unroll
+                    for (int ks = 0; ks < kStep / 16; ++ks)     // 16 keys: 16 rows of 128 bytes
+                        if (ks < ksteps) umma_f16_ta_warp(tm + 256, pa + ks * 8, v + ks * (2048 >> 4), id_o, j > 0 || ks > 0);
+                    umma_commit_warp(&bars.pv_done[t]);
+                    if (j + 1 == steps) {
+                        if (el) mbar_arrive(&bars.o_full[t]);   // the cleaner's word on the tile and the row sums go with it
+                        umma_commit_warp(&bars.o_full[t]);
+                    }
+                    if ((j & 1) || j + 1 == steps) umma_commit_warp(&bars.empty[st]);
+                    if (j + 2 < steps) {
+                        if (!(j & 1) && !(ok = wait_item(k_at) && wait_item(k_at + 1))) break;     // K of step j + 2, V for its product
+                        ready = mbar_test(&bars.p_full[t][(j + 1) & 1], (p_phase >> ((j + 1) & 1)) & 1);
+                        scores(j + 2);
+                    } else {
+                        ready = false;
+                    }
+                }
+            }
+            const int used = (steps + 1) / 2 * 2;
+            item += used;
+            stage = (stage + used) % kStages;
+            if (el) mbar_arrive(&bars.tile_empty[n & 1]);
+        }
+        if (!ok) {
+            umma_commit_warp(&bars.drain[t]);
+            mbar_drain(&bars.drain[t], 0);
+        }
+    } else if (warp == 14) {
+        // ---- tiles; Q, and K and V of keys 0.., 128.. of every tile
+        const TileOrder order(p, tile_pos, blockIdx.x == 0);
+        int item = 0, q_n = 0;
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+            // every other round backwards: a CTA's tiles even out
+            const unsigned int c = n * gridDim.x + ((n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            const Tile tl = order.find(c / p.nkv);
+            const int kvh = static_cast<int>(c % p.nkv);
+            if (lane == 0) {
+                ok = wait(&bars.tile_empty[n & 1], ((n >> 1) & 1) ^ 1);
+                int loads = 0, pos0 = 0;
+                if (ok) {
+                    TileWork w;
+                    w.some = tl.some;
+                    w.kvh = kvh;
+                    w.first = tl.first;
+                    w.pos0 = pos0 = tl.index * tile_pos;
+                    w.rows = min(tile_pos, tl.len - w.pos0) * p.G;
+                    w.mt = w.rows > 128 ? 2 : 1;
+                    const int pos1 = min(w.pos0 + tile_pos, tl.len) - 1;
+                    w.steps = tl.some ? pos1 / kStep + 1 : 0;
+                    w.last = (pos1 % kStep + 16) / 16 * 16;
+                    w.first_masked = (w.pos0 + 1) / kStep;
+                    w.dirty = 0;
+                    loads = (w.steps + 1) / 2 * 2;
+                    tile_s[n & 1] = w;
+                    mbar_arrive(&bars.tile_full[n & 1]);
+                }
+                const int x = kvh * kD;
+                for (int j = 0; j < loads && ok; ++j) {
+                    if (j == (n ? 2 : 0)) {             // behind the first K and V, which need not wait for the last tile's Q
+                        if (!(ok = wait(&bars.q_empty, (n & 1) ^ 1))) break;
+                        mbar_arrive_expect_tx(&bars.q_full, tile_pos * p.G * 256);
+                        tma_load_3d(&qmap, &bars.q_full, q_s, 0, kvh * p.G, tl.first + pos0);
+                        tma_load_3d(&qmap, &bars.q_full, q_s + 2 * kHalf, 64, kvh * p.G, tl.first + pos0);
+                        ++q_n;
+                    }
+                    const int st = item % kStages;
+                    if (!(ok = wait(&bars.empty[st], ((item / kStages) & 1) ^ 1))) break;
+                    uint8_t* dst = kv_s + st * kTileBytes;
+                    const int y = tl.first + j / 2 * kKeys;
+                    mbar_arrive_expect_tx(&bars.full[st], kTileBytes);
+                    const CUtensorMap* map = (j & 1) ? &vmap : &kmap;
+                    tma_load_2d(map, &bars.full[st], dst, x, y);
+                    tma_load_2d(map, &bars.full[st], dst + kHalf, x + 64, y);
+                    ++item;
+                }
+                if (ok && n && loads == 2) {            // no item behind the first K and V
+                    if ((ok = wait(&bars.q_empty, (n & 1) ^ 1))) {
+                        mbar_arrive_expect_tx(&bars.q_full, tile_pos * p.G * 256);
+                        tma_load_3d(&qmap, &bars.q_full, q_s, 0, kvh * p.G, tl.first + pos0);
+                        tma_load_3d(&qmap, &bars.q_full, q_s + 2 * kHalf, 64, kvh * p.G, tl.first + pos0);
+                        ++q_n;
+                    }
+                }
+                if (!ok) {   // loads in flight land before the block leaves
+                    for (int i = max(item - kStages, 0); i < item; ++i) mbar_drain(&bars.full[i % kStages], (i / kStages) & 1);
+                    if (q_n) mbar_drain(&bars.q_full, (q_n - 1) & 1);
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 0) && tl.some;
+        }
+    } else {
+        // ---- a weight of 0 must meet a finite value: V of positions that not every row attends
+        int masked = 0, item = 0;
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+            if (!(ok = all(wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
+            TileWork& w = tile_s[n & 1];
+            if (!w.some) break;
+            const int steps = w.steps;
+            for (int i = w.first_masked; i < steps; ++i) {
+                const int vi = item + i / 2 * 2 + 1;
+                ok = wait(&bars.go, masked++ & 1) && wait(&bars.full[vi % kStages], (vi / kStages) & 1);
+                if (!(ok = all(ok))) break;
+                uint8_t* v = kv_s + vi % kStages * kTileBytes + (i & 1) * (kStep * 128);
+                const int j0 = max(w.pos0 + 1 - i * kStep, 0);       // first such row of the step
+                const int j1 = i + 1 == steps ? w.last : kStep;
+                bool dirty = false;
+#pragma unroll 8
+                for (int c = lane; c < (j1 - j0) * 16; c += 32) {
+                    uint4* at = reinterpret_cast<uint4*>(v + (c & 1) * kHalf + (j0 + (c >> 4)) * 128 + ((c >> 1) & 7) * 16);
+                    uint4 x = *at;
+                    if (zero_nonfinite(x)) {
+                        *at = x;
+                        dirty = true;
+                    }
+                }
+                if (dirty) w.dirty = 1;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&bars.clean);
+            }
+            item += (steps + 1) / 2 * 2;
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.tile_empty[n & 1]);
         }
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 12) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
@@ -653,8 +763,9 @@ moe_status_t attn_prompt_packed(const void* q_bf16, long long q_stride, const vo
         return MOE_ERR_INVALID_ARGUMENT;
     if (T == 0 || num_seqs == 0) return MOE_OK;
     if (!q_bf16 || !k_bf16 || !v_bf16 || !cu_seqlens || !out_bf16) return MOE_ERR_INVALID_ARGUMENT;
-    if (!a16(q_bf16) || !a16(k_bf16) || !a16(v_bf16) || !a16(out_bf16)) return MOE_ERR_INVALID_ARGUMENT;
-    if (out_q && (!out_s || out_ld < T || !a16(out_q))) return MOE_ERR_INVALID_ARGUMENT;
+    auto a32 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 31) == 0; };
+    if (!a16(q_bf16) || !a16(k_bf16) || !a16(v_bf16) || !a32(out_bf16)) return MOE_ERR_INVALID_ARGUMENT;
+    if (out_q && (!out_s || out_ld < T || !a32(out_q))) return MOE_ERR_INVALID_ARGUMENT;
     PromptParams p;
     p.q = static_cast<const __nv_bfloat16*>(q_bf16);
     p.k = static_cast<const __nv_bfloat16*>(k_bf16);
