@@ -174,16 +174,23 @@ kv4_read_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__
 }
 
 // ---------------------------------------------------------------- decode
+//
+// One CTA per (context split, row x kv head), four warps that take two pages at
+// a time from bulk-copied rings of their own: codes to fragments with the fma of
+// the file's head, S = Q K^T and O += P V on mma.sync with the group's query
+// heads as M, one online softmax whose maximum is left behind by up to 2^8.
 
 constexpr int kWarps = 4;
-constexpr int kNst = 4;                                   // pages in flight per warp
-constexpr int kStage = 2 * kPage4;                        // K and V tile of one page
+constexpr int kNst = 3;                                   // page pairs in flight per warp
+constexpr int kTile = 2 * kPage4;                         // K and V of one page
+constexpr int kStage = 2 * kTile;
 constexpr int kMaxSplitPages = 512;                       // split_tokens <= 8192
 constexpr int kMergePad = kD + 4;
 constexpr size_t kRingBytes = static_cast<size_t>(kWarps) * kNst * kStage;
 constexpr size_t kDecodeSmem = kRingBytes + kMaxSplitPages * 4;
-// the warp merge reuses the rings: per warp 16 x 128 fp32 and 16 (m, l)
-static_assert(static_cast<size_t>(kWarps) * kGPad * (kMergePad + 2) * 4 <= kRingBytes, "merge scratch fits the rings");
+constexpr uint64_t kWaitNs = 2000000000ull;
+// the warp merge reuses the rings: per warp 16 x 128 fp32, then (m, l) and factors of its rows
+static_assert(static_cast<size_t>(kWarps) * kGPad * (kMergePad + 3) * 4 + kGPad * 8 <= kRingBytes, "merge scratch fits the rings");
 
 struct Kv4Params {
     const __nv_bfloat16* q;
@@ -195,8 +202,13 @@ struct Kv4Params {
     float* part_o;                 // [B * nkv][max_splits][G][128]
     float* part_ml;                // [B * nkv][max_splits][G][2]
     int* error_word;
+    __nv_bfloat16* out;            // [B][nq][128]
+    uint8_t* out_q;
+    float* out_s;
+    int out_ld;
     int nq, nkv, G, max_pages, num_cache_pages, split_tokens, max_splits, num_seqs;
-    float scale_log2;
+    float scale_log2;              // at least FLT_MIN: a sign is taken by the queries
+    uint32_t q_flip;               // 0x80008000 for a negative scale
 };
 
 __device__ __forceinline__ int clamp_len(int len, int max_pages, int split_tokens, int max_splits) {
@@ -221,22 +233,45 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {
     return ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
 }
 
+// One output row (128 threads, one dim each): bf16, and e4m3 with its scale.
+__device__ __forceinline__ void write_row(const Kv4Params& p, int b, int h, float v, float* red) {
+    const int d = threadIdx.x;
+    p.out[(static_cast<size_t>(b) * p.nq + h) * kD + d] = __float2bfloat16_rn(v);
+    if (p.out_q) {
+        float a = fabsf(v);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+        __syncthreads();
+        if ((d & 31) == 0) red[d >> 5] = a;
+        __syncthreads();
+        const float amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        uint8_t qv = 0;
+        if (amax > 0.0f) qv = static_cast<uint8_t>(cvt_e4m3x2(v * (448.0f / amax), 0.0f) & 0xFFu);
+        p.out_q[(static_cast<size_t>(b) * p.nq + h) * kD + d] = qv;
+        if (d == 0) p.out_s[static_cast<size_t>(h) * p.out_ld + b] = amax > 0.0f ? amax / 448.0f : 0.0f;
+    }
+}
+
 __global__ void __launch_bounds__(kWarps * 32, 3)
 kv4_decode_kernel(const Kv4Params p) {
     extern __shared__ __align__(128) uint8_t sm[];
+    __shared__ uint64_t full[kWarps][kNst];
+    __shared__ int abort_s;
+    __shared__ float red[kWarps];
     const int split = blockIdx.x;
     const int bk = blockIdx.y;
     const int b = bk / p.nkv, kvh = bk % p.nkv;
     const int seq = seq_of_row(p.row_seq, b, p.num_seqs);
-    if (seq < 0) {
-        if (split == 0 && threadIdx.x == 0 && kvh == 0 && p.error_word) atomicExch(p.error_word, 7);
-        return;
-    }
-    const int len_in = p.seq_lens[b];
+    if (seq < 0 && split == 0 && threadIdx.x == 0 && kvh == 0 && p.error_word) atomicExch(p.error_word, 7);
+    const int len_in = seq < 0 ? 0 : p.seq_lens[b];
     const int len = clamp_len(len_in, p.max_pages, p.split_tokens, p.max_splits);
     if (len < len_in && split == 0 && threadIdx.x == 0 && kvh == 0 && p.error_word) atomicExch(p.error_word, 5);
     const int t0 = split * p.split_tokens;
-    if (t0 >= len) return;
+    if (t0 >= len) {
+        if (p.max_splits == 1)                     // there is no merge kernel: an empty row's zeros
+            for (int r = 0; r < p.G; ++r) write_row(p, b, kvh * p.G + r, 0.0f, red);
+        return;
+    }
     const int t1 = min(t0 + p.split_tokens, len);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, tq = lane & 3;
@@ -254,6 +289,9 @@ kv4_decode_kernel(const Kv4Params p) {
             pid_s[i] = ok ? phys : -1;
         }
     }
+    if (lane < kNst) mbar_init(&full[warp][lane], 1);
+    if (threadIdx.x == 0) abort_s = 0;
+    fence_mbar_init();
     // Query fragments: MMA k-step 2j + u takes dims 32 j + 8 tq + {2u, 2u + 4, 2u + 1, 2u + 5} at this lane's
     // four contraction indices, the order the K codes unpack in.
     uint32_t qa[kD / 16][4];
@@ -266,6 +304,7 @@ kv4_decode_kernel(const Kv4Params p) {
             for (int j = 0; j < kGroups; ++j) {
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (r < p.G) v = *reinterpret_cast<const uint4*>(q0 + static_cast<size_t>(r) * kD + 32 * j + 8 * tq);
+                v.x ^= p.q_flip; v.y ^= p.q_flip; v.z ^= p.q_flip; v.w ^= p.q_flip;
                 // v: dims 0 1 | 2 3 | 4 5 | 6 7
                 qa[2 * j][h] = __byte_perm(v.x, v.z, 0x5410);          // 0, 4
                 qa[2 * j][2 + h] = __byte_perm(v.x, v.z, 0x7632);      // 1, 5
@@ -276,17 +315,28 @@ kv4_decode_kernel(const Kv4Params p) {
     }
     __syncthreads();
 
-    const int my_pages = npages > warp ? (npages - warp + kWarps - 1) / kWarps : 0;
-    auto load_page = [&](int i, int stage) {
-        int phys = pid_s[warp + i * kWarps];
-        const uint32_t nbytes = phys >= 0 ? 16u : 0u;     // a bad page reads as zero scales: zeros
-        phys = phys >= 0 ? phys : 0;
-        const size_t off = (static_cast<size_t>(phys) * p.nkv + kvh) * kPage4;
+    // Pairs of pages, dealt to the warps in turn.
+    const int npairs = (npages + 1) / 2;
+    const int mine = npairs > warp ? (npairs - warp + kWarps - 1) / kWarps : 0;
+    // Lanes 0-3 copy K and V of the pair's two pages; a page that is not there (an id outside the cache, or none behind
+    // the last) reads as zeros: scales of 0.
+    auto load_pair = [&](int i, int stage) {
         uint8_t* dst = ring + stage * kStage;
-        for (int c = lane; c < kStage / 16; c += 32) {
-            const uint8_t* src = c < kPage4 / 16 ? p.k_cache + off + c * 16 : p.v_cache + off + (c * 16 - kPage4);
-            cp_async16(dst + c * 16, src, nbytes);
+        const int at = 2 * (warp + i * kWarps);
+        const int id = lane < 4 && at + (lane >> 1) < npages ? pid_s[at + (lane >> 1)] : -1;
+        const uint32_t some = __ballot_sync(0xffffffffu, id >= 0);
+        if (lane == 0) mbar_arrive_expect_tx(&full[warp][stage], __popc(some) * kPage4);
+        if (some != 0xFu) {
+            for (int c = 0; c < 4; ++c)
+                if (!(some >> c & 1))
+                    for (int o = lane; o < kPage4 / 16; o += 32)
+                        *reinterpret_cast<uint4*>(dst + c * kPage4 + o * 16) = make_uint4(0, 0, 0, 0);
         }
+        __syncwarp();
+        if (id >= 0)
+            bulk_load(dst + lane * kPage4,
+                      ((lane & 1) ? p.v_cache : p.k_cache) + (static_cast<size_t>(id) * p.nkv + kvh) * kPage4, kPage4,
+                      &full[warp][stage]);
     };
 
     float o[kD / 8][4];
@@ -294,27 +344,35 @@ kv4_decode_kernel(const Kv4Params p) {
     for (int i = 0; i < kD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
     float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.0f, 0.0f};
 
+    for (int s = 0; s < kNst - 1 && s < mine; ++s) load_pair(s, s);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < mine; ++i) {
+        if (i + kNst - 1 < mine) load_pair(i + kNst - 1, stage == 0 ? kNst - 1 : stage - 1);
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][stage], phase, &abort_s, kWaitNs))) {
+            if (p.error_word) atomicExch(p.error_word, 1);
+            // the copies in flight get the same time once more before the rings are reused
+            const uint64_t begin = globaltimer_ns();
+            for (int k = i; k < mine && k < i + kNst; ++k) {
+                while (!mbar_try_wait(&full[warp][stage], phase) && globaltimer_ns() - begin < kWaitNs) {}
+                if (++stage == kNst) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            break;
+        }
+        const uint8_t* st = ring + stage * kStage;
+        const int valid = t1 - (page0 + 2 * (warp + i * kWarps)) * kPage;   // tokens of the pair inside the split, at least 1
+        const bool partial = valid < 2 * kPage;
+        // S = Q K^T, four tiles of eight tokens
+        float s[4][4];
 #pragma unroll
-    for (int s = 0; s < kNst - 1; ++s) {
-        if (s < my_pages) load_page(s, s);
-        cp_async_commit();
-    }
-    for (int i = 0; i < my_pages; ++i) {
-        cp_async_wait<kNst - 2>();
-        __syncwarp();
-        if (i + kNst - 1 < my_pages) load_page(i + kNst - 1, (i + kNst - 1) % kNst);
-        cp_async_commit();
-        const uint8_t* kt = ring + (i % kNst) * kStage;
-        const uint8_t* vt = kt + kPage4;
-        const int tok = (page0 + warp + i * kWarps) * kPage;
-        const int valid = t1 - tok;                        // tokens of this page inside the split, at least 1
-        // S = Q K^T, two tiles of eight tokens
-        float sv[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
-            const uint4 cw = *reinterpret_cast<const uint4*>(kt + (g + 8 * n) * 64 + tq * 16);
-            const uint2 sw = *reinterpret_cast<const uint2*>(kt + kCodes + (g + 8 * n) * 8);
+        for (int n = 0; n < 4; ++n) {
+            const uint8_t* kt = st + (n >> 1) * kTile;
+            s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            const uint4 cw = *reinterpret_cast<const uint4*>(kt + (g + 8 * (n & 1)) * 64 + tq * 16);
+            const uint2 sw = *reinterpret_cast<const uint2*>(kt + kCodes + (g + 8 * (n & 1)) * 8);
             const uint32_t w[4] = {cw.x, cw.y, cw.z, cw.w};
 #pragma unroll
             for (int j = 0; j < kGroups; ++j) {
@@ -323,85 +381,102 @@ kv4_decode_kernel(const Kv4Params p) {
                 uint32_t v[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) v[u] = bf2_fma(code_pair(w[j], u), s2, c2);
-                mma_bf16(s, qa[2 * j], v[0], v[1]);
-                mma_bf16(s, qa[2 * j + 1], v[2], v[3]);
+                mma_bf16(s[n], qa[2 * j], v[0], v[1]);
+                mma_bf16(s[n], qa[2 * j + 1], v[2], v[3]);
             }
-            sv[0][2 * n] = s[0]; sv[0][2 * n + 1] = s[1];
-            sv[1][2 * n] = s[2]; sv[1][2 * n + 1] = s[3];
         }
+        if (partial) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+            for (int n = 0; n < 4; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int t = 2 * tq + (j & 1) + 8 * (j >> 1);
-                sv[h][j] = t < valid ? sv[h][j] * p.scale_log2 : -INFINITY;
-            }
-        float alpha[2];
+                for (int e = 0; e < 4; ++e)
+                    if (8 * n + 2 * tq + (e & 1) >= valid) s[n][e] = -INFINITY;
+        }
+        float mx[2];
+        bool need = false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            float mx = fmaxf(fmaxf(sv[h][0], sv[h][1]), fmaxf(sv[h][2], sv[h][3]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m_r[h], mx);
-            const float ms = mn == -INFINITY ? 0.0f : mn;   // every score -inf so far: weights 0, not NaN
-            alpha[h] = exp2f(m_r[h] - ms);
-            m_r[h] = mn;
-            float rs = 0.0f;
+            mx[h] = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                sv[h][j] = exp2f(sv[h][j] - ms);
-                rs += sv[h][j];
-            }
-            l_r[h] = l_r[h] * alpha[h] + rs;
+            for (int n = 0; n < 4; ++n) mx[h] = fmaxf(mx[h], fmaxf(s[n][2 * h], s[n][2 * h + 1]));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+            need |= (mx[h] - m_r[h]) * p.scale_log2 > 8.0f;
         }
-        if (alpha[0] != 1.0f || alpha[1] != 1.0f) {
+        if (__any_sync(0xffffffffu, need)) {
+            float f[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float mn = fmaxf(m_r[h], mx[h]);
+                f[h] = mn == m_r[h] ? 1.0f : ex2((m_r[h] - mn) * p.scale_log2);
+                m_r[h] = mn;
+                l_r[h] *= f[h];
+            }
 #pragma unroll
             for (int nd = 0; nd < kD / 8; ++nd) {
-                o[nd][0] *= alpha[0]; o[nd][1] *= alpha[0];
-                o[nd][2] *= alpha[1]; o[nd][3] *= alpha[1];
+                o[nd][0] *= f[0]; o[nd][1] *= f[0];
+                o[nd][2] *= f[1]; o[nd][3] *= f[1];
             }
         }
-        // O += P V.  P is rounded to bf16, as the bf16 pages' decode rounds it (2^-9 of each weight).
-        uint32_t pa[4];
-        pa[0] = pack_bf16(sv[0][0], sv[0][1]);
-        pa[1] = pack_bf16(sv[1][0], sv[1][1]);
-        pa[2] = pack_bf16(sv[0][2], sv[0][3]);
-        pa[3] = pack_bf16(sv[1][2], sv[1][3]);
-        // codes and scales of tokens 2 tq, 2 tq + 1 (half a = 0) and 8 more (a = 1)
-        uint4 vc[2], vs[2];
+        // P is rounded to bf16, as the bf16 pages' decode rounds it (2^-8 of each weight at most); l sums the fp32 weights
+        uint32_t pa[2][4];
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            vc[a] = *reinterpret_cast<const uint4*>(vt + a * 512 + lane * 16);
-            vs[a] = *reinterpret_cast<const uint4*>(vt + kCodes + (8 * a + 2 * tq) * 8);
-            // a slot past the end may hold anything: weight 0 times value 0
-            if (8 * a + 2 * tq >= valid) vs[a].x = vs[a].y = 0;
-            if (8 * a + 2 * tq + 1 >= valid) vs[a].z = vs[a].w = 0;
+        for (int h = 0; h < 2; ++h) {
+            const float nm = m_r[h] == -INFINITY ? 0.0f : -m_r[h] * p.scale_log2;   // nothing but -inf yet: weights 0, not NaN
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const float x = ex2(fmaf(s[n][2 * h], p.scale_log2, nm)), y = ex2(fmaf(s[n][2 * h + 1], p.scale_log2, nm));
+                l_r[h] += x + y;
+                pa[n >> 1][(n & 1) * 2 + h] = pack_bf16(x, y);
+            }
         }
+        // O += P V, page by page: tokens 2 tq, 2 tq + 1 of its halves a = 0 and 1
 #pragma unroll
-        for (int j = 0; j < kGroups; ++j) {
-            uint32_t w[2], s2[2], c2[2];
+        for (int pg = 0; pg < 2; ++pg) {
+            const uint8_t* vt = st + pg * kTile + kPage4;
+            uint4 vc[2], vs[2];
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
-                const uint32_t sel = (j & 1) ? 0x7632 : 0x5410;
-                w[a] = __byte_perm(j < 2 ? vc[a].x : vc[a].y, j < 2 ? vc[a].z : vc[a].w, sel);
-                s2[a] = __byte_perm(j < 2 ? vs[a].x : vs[a].y, j < 2 ? vs[a].z : vs[a].w, sel);
-                c2[a] = bf2_mul(s2[a], kMinus136);
+                vc[a] = *reinterpret_cast<const uint4*>(vt + a * 512 + lane * 16);
+                vs[a] = *reinterpret_cast<const uint4*>(vt + kCodes + (8 * a + 2 * tq) * 8);
+                if (partial) {                     // a slot past the end may hold anything: weight 0 times value 0
+                    const int t = 16 * pg + 8 * a + 2 * tq;
+                    if (t >= valid) vs[a].x = vs[a].y = 0;
+                    if (t + 1 >= valid) vs[a].z = vs[a].w = 0;
+                }
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                mma_bf16(o[4 * j + u], pa, bf2_fma(code_pair(w[0], u), s2[0], c2[0]),
-                         bf2_fma(code_pair(w[1], u), s2[1], c2[1]));
+            for (int j = 0; j < kGroups; ++j) {
+                uint32_t w[2], s2[2], c2[2];
+#pragma unroll
+                for (int a = 0; a < 2; ++a) {
+                    const uint32_t sel = (j & 1) ? 0x7632 : 0x5410;
+                    w[a] = __byte_perm(j < 2 ? vc[a].x : vc[a].y, j < 2 ? vc[a].z : vc[a].w, sel);
+                    s2[a] = __byte_perm(j < 2 ? vs[a].x : vs[a].y, j < 2 ? vs[a].z : vs[a].w, sel);
+                    c2[a] = bf2_mul(s2[a], kMinus136);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    mma_bf16(o[4 * j + u], pa[pg], bf2_fma(code_pair(w[0], u), s2[0], c2[0]),
+                             bf2_fma(code_pair(w[1], u), s2[1], c2[1]));
+            }
+        }
+        __syncwarp();                              // the stage is read
+        if (++stage == kNst) {
+            stage = 0;
+            phase ^= 1;
         }
     }
-    cp_async_wait<0>();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         l_r[h] += __shfl_xor_sync(0xffffffffu, l_r[h], 1);
         l_r[h] += __shfl_xor_sync(0xffffffffu, l_r[h], 2);
+        m_r[h] *= p.scale_log2;                    // from here on in log2 units (-inf stays)
     }
     __syncthreads();   // every warp is done with its ring: reuse as merge scratch
     float* mo = reinterpret_cast<float*>(sm);                       // [warp][16][kMergePad]
-    float* mml = mo + kWarps * kGPad * kMergePad;                   // [warp][16][2]
+    float* mml = mo + kWarps * kGPad * kMergePad;                   // [16][warp][2]
+    float* fac = mml + kWarps * kGPad * 2;                          // [16][warp] factors, then [16][2] the split's (m, l)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int r = g + 8 * h;
@@ -413,39 +488,44 @@ kv4_decode_kernel(const Kv4Params p) {
             for (int e = 0; e < 2; ++e)
                 *reinterpret_cast<float4*>(ow + 32 * j + 8 * tq + 4 * e) =
                     make_float4(o[4 * j][2 * h + e], o[4 * j + 1][2 * h + e], o[4 * j + 2][2 * h + e], o[4 * j + 3][2 * h + e]);
-        if (tq == 0) {
-            mml[(warp * kGPad + r) * 2 + 0] = m_r[h];
-            mml[(warp * kGPad + r) * 2 + 1] = l_r[h];
+        if (tq == 0) *reinterpret_cast<float2*>(mml + (r * kWarps + warp) * 2) = make_float2(m_r[h], l_r[h]);
+    }
+    __syncthreads();
+    if (threadIdx.x < kGPad) {
+        const int r = threadIdx.x;
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, mml[(r * kWarps + w) * 2]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float mw = mml[(r * kWarps + w) * 2];
+            const float f = mw == -INFINITY ? 1.0f : ex2(mw - M);   // no weight yet: l and o are 0 or NaN
+            fac[r * kWarps + w] = f;
+            L += mml[(r * kWarps + w) * 2 + 1] * f;
         }
+        fac[kGPad * kWarps + r * 2] = M;
+        fac[kGPad * kWarps + r * 2 + 1] = L;
     }
     __syncthreads();
     const size_t base = (static_cast<size_t>(bk) * p.max_splits + split) * p.G;
+    const int d = threadIdx.x;
     for (int r = 0; r < p.G; ++r) {
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, mml[(w * kGPad + r) * 2]);
-        float L = 0.0f, acc = 0.0f;
-        const int d = threadIdx.x;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            const float mw = mml[(w * kGPad + r) * 2];
-            const float lw = mml[(w * kGPad + r) * 2 + 1];
-            const float f = (mw == -INFINITY) ? 1.0f : exp2f(mw - M);   // no weight yet: l and o are 0 or NaN
-            L += lw * f;
-            acc += mo[(w * kGPad + r) * kMergePad + d] * f;
-        }
-        p.part_o[(base + r) * kD + d] = acc;
-        if (d == 0) {
-            p.part_ml[(base + r) * 2 + 0] = M;
-            p.part_ml[(base + r) * 2 + 1] = L;
+        const float4 f = *reinterpret_cast<const float4*>(fac + r * kWarps);
+        const float* mr = mo + r * kMergePad + d;
+        const float acc = mr[0] * f.x + mr[kGPad * kMergePad] * f.y + mr[2 * kGPad * kMergePad] * f.z + mr[3 * kGPad * kMergePad] * f.w;
+        if (p.max_splits == 1) {
+            write_row(p, b, kvh * p.G + r, acc / fac[kGPad * kWarps + r * 2 + 1], red);
+        } else {
+            p.part_o[(base + r) * kD + d] = acc;
+            if (d < 2) p.part_ml[(base + r) * 2 + d] = fac[kGPad * kWarps + r * 2 + d];
         }
     }
 }
 
 // One block (128 threads = head_dim) per (row, query head): merges the splits.
 __global__ void __launch_bounds__(kD)
-kv4_merge_kernel(const Kv4Params p, __nv_bfloat16* __restrict__ out, uint8_t* __restrict__ out_q,
-                 float* __restrict__ out_s, int out_ld) {
+kv4_merge_kernel(const Kv4Params p) {
+    __shared__ float fac[kD], red[2][kD / 32];
     const int b = blockIdx.x / p.nq, h = blockIdx.x % p.nq;
     const int kvh = h / p.G, r = h % p.G;
     const int d = threadIdx.x;
@@ -453,31 +533,35 @@ kv4_merge_kernel(const Kv4Params p, __nv_bfloat16* __restrict__ out, uint8_t* __
                         ? 0 : clamp_len(p.seq_lens[b], p.max_pages, p.split_tokens, p.max_splits);
     const int ns = (len + p.split_tokens - 1) / p.split_tokens;
     const size_t base = (static_cast<size_t>(b) * p.nkv + kvh) * p.max_splits * p.G + r;
+    auto ml = [&](int s) { return *reinterpret_cast<const float2*>(p.part_ml + (base + static_cast<size_t>(s) * p.G) * 2); };
     float M = -INFINITY;
-    for (int s = 0; s < ns; ++s) M = fmaxf(M, p.part_ml[(base + static_cast<size_t>(s) * p.G) * 2]);
-    float L = 0.0f, acc = 0.0f;
-    for (int s = 0; s < ns; ++s) {
-        const size_t i = base + static_cast<size_t>(s) * p.G;
-        const float ms = p.part_ml[i * 2];
-        const float f = ms == -INFINITY ? 1.0f : exp2f(ms - M);
-        L += p.part_ml[i * 2 + 1] * f;
-        acc += p.part_o[i * kD + d] * f;
-    }
-    const float v = ns > 0 ? acc / L : 0.0f;
-    out[(static_cast<size_t>(b) * p.nq + h) * kD + d] = __float2bfloat16_rn(v);
-    if (out_q) {
-        __shared__ float red[kD / 32];
-        float a = fabsf(v);
+    for (int s = d; s < ns; s += kD) M = fmaxf(M, ml(s).x);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        if ((d & 31) == 0) red[d >> 5] = a;
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if ((d & 31) == 0) red[0][d >> 5] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    float L = 0.0f, acc = 0.0f;
+    for (int s0 = 0; s0 < ns; s0 += kD) {          // 128 splits at a time: factors by a thread each
         __syncthreads();
-        const float amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        uint8_t qv = 0;
-        if (amax > 0.0f) qv = static_cast<uint8_t>(cvt_e4m3x2(v * (448.0f / amax), 0.0f) & 0xFFu);
-        out_q[(static_cast<size_t>(b) * p.nq + h) * kD + d] = qv;
-        if (d == 0) out_s[static_cast<size_t>(h) * out_ld + b] = amax > 0.0f ? amax / 448.0f : 0.0f;
+        if (s0 + d < ns) {
+            const float2 x = ml(s0 + d);
+            const float f = x.x == -INFINITY ? 1.0f : ex2(x.x - M);
+            fac[d] = f;
+            L += x.y * f;
+        }
+        __syncthreads();
+        const int n = min(kD, ns - s0);
+        const float* po = p.part_o + (base + static_cast<size_t>(s0) * p.G) * kD + d;
+#pragma unroll 8
+        for (int s = 0; s < n; ++s) acc += po[static_cast<size_t>(s) * p.G * kD] * fac[s];
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if ((d & 31) == 0) red[1][d >> 5] = L;
+    __syncthreads();
+    L = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+    write_row(p, b, h, ns > 0 ? acc / L : 0.0f, red[0]);
 }
 
 }  // namespace
@@ -581,13 +665,17 @@ moe_status_t attn_kv4_decode_rows(const void* q_bf16, const void* k_cache, const
     p.split_tokens = split_tokens;
     p.max_splits = max_splits;
     p.num_seqs = num_seqs;
-    p.scale_log2 = scale * kLog2e;
+    p.out = static_cast<__nv_bfloat16*>(out_bf16);
+    p.out_q = static_cast<uint8_t*>(out_q);
+    p.out_s = out_s;
+    p.out_ld = out_ld;
+    p.q_flip = scale < 0.0f ? 0x80008000u : 0u;
+    p.scale_log2 = fmaxf(fabsf(scale * kLog2e), 1.17549435e-38f);   // 0: every finite score alike, masked ones still -inf
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     kv4_decode_kernel<<<dim3(max_splits, B * nkv), kWarps * 32, kDecodeSmem, st>>>(p);
-    moe_status_t s = launch_status();
-    if (s != MOE_OK) return s;
-    kv4_merge_kernel<<<B * nq, kD, 0, st>>>(p, static_cast<__nv_bfloat16*>(out_bf16), static_cast<uint8_t*>(out_q), out_s,
-                                           out_ld);
+    const moe_status_t s = launch_status();
+    if (s != MOE_OK || max_splits == 1) return s;
+    kv4_merge_kernel<<<B * nq, kD, 0, st>>>(p);
     return launch_status();
 }
 
