@@ -226,11 +226,22 @@ __device__ __forceinline__ uint32_t bf2_mul(uint32_t a, uint32_t b) {
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
+// mma_bf16 for the compiler to place: nothing here depends on its order
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+        "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 constexpr uint32_t kMinus136 = 0xC308C308u;   // bf16x2
 
-// The codes at nibble i of both halves of w as the bf16 pair 136 + n.
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i) {
-    return ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+// The codes at nibble i of both halves of w as the bf16 pair 136 + n, one lop3
+// after the shift.  `magic` is 0x43004300 in a register: as an immediate beside
+// the mask it would take a second lop3.
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int i, uint32_t magic) {
+    uint32_t d;
+    asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(d) : "r"(w >> (4 * i)), "r"(magic));
+    return d;
 }
 
 // One output row (128 threads, one dim each): bf16, and e4m3 with its scale.
@@ -339,6 +350,8 @@ kv4_decode_kernel(const Kv4Params p) {
                       &full[warp][stage]);
     };
 
+    uint32_t magic;
+    asm volatile("mov.u32 %0, 0x43004300;" : "=r"(magic));
     float o[kD / 8][4];
 #pragma unroll
     for (int i = 0; i < kD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -365,26 +378,29 @@ kv4_decode_kernel(const Kv4Params p) {
         const uint8_t* st = ring + stage * kStage;
         const int valid = t1 - (page0 + 2 * (warp + i * kWarps)) * kPage;   // tokens of the pair inside the split, at least 1
         const bool partial = valid < 2 * kPage;
-        // S = Q K^T, four tiles of eight tokens
+        // S = Q K^T, four tiles of eight tokens side by side: an MMA's result is not waited for by the next
         float s[4][4];
+        uint4 kc[4];
+        uint2 ks[4];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const uint8_t* kt = st + (n >> 1) * kTile;
             s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-            const uint4 cw = *reinterpret_cast<const uint4*>(kt + (g + 8 * (n & 1)) * 64 + tq * 16);
-            const uint2 sw = *reinterpret_cast<const uint2*>(kt + kCodes + (g + 8 * (n & 1)) * 8);
-            const uint32_t w[4] = {cw.x, cw.y, cw.z, cw.w};
-#pragma unroll
-            for (int j = 0; j < kGroups; ++j) {
-                const uint32_t s2 = __byte_perm(j < 2 ? sw.x : sw.y, 0, (j & 1) ? 0x3232 : 0x1010);
-                const uint32_t c2 = bf2_mul(s2, kMinus136);
-                uint32_t v[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) v[u] = bf2_fma(code_pair(w[j], u), s2, c2);
-                mma_bf16(s[n], qa[2 * j], v[0], v[1]);
-                mma_bf16(s[n], qa[2 * j + 1], v[2], v[3]);
-            }
+            kc[n] = *reinterpret_cast<const uint4*>(kt + (g + 8 * (n & 1)) * 64 + tq * 16);
+            ks[n] = *reinterpret_cast<const uint2*>(kt + kCodes + (g + 8 * (n & 1)) * 8);
         }
+#pragma unroll
+        for (int j = 0; j < kGroups; ++j)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const uint32_t w = j == 0 ? kc[n].x : j == 1 ? kc[n].y : j == 2 ? kc[n].z : kc[n].w;
+                    const uint32_t s2 = __byte_perm(j < 2 ? ks[n].x : ks[n].y, 0, (j & 1) ? 0x3232 : 0x1010);
+                    const uint32_t c2 = bf2_mul(s2, kMinus136);
+                    mma(s[n], qa[2 * j + u], bf2_fma(code_pair(w, 2 * u, magic), s2, c2),
+                        bf2_fma(code_pair(w, 2 * u + 1, magic), s2, c2));
+                }
         if (partial) {
 #pragma unroll
             for (int n = 0; n < 4; ++n)
@@ -457,8 +473,8 @@ kv4_decode_kernel(const Kv4Params p) {
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    mma_bf16(o[4 * j + u], pa[pg], bf2_fma(code_pair(w[0], u), s2[0], c2[0]),
-                             bf2_fma(code_pair(w[1], u), s2[1], c2[1]));
+                    mma(o[4 * j + u], pa[pg], bf2_fma(code_pair(w[0], u, magic), s2[0], c2[0]),
+                             bf2_fma(code_pair(w[1], u, magic), s2[1], c2[1]));
             }
         }
         __syncwarp();                              // the stage is read
