@@ -12,6 +12,7 @@
 
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "attn_common.cuh"
 #include "kv_cache.h"
@@ -274,10 +275,15 @@ kv4_decode_kernel(const Kv4Params p) {
     const int b = bk / p.nkv, kvh = bk % p.nkv;
     const int seq = seq_of_row(p.row_seq, b, p.num_seqs);
     if (seq < 0 && split == 0 && threadIdx.x == 0 && kvh == 0 && p.error_word) atomicExch(p.error_word, 7);
+    const int t0 = split * p.split_tokens;
+    const int page0 = t0 / kPage;
+    // the split's first page ids come with the length, not after it
+    const int32_t* ptb = p.page_table + static_cast<size_t>(max(seq, 0)) * p.max_pages + page0;
+    const int split_pages = min(p.split_tokens / kPage, p.max_pages - page0);
+    int first_id = static_cast<int>(threadIdx.x) < split_pages ? ptb[threadIdx.x] : -1;
     const int len_in = seq < 0 ? 0 : p.seq_lens[b];
     const int len = clamp_len(len_in, p.max_pages, p.split_tokens, p.max_splits);
     if (len < len_in && split == 0 && threadIdx.x == 0 && kvh == 0 && p.error_word) atomicExch(p.error_word, 5);
-    const int t0 = split * p.split_tokens;
     if (t0 >= len) {
         if (p.max_splits == 1)                     // there is no merge kernel: an empty row's zeros
             for (int r = 0; r < p.G; ++r) write_row(p, b, kvh * p.G + r, 0.0f, red);
@@ -289,16 +295,12 @@ kv4_decode_kernel(const Kv4Params p) {
 
     uint8_t* ring = sm + static_cast<size_t>(warp) * kNst * kStage;
     int* pid_s = reinterpret_cast<int*>(sm + kRingBytes);
-    const int page0 = t0 / kPage;
     const int npages = (t1 - 1) / kPage - page0 + 1;
-    {
-        const int32_t* ptb = p.page_table + static_cast<size_t>(seq) * p.max_pages + page0;
-        for (int i = threadIdx.x; i < npages; i += blockDim.x) {
-            const int phys = ptb[i];
-            const bool ok = phys >= 0 && phys < p.num_cache_pages;
-            if (!ok && p.error_word) atomicExch(p.error_word, 6);
-            pid_s[i] = ok ? phys : -1;
-        }
+    for (int i = threadIdx.x; i < npages; i += blockDim.x) {
+        const int phys = i == static_cast<int>(threadIdx.x) ? first_id : ptb[i];
+        const bool ok = phys >= 0 && phys < p.num_cache_pages;
+        if (!ok && p.error_word) atomicExch(p.error_word, 6);
+        pid_s[i] = ok ? phys : -1;
     }
     if (lane < kNst) mbar_init(&full[warp][lane], 1);
     if (threadIdx.x == 0) abort_s = 0;
@@ -358,26 +360,8 @@ kv4_decode_kernel(const Kv4Params p) {
     float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.0f, 0.0f};
 
     for (int s = 0; s < kNst - 1 && s < mine; ++s) load_pair(s, s);
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int i = 0; i < mine; ++i) {
-        if (i + kNst - 1 < mine) load_pair(i + kNst - 1, stage == 0 ? kNst - 1 : stage - 1);
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][stage], phase, &abort_s, kWaitNs))) {
-            if (p.error_word) atomicExch(p.error_word, 1);
-            // the copies in flight get the same time once more before the rings are reused
-            const uint64_t begin = globaltimer_ns();
-            for (int k = i; k < mine && k < i + kNst; ++k) {
-                while (!mbar_try_wait(&full[warp][stage], phase) && globaltimer_ns() - begin < kWaitNs) {}
-                if (++stage == kNst) {
-                    stage = 0;
-                    phase ^= 1;
-                }
-            }
-            break;
-        }
-        const uint8_t* st = ring + stage * kStage;
-        const int valid = t1 - (page0 + 2 * (warp + i * kWarps)) * kPage;   // tokens of the pair inside the split, at least 1
-        const bool partial = valid < 2 * kPage;
+    // One pair out of stage `st`; `partial` where only `valid` of its tokens are inside the split (the last pair).
+    auto attend = [&](const uint8_t* st, const int valid, auto partial) {
         // S = Q K^T, four tiles of eight tokens side by side: an MMA's result is not waited for by the next
         float s[4][4];
         uint4 kc[4];
@@ -401,7 +385,7 @@ kv4_decode_kernel(const Kv4Params p) {
                     mma(s[n], qa[2 * j + u], bf2_fma(code_pair(w, 2 * u, magic), s2, c2),
                         bf2_fma(code_pair(w, 2 * u + 1, magic), s2, c2));
                 }
-        if (partial) {
+        if constexpr (partial.value) {
 #pragma unroll
             for (int n = 0; n < 4; ++n)
 #pragma unroll
@@ -455,7 +439,7 @@ kv4_decode_kernel(const Kv4Params p) {
             for (int a = 0; a < 2; ++a) {
                 vc[a] = *reinterpret_cast<const uint4*>(vt + a * 512 + lane * 16);
                 vs[a] = *reinterpret_cast<const uint4*>(vt + kCodes + (8 * a + 2 * tq) * 8);
-                if (partial) {                     // a slot past the end may hold anything: weight 0 times value 0
+                if constexpr (partial.value) {                     // a slot past the end may hold anything: weight 0 times value 0
                     const int t = 16 * pg + 8 * a + 2 * tq;
                     if (t >= valid) vs[a].x = vs[a].y = 0;
                     if (t + 1 >= valid) vs[a].z = vs[a].w = 0;
@@ -477,6 +461,29 @@ kv4_decode_kernel(const Kv4Params p) {
                              bf2_fma(code_pair(w[1], u, magic), s2[1], c2[1]));
             }
         }
+    };
+
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int i = 0; i < mine; ++i) {
+        if (i + kNst - 1 < mine) load_pair(i + kNst - 1, stage == 0 ? kNst - 1 : stage - 1);
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][stage], phase, &abort_s, kWaitNs))) {
+            if (p.error_word) atomicExch(p.error_word, 1);
+            // the copies in flight get the same time once more before the rings are reused
+            const uint64_t begin = globaltimer_ns();
+            for (int k = i; k < mine && k < i + kNst; ++k) {
+                while (!mbar_try_wait(&full[warp][stage], phase) && globaltimer_ns() - begin < kWaitNs) {}
+                if (++stage == kNst) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            break;
+        }
+        const uint8_t* st = ring + stage * kStage;
+        const int valid = t1 - (page0 + 2 * (warp + i * kWarps)) * kPage;   // tokens of the pair inside the split, at least 1
+        if (valid < 2 * kPage) attend(st, valid, std::true_type());
+        else attend(st, valid, std::false_type());
         __syncwarp();                              // the stage is read
         if (++stage == kNst) {
             stage = 0;
