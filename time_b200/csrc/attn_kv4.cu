@@ -296,11 +296,13 @@ kv4_decode_kernel(const Kv4Params p) {
     uint8_t* ring = sm + static_cast<size_t>(warp) * kNst * kStage;
     int* pid_s = reinterpret_cast<int*>(sm + kRingBytes);
     const int npages = (t1 - 1) / kPage - page0 + 1;
+    bool bad = false;                              // an id outside the cache
     for (int i = threadIdx.x; i < npages; i += blockDim.x) {
         const int phys = i == static_cast<int>(threadIdx.x) ? first_id : ptb[i];
         const bool ok = phys >= 0 && phys < p.num_cache_pages;
         if (!ok && p.error_word) atomicExch(p.error_word, 6);
         pid_s[i] = ok ? phys : -1;
+        bad |= !ok;
     }
     if (lane < kNst) mbar_init(&full[warp][lane], 1);
     if (threadIdx.x == 0) abort_s = 0;
@@ -326,30 +328,35 @@ kv4_decode_kernel(const Kv4Params p) {
             }
         }
     }
-    __syncthreads();
+    const bool whole = !__syncthreads_or(bad);
 
     // Pairs of pages, dealt to the warps in turn.
     const int npairs = (npages + 1) / 2;
+    const uint8_t* cache = ((lane & 1) ? p.v_cache : p.k_cache) + static_cast<size_t>(kvh) * kPage4;
+    const size_t page_stride = static_cast<size_t>(p.nkv) * kPage4;
     const int mine = npairs > warp ? (npairs - warp + kWarps - 1) / kWarps : 0;
-    // Lanes 0-3 copy K and V of the pair's two pages; a page that is not there (an id outside the cache, or none behind
-    // the last) reads as zeros: scales of 0.
+    // Lanes 0-3 copy K and V of the pair's two pages.  A page that is not there (none behind the last, or an id outside
+    // the cache) reads as zeros: scales of 0.
     auto load_pair = [&](int i, int stage) {
         uint8_t* dst = ring + stage * kStage;
         const int at = 2 * (warp + i * kWarps);
+        if (whole && at + 1 < npages) {
+            if (lane == 0) mbar_arrive_expect_tx(&full[warp][stage], kStage);
+            __syncwarp();
+            if (lane < 4)
+                bulk_load(dst + lane * kPage4, cache + static_cast<size_t>(pid_s[at + (lane >> 1)]) * page_stride, kPage4,
+                          &full[warp][stage]);
+            return;
+        }
         const int id = lane < 4 && at + (lane >> 1) < npages ? pid_s[at + (lane >> 1)] : -1;
         const uint32_t some = __ballot_sync(0xffffffffu, id >= 0);
         if (lane == 0) mbar_arrive_expect_tx(&full[warp][stage], __popc(some) * kPage4);
-        if (some != 0xFu) {
-            for (int c = 0; c < 4; ++c)
-                if (!(some >> c & 1))
-                    for (int o = lane; o < kPage4 / 16; o += 32)
-                        *reinterpret_cast<uint4*>(dst + c * kPage4 + o * 16) = make_uint4(0, 0, 0, 0);
-        }
+        for (int c = 0; c < 4; ++c)
+            if (!(some >> c & 1))
+                for (int o = lane; o < kPage4 / 16; o += 32)
+                    *reinterpret_cast<uint4*>(dst + c * kPage4 + o * 16) = make_uint4(0, 0, 0, 0);
         __syncwarp();
-        if (id >= 0)
-            bulk_load(dst + lane * kPage4,
-                      ((lane & 1) ? p.v_cache : p.k_cache) + (static_cast<size_t>(id) * p.nkv + kvh) * kPage4, kPage4,
-                      &full[warp][stage]);
+        if (id >= 0) bulk_load(dst + lane * kPage4, cache + static_cast<size_t>(id) * page_stride, kPage4, &full[warp][stage]);
     };
 
     uint32_t magic;
@@ -357,7 +364,9 @@ kv4_decode_kernel(const Kv4Params p) {
     float o[kD / 8][4];
 #pragma unroll
     for (int i = 0; i < kD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-    float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.0f, 0.0f};
+    float m_r[2] = {-INFINITY, -INFINITY}, top_r[2] = {-INFINITY, -INFINITY}, nm_r[2] = {0.0f, 0.0f};
+    float2 l_r[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+    const float lag = 8.0f / p.scale_log2;         // of raw scores
 
     for (int s = 0; s < kNst - 1 && s < mine; ++s) load_pair(s, s);
     // One pair out of stage `st`; `partial` where only `valid` of its tokens are inside the split (the last pair).
@@ -392,25 +401,29 @@ kv4_decode_kernel(const Kv4Params p) {
                 for (int e = 0; e < 4; ++e)
                     if (8 * n + 2 * tq + (e & 1) >= valid) s[n][e] = -INFINITY;
         }
+        // the maximum moves when a score passes it by 8 in log2 units; only then do the lanes of a row compare theirs
         float mx[2];
         bool need = false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            mx[h] = -INFINITY;
+            mx[h] = fmaxf(s[0][2 * h], s[0][2 * h + 1]);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) mx[h] = fmaxf(mx[h], fmaxf(s[n][2 * h], s[n][2 * h + 1]));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            need |= (mx[h] - m_r[h]) * p.scale_log2 > 8.0f;
+            for (int n = 1; n < 4; ++n) mx[h] = fmaxf(mx[h], fmaxf(s[n][2 * h], s[n][2 * h + 1]));
+            need |= mx[h] > top_r[h];
         }
         if (__any_sync(0xffffffffu, need)) {
             float f[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
                 const float mn = fmaxf(m_r[h], mx[h]);
                 f[h] = mn == m_r[h] ? 1.0f : ex2((m_r[h] - mn) * p.scale_log2);
                 m_r[h] = mn;
-                l_r[h] *= f[h];
+                top_r[h] = mn + lag;
+                nm_r[h] = mn == -INFINITY ? 0.0f : -mn * p.scale_log2;     // nothing but -inf yet: weights 0, not NaN
+                l_r[h].x *= f[h];
+                l_r[h].y *= f[h];
             }
 #pragma unroll
             for (int nd = 0; nd < kD / 8; ++nd) {
@@ -421,15 +434,16 @@ kv4_decode_kernel(const Kv4Params p) {
         // P is rounded to bf16, as the bf16 pages' decode rounds it (2^-8 of each weight at most); l sums the fp32 weights
         uint32_t pa[2][4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float nm = m_r[h] == -INFINITY ? 0.0f : -m_r[h] * p.scale_log2;   // nothing but -inf yet: weights 0, not NaN
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
-                const float x = ex2(fmaf(s[n][2 * h], p.scale_log2, nm)), y = ex2(fmaf(s[n][2 * h + 1], p.scale_log2, nm));
-                l_r[h] += x + y;
-                pa[n >> 1][(n & 1) * 2 + h] = pack_bf16(x, y);
+                float2 x = ffma2(make_float2(s[n][2 * h], s[n][2 * h + 1]), make_float2(p.scale_log2, p.scale_log2),
+                                 make_float2(nm_r[h], nm_r[h]));
+                x.x = ex2(x.x);
+                x.y = ex2(x.y);
+                l_r[h] = fadd2(l_r[h], x);
+                pa[n >> 1][(n & 1) * 2 + h] = pack_bf16(x.x, x.y);
             }
-        }
         // O += P V, page by page: tokens 2 tq, 2 tq + 1 of its halves a = 0 and 1
 #pragma unroll
         for (int pg = 0; pg < 2; ++pg) {
@@ -467,7 +481,8 @@ kv4_decode_kernel(const Kv4Params p) {
     uint32_t phase = 0;
     for (int i = 0; i < mine; ++i) {
         if (i + kNst - 1 < mine) load_pair(i + kNst - 1, stage == 0 ? kNst - 1 : stage - 1);
-        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][stage], phase, &abort_s, kWaitNs))) {
+        if (!__all_sync(0xffffffffu, mbar_try_wait(&full[warp][stage], phase)) &&
+            !__all_sync(0xffffffffu, mbar_wait_bounded(&full[warp][stage], phase, &abort_s, kWaitNs))) {
             if (p.error_word) atomicExch(p.error_word, 1);
             // the copies in flight get the same time once more before the rings are reused
             const uint64_t begin = globaltimer_ns();
@@ -492,8 +507,9 @@ kv4_decode_kernel(const Kv4Params p) {
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        l_r[h] += __shfl_xor_sync(0xffffffffu, l_r[h], 1);
-        l_r[h] += __shfl_xor_sync(0xffffffffu, l_r[h], 2);
+        l_r[h].x += l_r[h].y;
+        l_r[h].x += __shfl_xor_sync(0xffffffffu, l_r[h].x, 1);
+        l_r[h].x += __shfl_xor_sync(0xffffffffu, l_r[h].x, 2);
         m_r[h] *= p.scale_log2;                    // from here on in log2 units (-inf stays)
     }
     __syncthreads();   // every warp is done with its ring: reuse as merge scratch
@@ -511,7 +527,7 @@ kv4_decode_kernel(const Kv4Params p) {
             for (int e = 0; e < 2; ++e)
                 *reinterpret_cast<float4*>(ow + 32 * j + 8 * tq + 4 * e) =
                     make_float4(o[4 * j][2 * h + e], o[4 * j + 1][2 * h + e], o[4 * j + 2][2 * h + e], o[4 * j + 3][2 * h + e]);
-        if (tq == 0) *reinterpret_cast<float2*>(mml + (r * kWarps + warp) * 2) = make_float2(m_r[h], l_r[h]);
+        if (tq == 0) *reinterpret_cast<float2*>(mml + (r * kWarps + warp) * 2) = make_float2(m_r[h], l_r[h].x);
     }
     __syncthreads();
     if (threadIdx.x < kGPad) {

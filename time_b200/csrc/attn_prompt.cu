@@ -206,12 +206,6 @@ __device__ __forceinline__ void st_global_32(void* dst, const uint32_t* r) {
                  : "memory");
 }
 
-__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
-    uint64_t ar = *reinterpret_cast<uint64_t*>(&a), br = *reinterpret_cast<uint64_t*>(&b), d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(ar), "l"(br));
-    return *reinterpret_cast<float2*>(&d);
-}
-
 // 2^x for x up to 127 on the FMA pipe, which the softmax leaves idle while the
 // MUFU is its limit: x = n + f with n the nearest integer, a polynomial for 2^f
 // on [-1/2, 1/2] (least largest relative error with P(0) = 1: 2.8e-6), n added
