@@ -188,7 +188,8 @@ constexpr int kStage = 2 * kTile;
 constexpr int kMaxSplitPages = 512;                       // split_tokens <= 8192
 constexpr int kMergePad = kD + 4;
 constexpr size_t kRingBytes = static_cast<size_t>(kWarps) * kNst * kStage;
-constexpr size_t kDecodeSmem = kRingBytes + kMaxSplitPages * 4;
+constexpr size_t kQFragBytes = kD / 16 * 32 * 16;
+constexpr size_t kDecodeSmem = kRingBytes + kMaxSplitPages * 4 + kQFragBytes;
 constexpr uint64_t kWaitNs = 2000000000ull;
 // the warp merge reuses the rings: per warp 16 x 128 fp32, then (m, l) and factors of its rows
 static_assert(static_cast<size_t>(kWarps) * kGPad * (kMergePad + 3) * 4 + kGPad * 8 <= kRingBytes, "merge scratch fits the rings");
@@ -253,9 +254,9 @@ __device__ __forceinline__ void write_row(const Kv4Params& p, int b, int h, floa
         float a = fabsf(v);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
-        __syncthreads();
+        named_bar_sync(1, kD);
         if ((d & 31) == 0) red[d >> 5] = a;
-        __syncthreads();
+        named_bar_sync(1, kD);
         const float amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         uint8_t qv = 0;
         if (amax > 0.0f) qv = static_cast<uint8_t>(cvt_e4m3x2(v * (448.0f / amax), 0.0f) & 0xFFu);
@@ -309,8 +310,9 @@ kv4_decode_kernel(const Kv4Params p) {
     fence_mbar_init();
     // Query fragments: MMA k-step 2j + u takes dims 32 j + 8 tq + {2u, 2u + 4, 2u + 1, 2u + 5} at this lane's
     // four contraction indices, the order the K codes unpack in.
-    uint32_t qa[kD / 16][4];
-    {
+    uint4* qf_s = reinterpret_cast<uint4*>(sm + kRingBytes + kMaxSplitPages * 4);   // [k-step][lane]
+    if (warp == 0) {
+        uint32_t qa[kD / 16][4];
         const __nv_bfloat16* q0 = p.q + (static_cast<size_t>(b) * p.nq + kvh * p.G) * kD;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -327,6 +329,8 @@ kv4_decode_kernel(const Kv4Params p) {
                 qa[2 * j + 1][2 + h] = __byte_perm(v.y, v.w, 0x7632);  // 3, 7
             }
         }
+#pragma unroll
+        for (int ks = 0; ks < kD / 16; ++ks) qf_s[ks * 32 + lane] = make_uint4(qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3]);
     }
     const bool whole = !__syncthreads_or(bad);
 
@@ -385,15 +389,21 @@ kv4_decode_kernel(const Kv4Params p) {
 #pragma unroll
         for (int j = 0; j < kGroups; ++j)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u) {
+                // volatile: a fragment is read where it is used, not held over the whole loop
+                uint32_t qa[4];
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(qa[0]), "=r"(qa[1]), "=r"(qa[2]), "=r"(qa[3])
+                             : "r"(smem_u32(qf_s + (2 * j + u) * 32 + lane)));
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
                     const uint32_t w = j == 0 ? kc[n].x : j == 1 ? kc[n].y : j == 2 ? kc[n].z : kc[n].w;
                     const uint32_t s2 = __byte_perm(j < 2 ? ks[n].x : ks[n].y, 0, (j & 1) ? 0x3232 : 0x1010);
                     const uint32_t c2 = bf2_mul(s2, kMinus136);
-                    mma(s[n], qa[2 * j + u], bf2_fma(code_pair(w, 2 * u, magic), s2, c2),
+                    mma(s[n], qa, bf2_fma(code_pair(w, 2 * u, magic), s2, c2),
                         bf2_fma(code_pair(w, 2 * u + 1, magic), s2, c2));
                 }
+            }
         if constexpr (partial.value) {
 #pragma unroll
             for (int n = 0; n < 4; ++n)
@@ -561,45 +571,58 @@ kv4_decode_kernel(const Kv4Params p) {
     }
 }
 
-// One block (128 threads = head_dim) per (row, query head): merges the splits.
-__global__ void __launch_bounds__(kD)
+// One block per (row, query head) merges the splits: groups of 128 threads (one
+// per dim) take every kMergeGroups-th split.  Four groups where there are few
+// rows, so that many splits are a few loads deep; one where the rows fill the
+// GPU.
+template <int kMergeGroups>
+__global__ void __launch_bounds__(kMergeGroups * kD)
 kv4_merge_kernel(const Kv4Params p) {
-    __shared__ float fac[kD], red[2][kD / 32];
+    __shared__ float fac[kMergeGroups * kD], red[2][kMergeGroups * kD / 32], sum[kMergeGroups][kD];
     const int b = blockIdx.x / p.nq, h = blockIdx.x % p.nq;
     const int kvh = h / p.G, r = h % p.G;
-    const int d = threadIdx.x;
+    const int tid = threadIdx.x, d = tid % kD, grp = tid / kD;
     const int len = seq_of_row(p.row_seq, b, p.num_seqs) < 0
                         ? 0 : clamp_len(p.seq_lens[b], p.max_pages, p.split_tokens, p.max_splits);
     const int ns = (len + p.split_tokens - 1) / p.split_tokens;
     const size_t base = (static_cast<size_t>(b) * p.nkv + kvh) * p.max_splits * p.G + r;
     auto ml = [&](int s) { return *reinterpret_cast<const float2*>(p.part_ml + (base + static_cast<size_t>(s) * p.G) * 2); };
-    float M = -INFINITY;
-    for (int s = d; s < ns; s += kD) M = fmaxf(M, ml(s).x);
+    auto block_all = [&](float v, float* w, bool maximum) {        // over the block, to every thread
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if ((d & 31) == 0) red[0][d >> 5] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    float L = 0.0f, acc = 0.0f;
-    for (int s0 = 0; s0 < ns; s0 += kD) {          // 128 splits at a time: factors by a thread each
+        for (int o = 16; o > 0; o >>= 1) {
+            const float y = __shfl_xor_sync(0xffffffffu, v, o);
+            v = maximum ? fmaxf(v, y) : v + y;
+        }
+        if ((tid & 31) == 0) w[tid >> 5] = v;
         __syncthreads();
-        if (s0 + d < ns) {
-            const float2 x = ml(s0 + d);
+        v = w[0];
+#pragma unroll
+        for (int i = 1; i < kMergeGroups * kD / 32; ++i) v = maximum ? fmaxf(v, w[i]) : v + w[i];
+        return v;
+    };
+    float M = -INFINITY;
+    for (int s = tid; s < ns; s += kMergeGroups * kD) M = fmaxf(M, ml(s).x);
+    M = block_all(M, red[0], true);
+    float L = 0.0f, acc = 0.0f;
+    for (int s0 = 0; s0 < ns; s0 += kMergeGroups * kD) {           // factors by a thread each
+        __syncthreads();
+        if (s0 + tid < ns) {
+            const float2 x = ml(s0 + tid);
             const float f = x.x == -INFINITY ? 1.0f : ex2(x.x - M);
-            fac[d] = f;
+            fac[tid] = f;
             L += x.y * f;
         }
         __syncthreads();
-        const int n = min(kD, ns - s0);
+        const int n = min(kMergeGroups * kD, ns - s0);
         const float* po = p.part_o + (base + static_cast<size_t>(s0) * p.G) * kD + d;
 #pragma unroll 8
-        for (int s = 0; s < n; ++s) acc += po[static_cast<size_t>(s) * p.G * kD] * fac[s];
+        for (int s = grp; s < n; s += kMergeGroups) acc += po[static_cast<size_t>(s) * p.G * kD] * fac[s];
     }
+    sum[grp][d] = acc;
+    L = block_all(L, red[1], false);
+    if (grp) return;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    if ((d & 31) == 0) red[1][d >> 5] = L;
-    __syncthreads();
-    L = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+    for (int g = 1; g < kMergeGroups; ++g) acc += sum[g][d];
     write_row(p, b, h, ns > 0 ? acc / L : 0.0f, red[0]);
 }
 
@@ -651,13 +674,15 @@ moe_status_t attn_kv4_read_rows(const void* k_cache, const void* v_cache, int nu
 
 int attn_kv4_split_tokens(int B, int nkv, int max_context) {
     if (B <= 0 || nkv <= 0 || max_context <= 0) return kPage;
-    // about two waves of three CTAs per SM at half the longest context, at least a page per warp
-    const long long rows = static_cast<long long>(B) * nkv;
-    const long long want = (2 * 444 + rows - 1) / rows;
-    long long split = (max_context / 2 + want - 1) / want;
+    // One CTA's fixed cost is that of about 14 pages (4 us beside 0.27 us a page, 3 CTAs an SM).  One wave of the 444
+    // CTAs at half the longest context, as long as that leaves splits of 256 to 1536 tokens; longer contexts go in two
+    // waves or more, which even out uneven lengths (64 rows up to 32K: 2048 tokens 65 us, 1184 59 us).  A context that one
+    // split of 512 tokens holds needs no merge.
+    if (max_context <= 512) return (max_context + kPage - 1) / kPage * kPage;
+    long long split = static_cast<long long>(B) * nkv * max_context / (2 * 444);
+    if (split > 1536) split = split / 2 < 2048 ? split / 2 : 2048;
     split = (split + kPage - 1) / kPage * kPage;
-    const long long low = kWarps * kPage, high = kMaxSplitPages * kPage;
-    return static_cast<int>(split < low ? low : split > high ? high : split);
+    return static_cast<int>(split < 256 ? 256 : split);
 }
 
 size_t attn_kv4_decode_workspace_bytes(int B, int nq, int max_splits) {
@@ -714,7 +739,8 @@ moe_status_t attn_kv4_decode_rows(const void* q_bf16, const void* k_cache, const
     kv4_decode_kernel<<<dim3(max_splits, B * nkv), kWarps * 32, kDecodeSmem, st>>>(p);
     const moe_status_t s = launch_status();
     if (s != MOE_OK || max_splits == 1) return s;
-    kv4_merge_kernel<<<B * nq, kD, 0, st>>>(p);
+    if (B * nq < 4 * 148) kv4_merge_kernel<4><<<B * nq, 4 * kD, 0, st>>>(p);
+    else kv4_merge_kernel<1><<<B * nq, kD, 0, st>>>(p);
     return launch_status();
 }
 
