@@ -333,6 +333,7 @@ kv4_decode_kernel(const Kv4Params p) {
         for (int ks = 0; ks < kD / 16; ++ks) qf_s[ks * 32 + lane] = make_uint4(qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3]);
     }
     const bool whole = !__syncthreads_or(bad);
+    grid_dependents_launch();                      // the merge may take its places; it waits for this grid's end
 
     // Pairs of pages, dealt to the warps in turn.
     const int npairs = (npages + 1) / 2;
@@ -571,59 +572,73 @@ kv4_decode_kernel(const Kv4Params p) {
     }
 }
 
-// One block per (row, query head) merges the splits: groups of 128 threads (one
-// per dim) take every kMergeGroups-th split.  Four groups where there are few
-// rows, so that many splits are a few loads deep; one where the rows fill the
-// GPU.
-template <int kMergeGroups>
-__global__ void __launch_bounds__(kMergeGroups * kD)
+// Merge of a (row, query head)'s splits by 128 threads, one per dim, in kGroups
+// groups that take every kGroups-th split: four where there are few rows, so
+// that many splits are a few loads deep, one where the rows fill the GPU.  Every
+// warp works out the factors of 32 splits by itself, so the partials' loads wait
+// for nothing but the length.
+template <int kGroups>
+__global__ void __launch_bounds__(kGroups * kD)
 kv4_merge_kernel(const Kv4Params p) {
-    __shared__ float fac[kMergeGroups * kD], red[2][kMergeGroups * kD / 32], sum[kMergeGroups][kD];
+    __shared__ float red[kWarps], sum[kGroups][kD + 2];
     const int b = blockIdx.x / p.nq, h = blockIdx.x % p.nq;
     const int kvh = h / p.G, r = h % p.G;
-    const int tid = threadIdx.x, d = tid % kD, grp = tid / kD;
+    const int d = threadIdx.x % kD, grp = threadIdx.x / kD, lane = threadIdx.x & 31;
     const int len = seq_of_row(p.row_seq, b, p.num_seqs) < 0
                         ? 0 : clamp_len(p.seq_lens[b], p.max_pages, p.split_tokens, p.max_splits);
     const int ns = (len + p.split_tokens - 1) / p.split_tokens;
     const size_t base = (static_cast<size_t>(b) * p.nkv + kvh) * p.max_splits * p.G + r;
-    auto ml = [&](int s) { return *reinterpret_cast<const float2*>(p.part_ml + (base + static_cast<size_t>(s) * p.G) * 2); };
-    auto block_all = [&](float v, float* w, bool maximum) {        // over the block, to every thread
+    const size_t step = static_cast<size_t>(p.G) * kGroups;       // rows of the partials from one of the group's splits to its next
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + base + static_cast<size_t>(grp) * p.G;
+    const float* po = p.part_o + (base + static_cast<size_t>(grp) * p.G) * kD + d;
+    const int mine = ns > grp ? (ns - grp + kGroups - 1) / kGroups : 0;
+    grid_dependency_wait();                        // the splits
+    float M = -INFINITY, L = 0.0f, acc = 0.0f;
+    for (int s0 = 0; s0 < mine; s0 += 32) {
+        const int n = min(32, mine - s0);
+        const float2 x = lane < n ? ml[static_cast<size_t>(s0 + lane) * step] : make_float2(-INFINITY, 0.0f);
+        float m = x.x;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const float y = __shfl_xor_sync(0xffffffffu, v, o);
-            v = maximum ? fmaxf(v, y) : v + y;
-        }
-        if ((tid & 31) == 0) w[tid >> 5] = v;
-        __syncthreads();
-        v = w[0];
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float mn = fmaxf(M, m);
+        const float keep = M == -INFINITY ? 1.0f : ex2(M - mn);
+        const float f = x.x == -INFINITY ? 1.0f : ex2(x.x - mn);   // no weight: l and o are 0 or NaN
+        acc *= keep;
+        float l = lane < n ? x.y * f : 0.0f;
 #pragma unroll
-        for (int i = 1; i < kMergeGroups * kD / 32; ++i) v = maximum ? fmaxf(v, w[i]) : v + w[i];
-        return v;
-    };
-    float M = -INFINITY;
-    for (int s = tid; s < ns; s += kMergeGroups * kD) M = fmaxf(M, ml(s).x);
-    M = block_all(M, red[0], true);
-    float L = 0.0f, acc = 0.0f;
-    for (int s0 = 0; s0 < ns; s0 += kMergeGroups * kD) {           // factors by a thread each
-        __syncthreads();
-        if (s0 + tid < ns) {
-            const float2 x = ml(s0 + tid);
-            const float f = x.x == -INFINITY ? 1.0f : ex2(x.x - M);
-            fac[tid] = f;
-            L += x.y * f;
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        L = L * keep + l;
+        M = mn;
+#pragma unroll
+        for (int c = 0; c < 32; c += 8) {
+            if (c >= n) break;
+            float v[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) v[s] = c + s < n ? po[static_cast<size_t>(s0 + c + s) * step * kD] : 0.0f;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) acc += v[s] * __shfl_sync(0xffffffffu, f, c + s);
         }
-        __syncthreads();
-        const int n = min(kMergeGroups * kD, ns - s0);
-        const float* po = p.part_o + (base + static_cast<size_t>(s0) * p.G) * kD + d;
-#pragma unroll 8
-        for (int s = grp; s < n; s += kMergeGroups) acc += po[static_cast<size_t>(s) * p.G * kD] * fac[s];
     }
-    sum[grp][d] = acc;
-    L = block_all(L, red[1], false);
-    if (grp) return;
+    if constexpr (kGroups > 1) {
+        sum[grp][d] = acc;
+        if (d == 0) {
+            sum[grp][kD] = M;
+            sum[grp][kD + 1] = L;
+        }
+        __syncthreads();
+        if (grp) return;
+        float top = M;
 #pragma unroll
-    for (int g = 1; g < kMergeGroups; ++g) acc += sum[g][d];
-    write_row(p, b, h, ns > 0 ? acc / L : 0.0f, red[0]);
+        for (int g = 1; g < kGroups; ++g) top = fmaxf(top, sum[g][kD]);
+        acc = L = 0.0f;
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) {
+            const float f = sum[g][kD] == -INFINITY ? 1.0f : ex2(sum[g][kD] - top);
+            acc += sum[g][d] * f;
+            L += sum[g][kD + 1] * f;
+        }
+    }
+    write_row(p, b, h, ns > 0 ? acc / L : 0.0f, red);
 }
 
 }  // namespace
@@ -739,9 +754,9 @@ moe_status_t attn_kv4_decode_rows(const void* q_bf16, const void* k_cache, const
     kv4_decode_kernel<<<dim3(max_splits, B * nkv), kWarps * 32, kDecodeSmem, st>>>(p);
     const moe_status_t s = launch_status();
     if (s != MOE_OK || max_splits == 1) return s;
-    if (B * nq < 4 * 148) kv4_merge_kernel<4><<<B * nq, 4 * kD, 0, st>>>(p);
-    else kv4_merge_kernel<1><<<B * nq, kD, 0, st>>>(p);
-    return launch_status();
+    const cudaError_t e = B * nq < 4 * 148 ? launch_dependent(kv4_merge_kernel<4>, B * nq, 4 * kD, st, p)
+                                           : launch_dependent(kv4_merge_kernel<1>, B * nq, kD, st, p);
+    return e == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
 }
 
 }  // extern "C"

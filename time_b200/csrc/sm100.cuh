@@ -388,6 +388,14 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
 
+// ---------------------------------------------------------------- dependent launches
+
+// A kernel launched by launch_dependent may start while the one before it in
+// the stream still runs; it waits here for that one's end and its writes.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Lets the dependent kernel start once every block has come here or left.
+__device__ __forceinline__ void grid_dependents_launch() { asm volatile("griddepcontrol.launch_dependents;"); }
+
 // ---------------------------------------------------------------- math
 
 // d = a * b + c on two fp32 lanes at once (each lane IEEE fma, RN).
@@ -459,6 +467,23 @@ inline cudaError_t smem_optin_once(F* kernel, int bytes, bool (&done)[kMaxDevice
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess && cached) done[dev] = true;
     return e;
+}
+
+// Launches `kernel` so that it may begin under the kernel before it in the
+// stream; it has to call grid_dependency_wait before it touches what that one
+// writes, or anything that earlier work in the stream may still use.
+template <typename... P, typename... A>
+inline cudaError_t launch_dependent(void (*kernel)(P...), int blocks, int threads, cudaStream_t stream, A&&... args) {
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
 }  // namespace tb
