@@ -38,6 +38,7 @@ __host__ __device__ constexpr int v_code_byte(int t, int d) {
 // ---------------------------------------------------------------- write
 
 constexpr int kWriteWarps = 8;
+constexpr int kWriteUnroll = 4;                      // pairs of heads a warp has in flight
 
 // Scale of a group whose largest |x| has the bits `amax`, and 0 for a group
 // that is stored as NaN.
@@ -47,108 +48,164 @@ __device__ __forceinline__ float group_scale(uint32_t amax) {
     return fmaxf(__uint_as_float((b + 0x000FFFFFu) & ~0x000FFFFFu), 1.17549435e-38f);
 }
 
-// One block per (row, share of the heads), one warp per head; lane l holds dims
-// 4l .. 4l+3, so a group of 32 dims is eight lanes.  The kernel is bound by the
-// rows in and the q rows out.
+// (lo, hi) of a pair after rotation; products rounded before the sum, so the
+// result does not hang on what the compiler contracts.
+__device__ __forceinline__ float rotate_lo(float a, float c, float cs, float sn) { return __fsub_rn(__fmul_rn(a, cs), __fmul_rn(c, sn)); }
+__device__ __forceinline__ float rotate_hi(float a, float c, float cs, float sn) { return __fadd_rn(__fmul_rn(a, sn), __fmul_rn(c, cs)); }
+
+struct WriteParams {
+    const __nv_bfloat16* qkv;
+    const float* inv_freq;
+    const int32_t* positions;
+    const int32_t* row_seq;
+    const int32_t* page_table;
+    __nv_bfloat16* q_out;
+    __nv_bfloat16* k_out;
+    uint8_t* k_cache;
+    uint8_t* v_cache;
+    int32_t* seq_lens_out;
+    int* error_word;
+    int nq, nkv, rot, num_seqs, max_pages, num_cache_pages;
+};
+
+// Eight dims 8 l .. 8 l + 7 of a head, by lane l of a half-warp, quantised into
+// token t of the (page, head) tile; the whole warp comes here, `store` says
+// which half has a tile.
+__device__ __forceinline__ void quantise_store(const __nv_bfloat16 (&x)[8], uint8_t* page, int t, int l, bool is_k, bool store) {
+    uint32_t amax = 0;                               // as bits: a NaN is above every number
+#pragma unroll
+    for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(__bfloat162float(x[e])) & 0x7FFFFFFFu);
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));       // a group of 32 dims is four lanes
+    if (!store) return;
+    const float s = group_scale(amax);
+    uint32_t codes = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float n = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(__bfloat162float(x[e]), s)), -8.0f), 7.0f) : 0.0f;
+        codes |= static_cast<uint32_t>(static_cast<int>(n) + 8) << (4 * e);
+    }
+    if (is_k) {
+        *reinterpret_cast<uint32_t*>(page + k_code_byte(t, 8 * l)) = codes;
+    } else {
+        *reinterpret_cast<uint16_t*>(page + v_code_byte(t, 8 * l)) = static_cast<uint16_t>(codes);
+        *reinterpret_cast<uint16_t*>(page + v_code_byte(t, 8 * l + 4)) = static_cast<uint16_t>(codes >> 16);
+    }
+    if ((l & 3) == 0)
+        *reinterpret_cast<uint16_t*>(page + kCodes + (t * kGroups + l / 4) * 2) =
+            s > 0.0f ? static_cast<uint16_t>(__float_as_uint(s) >> 16) : static_cast<uint16_t>(0x7FC0);   // s is a bf16 number
+}
+
+// One block per (row, share of the heads), a half-warp per head with 16 bytes a
+// lane and kWriteUnroll heads in flight; bound by the rows in and the q rows
+// out.  kLanes: the rotated halves are whole lanes, a dim's partner comes from
+// lane l +- half / 8 and a lane's cosines stay in registers; else partners come
+// from memory.
+template <bool kLanes>
 __global__ void __launch_bounds__(kWriteWarps * 32)
-kv4_rope_write_kernel(const __nv_bfloat16* __restrict__ qkv, int nq, int nkv, int rot,
-                      const float* __restrict__ inv_freq, const int32_t* __restrict__ positions,
-                      const int32_t* __restrict__ row_seq, int num_seqs, const int32_t* __restrict__ page_table,
-                      int max_pages, int num_cache_pages, __nv_bfloat16* __restrict__ q_out,
-                      __nv_bfloat16* __restrict__ k_out, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache,
-                      int32_t* __restrict__ seq_lens_out, int* __restrict__ error_word) {
+kv4_rope_write_kernel(const WriteParams p) {
     __shared__ float cs_s[kD / 2], sn_s[kD / 2];
-    const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 15;
     const bool first = blockIdx.y == 0 && threadIdx.x == 0;
-    const int pos = positions[b];
-    const int seq = seq_of_row(row_seq, b, num_seqs);
-    if (first && seq_lens_out) seq_lens_out[b] = (pos >= 0 && seq >= 0) ? pos + 1 : 0;
-    if (seq < 0) {
-        if (first && error_word) atomicExch(error_word, 7);
+    const int pos = p.positions[b];
+    const int seq = seq_of_row(p.row_seq, b, p.num_seqs);
+    if (first && p.seq_lens_out) p.seq_lens_out[b] = (pos >= 0 && seq >= 0) ? pos + 1 : 0;
+    int phys = 0, err = 0;
+    if (seq < 0) err = 7;
+    else if (pos < 0 || pos / kPage >= p.max_pages) err = 4;
+    else {
+        phys = p.page_table[static_cast<size_t>(seq) * p.max_pages + pos / kPage];
+        if (phys < 0 || phys >= p.num_cache_pages) err = 6;
+    }
+    if (err) {
+        if (first && p.error_word) atomicExch(p.error_word, err);
         return;
     }
-    if (pos < 0 || pos / kPage >= max_pages) {
-        if (first && error_word) atomicExch(error_word, 4);
-        return;
-    }
-    const int phys = page_table[static_cast<size_t>(seq) * max_pages + pos / kPage];
-    if (phys < 0 || phys >= num_cache_pages) {
-        if (first && error_word) atomicExch(error_word, 6);
-        return;
-    }
-    const int half = rot / 2;
-    for (int i = threadIdx.x; i < half; i += blockDim.x) {
+    const int half = p.rot / 2;
+    for (int i = threadIdx.x; i < half; i += blockDim.x)
         // the angle is the fp32 product, as in the bf16 page write
-        sincosf(static_cast<float>(pos) * inv_freq[i], &sn_s[i], &cs_s[i]);
-    }
+        sincosf(static_cast<float>(pos) * p.inv_freq[i], &sn_s[i], &cs_s[i]);
     __syncthreads();
     const int t = pos % kPage;
-    const int heads = nq + 2 * nkv;
-    for (int h = blockIdx.y * kWriteWarps + warp; h < heads; h += gridDim.y * kWriteWarps) {
-        const __nv_bfloat16* src = qkv + (static_cast<size_t>(b) * heads + h) * kD;
-        const uint2 own = *reinterpret_cast<const uint2*>(src + 4 * lane);
-        const __nv_bfloat16* ob = reinterpret_cast<const __nv_bfloat16*>(&own);
-        __nv_bfloat16 x[4];
+    const int heads = p.nq + 2 * p.nkv;
+    const __nv_bfloat16* row = p.qkv + static_cast<size_t>(b) * heads * kD;
+    // this lane's dims: below half, above it, or not rotated
+    const bool rotated = 8 * l < p.rot, lo = 8 * l < half;
+    float cs[8], sn[8];
+    if constexpr (kLanes) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int d = 4 * lane + e;
-            x[e] = ob[e];
-            if (h < nq + nkv && d < rot) {
-                const bool lo = d < half;
-                const int i = lo ? d : d - half;
-                const float a = __bfloat162float(lo ? ob[e] : src[i]);
-                const float c = __bfloat162float(lo ? src[i + half] : ob[e]);
-                // products rounded before the sum: one result whatever the compiler contracts
-                x[e] = __float2bfloat16_rn(lo ? __fsub_rn(__fmul_rn(a, cs_s[i]), __fmul_rn(c, sn_s[i]))
-                                              : __fadd_rn(__fmul_rn(a, sn_s[i]), __fmul_rn(c, cs_s[i])));
+        for (int e = 0; e < 8; ++e) {
+            const int i = rotated ? 8 * l + e - (lo ? 0 : half) : 0;
+            cs[e] = rotated ? cs_s[i] : 1.0f;
+            sn[e] = rotated ? sn_s[i] : 0.0f;
+        }
+    }
+    const int partner = lo ? lane + half / 8 : lane - half / 8;
+    const int stride = gridDim.y * kWriteWarps * 2;
+    for (int h0 = (blockIdx.y * kWriteWarps + warp) * 2 + (lane >> 4); h0 - (lane >> 4) < heads; h0 += stride * kWriteUnroll) {
+        uint4 in[kWriteUnroll];
+#pragma unroll
+        for (int u = 0; u < kWriteUnroll; ++u)
+            if (h0 + u * stride < heads) in[u] = *reinterpret_cast<const uint4*>(row + static_cast<size_t>(h0 + u * stride) * kD + 8 * l);
+#pragma unroll
+        for (int u = 0; u < kWriteUnroll; ++u) {
+            const int h = h0 + u * stride;
+            if (h - (lane >> 4) >= heads) break;     // for the whole warp: what follows shuffles
+            const bool some = h < heads;
+            const __nv_bfloat16* ib = reinterpret_cast<const __nv_bfloat16*>(&in[u]);
+            __nv_bfloat16 x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = ib[e];
+            if constexpr (kLanes) {
+                uint4 other;
+                other.x = __shfl_sync(0xffffffffu, in[u].x, partner & 31);
+                other.y = __shfl_sync(0xffffffffu, in[u].y, partner & 31);
+                other.z = __shfl_sync(0xffffffffu, in[u].z, partner & 31);
+                other.w = __shfl_sync(0xffffffffu, in[u].w, partner & 31);
+                const __nv_bfloat16* ob = reinterpret_cast<const __nv_bfloat16*>(&other);
+                if (rotated && h < p.nq + p.nkv) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float mine = __bfloat162float(ib[e]), theirs = __bfloat162float(ob[e]);
+                        x[e] = __float2bfloat16_rn(lo ? rotate_lo(mine, theirs, cs[e], sn[e]) : rotate_hi(theirs, mine, cs[e], sn[e]));
+                    }
+                }
+            } else if (some && h < p.nq + p.nkv) {
+                const __nv_bfloat16* src = row + static_cast<size_t>(h) * kD;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int d = 8 * l + e;
+                    if (d < half) x[e] = __float2bfloat16_rn(rotate_lo(__bfloat162float(ib[e]), __bfloat162float(src[d + half]), cs_s[d], sn_s[d]));
+                    else if (d < p.rot) x[e] = __float2bfloat16_rn(rotate_hi(__bfloat162float(src[d - half]), __bfloat162float(ib[e]), cs_s[d - half], sn_s[d - half]));
+                }
             }
+            const uint4 xv = *reinterpret_cast<const uint4*>(x);
+            if (some && h < p.nq) *reinterpret_cast<uint4*>(p.q_out + (static_cast<size_t>(b) * p.nq + h) * kD + 8 * l) = xv;
+            if (h - (lane >> 4) + 1 < p.nq) continue;        // both heads of the warp are queries
+            const bool is_k = h < p.nq + p.nkv;
+            const int kvh = is_k ? h - p.nq : h - p.nq - p.nkv;
+            const bool kv = some && h >= p.nq;
+            if (kv && is_k && p.k_out) *reinterpret_cast<uint4*>(p.k_out + (static_cast<size_t>(b) * p.nkv + kvh) * kD + 8 * l) = xv;
+            uint8_t* page = (is_k ? p.k_cache : p.v_cache) + (static_cast<size_t>(phys) * p.nkv + (kv ? kvh : 0)) * kPage4;
+            quantise_store(x, page, t, l, is_k, kv);
         }
-        const uint2 xv = *reinterpret_cast<const uint2*>(x);
-        if (h < nq) {
-            *reinterpret_cast<uint2*>(q_out + (static_cast<size_t>(b) * nq + h) * kD + 4 * lane) = xv;
-            continue;
-        }
-        const bool is_k = h < nq + nkv;
-        const int kvh = is_k ? h - nq : h - nq - nkv;
-        if (is_k && k_out) *reinterpret_cast<uint2*>(k_out + (static_cast<size_t>(b) * nkv + kvh) * kD + 4 * lane) = xv;
-        uint32_t amax = 0;   // as bits: a NaN is above every number
-#pragma unroll
-        for (int e = 0; e < 4; ++e) amax = max(amax, __float_as_uint(__bfloat162float(x[e])) & 0x7FFFFFFFu);
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        const float s = group_scale(amax);
-        uint32_t codes = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float n = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(__bfloat162float(x[e]), s)), -8.0f), 7.0f) : 0.0f;
-            codes |= static_cast<uint32_t>(static_cast<int>(n) + 8) << (4 * e);
-        }
-        uint8_t* page = (is_k ? k_cache : v_cache) + (static_cast<size_t>(phys) * nkv + kvh) * kPage4;
-        *reinterpret_cast<uint16_t*>(page + (is_k ? k_code_byte(t, 4 * lane) : v_code_byte(t, 4 * lane))) =
-            static_cast<uint16_t>(codes);
-        if ((lane & 7) == 0)
-            *reinterpret_cast<uint16_t*>(page + kCodes + (t * kGroups + lane / 8) * 2) =
-                s > 0.0f ? static_cast<uint16_t>(__float_as_uint(s) >> 16) : static_cast<uint16_t>(0x7FC0);   // s is a bf16 number
     }
 }
 
 // ---------------------------------------------------------------- read
 
 constexpr int kReadWarps = 8;
+constexpr int kReadUnroll = 8;
 
-// One warp per (row, kv head, K or V).
+// One warp per row, a half-warp per (K or V, head) with 16 bytes out a lane.
 __global__ void __launch_bounds__(kReadWarps * 32)
 kv4_read_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, int num_cache_pages,
                 const int32_t* __restrict__ positions, const int32_t* __restrict__ row_seq, int num_seqs,
                 const int32_t* __restrict__ page_table, int max_pages, int B, int nkv,
                 __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ error_word) {
-    const long long w = static_cast<long long>(blockIdx.x) * kReadWarps + (threadIdx.x >> 5);
-    if (w >= 2ll * B * nkv) return;
-    const int lane = threadIdx.x & 31;
-    const bool is_k = w % 2 == 0;
-    const int kvh = static_cast<int>(w / 2 % nkv), b = static_cast<int>(w / 2 / nkv);
-    __nv_bfloat16* out = is_k ? k_out : v_out;
-    if (!out) return;
+    const int b = blockIdx.x * kReadWarps + (threadIdx.x >> 5);
+    if (b >= B) return;
+    const int lane = threadIdx.x & 31, l = lane & 15;
     const int pos = positions[b];
     const int seq = seq_of_row(row_seq, b, num_seqs);
     int phys = -1, err = 0;
@@ -159,19 +216,40 @@ kv4_read_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__
         if (phys < 0 || phys >= num_cache_pages) err = 6;
     }
     if (err && lane == 0 && error_word) atomicExch(error_word, err);
-    __nv_bfloat16 x[4];
-    if (err) {
-        for (int e = 0; e < 4; ++e) x[e] = __float2bfloat16_rn(0.0f);
-    } else {
-        const int t = pos % kPage;
-        const uint8_t* page = (is_k ? k_cache : v_cache) + (static_cast<size_t>(phys) * nkv + kvh) * kPage4;
-        const uint32_t codes = *reinterpret_cast<const uint16_t*>(page + (is_k ? k_code_byte(t, 4 * lane) : v_code_byte(t, 4 * lane)));
-        const float s = __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(page + kCodes + (t * kGroups + lane / 8) * 2));
+    const int t = err ? 0 : pos % kPage;
+    const size_t page0 = static_cast<size_t>(err ? 0 : phys) * nkv * kPage4;
+    const int items = 2 * nkv;                       // K of every head, then V
+    for (int i0 = lane >> 4; i0 < items; i0 += 2 * kReadUnroll) {
+        uint32_t codes[kReadUnroll], scale[kReadUnroll];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            x[e] = __float2bfloat16_rn(static_cast<float>(static_cast<int>((codes >> (4 * e)) & 15u) - 8) * s);
+        for (int u = 0; u < kReadUnroll; ++u) {
+            const int i = i0 + 2 * u;
+            const bool is_k = i < nkv;
+            codes[u] = 0x88888888u;
+            scale[u] = 0;
+            if (i < items && !err && (is_k ? k_out : v_out)) {
+                const uint8_t* page = (is_k ? k_cache : v_cache) + page0 + static_cast<size_t>(is_k ? i : i - nkv) * kPage4;
+                if (is_k) codes[u] = *reinterpret_cast<const uint32_t*>(page + k_code_byte(t, 8 * l));
+                else codes[u] = *reinterpret_cast<const uint16_t*>(page + v_code_byte(t, 8 * l)) |
+                                static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(page + v_code_byte(t, 8 * l + 4))) << 16;
+                scale[u] = *reinterpret_cast<const uint16_t*>(page + kCodes + (t * kGroups + l / 4) * 2);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kReadUnroll; ++u) {
+            const int i = i0 + 2 * u;
+            const bool is_k = i < nkv;
+            __nv_bfloat16* out = is_k ? k_out : v_out;
+            if (i >= items || !out) continue;
+            const float s = __uint_as_float(scale[u] << 16);
+            __nv_bfloat16 x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[e] = __float2bfloat16_rn(static_cast<float>(static_cast<int>((codes[u] >> (4 * e)) & 15u) - 8) * s);
+            *reinterpret_cast<uint4*>(out + (static_cast<size_t>(b) * nkv + (is_k ? i : i - nkv)) * kD + 8 * l) =
+                *reinterpret_cast<const uint4*>(x);
+        }
     }
-    *reinterpret_cast<uint2*>(out + (static_cast<size_t>(b) * nkv + kvh) * kD + 4 * lane) = *reinterpret_cast<const uint2*>(x);
 }
 
 // ---------------------------------------------------------------- decode
@@ -660,11 +738,31 @@ moe_status_t attn_kv4_rope_write_rows(const void* qkv_bf16, int B, int nq, int n
         return MOE_ERR_INVALID_ARGUMENT;
     if (!a16(qkv_bf16) || !a16(q_out_bf16) || !a16(k_out_bf16) || !a16(k_cache) || !a16(v_cache))
         return MOE_ERR_INVALID_ARGUMENT;
-    const int groups = (nq + 2 * nkv + kWriteWarps - 1) / kWriteWarps;
-    kv4_rope_write_kernel<<<dim3(B, groups < 65535 ? groups : 65535), kWriteWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const __nv_bfloat16*>(qkv_bf16), nq, nkv, rot, inv_freq, positions, row_seq, num_seqs, page_table,
-        max_pages, num_cache_pages, static_cast<__nv_bfloat16*>(q_out_bf16), static_cast<__nv_bfloat16*>(k_out_bf16),
-        static_cast<uint8_t*>(k_cache), static_cast<uint8_t*>(v_cache), seq_lens_out, error_word);
+    WriteParams p;
+    p.qkv = static_cast<const __nv_bfloat16*>(qkv_bf16);
+    p.inv_freq = inv_freq;
+    p.positions = positions;
+    p.row_seq = row_seq;
+    p.page_table = page_table;
+    p.q_out = static_cast<__nv_bfloat16*>(q_out_bf16);
+    p.k_out = static_cast<__nv_bfloat16*>(k_out_bf16);
+    p.k_cache = static_cast<uint8_t*>(k_cache);
+    p.v_cache = static_cast<uint8_t*>(v_cache);
+    p.seq_lens_out = seq_lens_out;
+    p.error_word = error_word;
+    p.nq = nq;
+    p.nkv = nkv;
+    p.rot = rot;
+    p.num_seqs = num_seqs;
+    p.max_pages = max_pages;
+    p.num_cache_pages = num_cache_pages;
+    // a row's heads over as many blocks as it takes to fill the GPU (four blocks an SM), each warp at least one pair
+    const int most = (nq + 2 * nkv + 2 * kWriteWarps - 1) / (2 * kWriteWarps);
+    const int want = (4 * 148 + B - 1) / B;
+    const dim3 grid(B, want < most ? want : most < 65535 ? most : 65535);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (rot % 16 == 0) kv4_rope_write_kernel<true><<<grid, kWriteWarps * 32, 0, st>>>(p);
+    else kv4_rope_write_kernel<false><<<grid, kWriteWarps * 32, 0, st>>>(p);
     return launch_status();
 }
 
@@ -678,9 +776,7 @@ moe_status_t attn_kv4_read_rows(const void* k_cache, const void* v_cache, int nu
     if (B == 0 || (!k_out_bf16 && !v_out_bf16)) return MOE_OK;
     if (!positions || !page_table || (k_out_bf16 && !k_cache) || (v_out_bf16 && !v_cache)) return MOE_ERR_INVALID_ARGUMENT;
     if (!a16(k_cache) || !a16(v_cache) || !a16(k_out_bf16) || !a16(v_out_bf16)) return MOE_ERR_INVALID_ARGUMENT;
-    const long long blocks = (2ll * B * nkv + kReadWarps - 1) / kReadWarps;
-    if (blocks > 0x7FFFFFFF) return MOE_ERR_UNSUPPORTED;
-    kv4_read_kernel<<<static_cast<int>(blocks), kReadWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(
+    kv4_read_kernel<<<(B + kReadWarps - 1) / kReadWarps, kReadWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint8_t*>(k_cache), static_cast<const uint8_t*>(v_cache), num_cache_pages, positions, row_seq,
         num_seqs, page_table, max_pages, B, nkv, static_cast<__nv_bfloat16*>(k_out_bf16),
         static_cast<__nv_bfloat16*>(v_out_bf16), error_word);
