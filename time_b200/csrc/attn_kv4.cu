@@ -107,6 +107,17 @@ kv4_rope_write_kernel(const WriteParams p) {
     __shared__ float cs_s[kD / 2], sn_s[kD / 2];
     const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 15;
     const bool first = blockIdx.y == 0 && threadIdx.x == 0;
+    const int heads = p.nq + 2 * p.nkv;
+    const __nv_bfloat16* row = p.qkv + static_cast<size_t>(b) * heads * kD;
+    const int stride = gridDim.y * kWriteWarps * 2;
+    int h0 = (blockIdx.y * kWriteWarps + warp) * 2 + (lane >> 4);
+    uint4 in[kWriteUnroll];
+    auto load = [&] {
+#pragma unroll
+        for (int u = 0; u < kWriteUnroll; ++u)
+            if (h0 + u * stride < heads) in[u] = *reinterpret_cast<const uint4*>(row + static_cast<size_t>(h0 + u * stride) * kD + 8 * l);
+    };
+    load();                                          // under the position's and the page's way here
     const int pos = p.positions[b];
     const int seq = seq_of_row(p.row_seq, b, p.num_seqs);
     if (first && p.seq_lens_out) p.seq_lens_out[b] = (pos >= 0 && seq >= 0) ? pos + 1 : 0;
@@ -127,8 +138,6 @@ kv4_rope_write_kernel(const WriteParams p) {
         sincosf(static_cast<float>(pos) * p.inv_freq[i], &sn_s[i], &cs_s[i]);
     __syncthreads();
     const int t = pos % kPage;
-    const int heads = p.nq + 2 * p.nkv;
-    const __nv_bfloat16* row = p.qkv + static_cast<size_t>(b) * heads * kD;
     // this lane's dims: below half, above it, or not rotated
     const bool rotated = 8 * l < p.rot, lo = 8 * l < half;
     float cs[8], sn[8];
@@ -141,12 +150,7 @@ kv4_rope_write_kernel(const WriteParams p) {
         }
     }
     const int partner = lo ? lane + half / 8 : lane - half / 8;
-    const int stride = gridDim.y * kWriteWarps * 2;
-    for (int h0 = (blockIdx.y * kWriteWarps + warp) * 2 + (lane >> 4); h0 - (lane >> 4) < heads; h0 += stride * kWriteUnroll) {
-        uint4 in[kWriteUnroll];
-#pragma unroll
-        for (int u = 0; u < kWriteUnroll; ++u)
-            if (h0 + u * stride < heads) in[u] = *reinterpret_cast<const uint4*>(row + static_cast<size_t>(h0 + u * stride) * kD + 8 * l);
+    while (h0 - (lane >> 4) < heads) {
 #pragma unroll
         for (int u = 0; u < kWriteUnroll; ++u) {
             const int h = h0 + u * stride;
@@ -189,21 +193,27 @@ kv4_rope_write_kernel(const WriteParams p) {
             uint8_t* page = (is_k ? p.k_cache : p.v_cache) + (static_cast<size_t>(phys) * p.nkv + (kv ? kvh : 0)) * kPage4;
             quantise_store(x, page, t, l, is_k, kv);
         }
+        h0 += stride * kWriteUnroll;
+        load();
     }
 }
 
 // ---------------------------------------------------------------- read
 
 constexpr int kReadWarps = 8;
-constexpr int kReadUnroll = 8;
+constexpr int kReadUnroll = 4;
 
-// One warp per row, a half-warp per (K or V, head) with 16 bytes out a lane.
+// A warp per eight (K or V, head) tiles of a row, a half-warp per tile with 16
+// bytes out a lane.
 __global__ void __launch_bounds__(kReadWarps * 32)
 kv4_read_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, int num_cache_pages,
                 const int32_t* __restrict__ positions, const int32_t* __restrict__ row_seq, int num_seqs,
                 const int32_t* __restrict__ page_table, int max_pages, int B, int nkv,
                 __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int* __restrict__ error_word) {
-    const int b = blockIdx.x * kReadWarps + (threadIdx.x >> 5);
+    const int items = 2 * nkv;                       // K of every head, then V
+    const int parts = (items + 2 * kReadUnroll - 1) / (2 * kReadUnroll);
+    const int w = blockIdx.x * kReadWarps + (threadIdx.x >> 5);
+    const int b = w / parts;
     if (b >= B) return;
     const int lane = threadIdx.x & 31, l = lane & 15;
     const int pos = positions[b];
@@ -218,8 +228,8 @@ kv4_read_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__
     if (err && lane == 0 && error_word) atomicExch(error_word, err);
     const int t = err ? 0 : pos % kPage;
     const size_t page0 = static_cast<size_t>(err ? 0 : phys) * nkv * kPage4;
-    const int items = 2 * nkv;                       // K of every head, then V
-    for (int i0 = lane >> 4; i0 < items; i0 += 2 * kReadUnroll) {
+    {
+        const int i0 = w % parts * 2 * kReadUnroll + (lane >> 4);
         uint32_t codes[kReadUnroll], scale[kReadUnroll];
 #pragma unroll
         for (int u = 0; u < kReadUnroll; ++u) {
@@ -776,7 +786,9 @@ moe_status_t attn_kv4_read_rows(const void* k_cache, const void* v_cache, int nu
     if (B == 0 || (!k_out_bf16 && !v_out_bf16)) return MOE_OK;
     if (!positions || !page_table || (k_out_bf16 && !k_cache) || (v_out_bf16 && !v_cache)) return MOE_ERR_INVALID_ARGUMENT;
     if (!a16(k_cache) || !a16(v_cache) || !a16(k_out_bf16) || !a16(v_out_bf16)) return MOE_ERR_INVALID_ARGUMENT;
-    kv4_read_kernel<<<(B + kReadWarps - 1) / kReadWarps, kReadWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(
+    const long long warps = static_cast<long long>(B) * ((2ll * nkv + 2 * kReadUnroll - 1) / (2 * kReadUnroll));
+    if (warps > 0x7FFFFFFF - kReadWarps) return MOE_ERR_UNSUPPORTED;
+    kv4_read_kernel<<<static_cast<int>((warps + kReadWarps - 1) / kReadWarps), kReadWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint8_t*>(k_cache), static_cast<const uint8_t*>(v_cache), num_cache_pages, positions, row_seq,
         num_seqs, page_table, max_pages, B, nkv, static_cast<__nv_bfloat16*>(k_out_bf16),
         static_cast<__nv_bfloat16*>(v_out_bf16), error_word);
