@@ -102,7 +102,7 @@ __device__ __forceinline__ void quantise_store(const __nv_bfloat16 (&x)[8], uint
 // lane l +- half / 8 and a lane's cosines stay in registers; else partners come
 // from memory.
 template <bool kLanes>
-__global__ void __launch_bounds__(kWriteWarps * 32)
+__global__ void __launch_bounds__(kWriteWarps * 32, 4)
 kv4_rope_write_kernel(const WriteParams p) {
     __shared__ float cs_s[kD / 2], sn_s[kD / 2];
     const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane & 15;

@@ -89,11 +89,10 @@ __device__ __forceinline__ int owned_page(const PageParams& p, const Row& r, int
 
 constexpr int kMarkWarps = 8;
 
-__global__ void __launch_bounds__(kMarkWarps * 32)
-pages_mark_kernel(const PageParams p) {
+// Marks the pages of rows first, first + step, ...: one warp a row.
+__device__ __forceinline__ void mark_rows(const PageParams& p, int first, int step) {
     const int lane = threadIdx.x & 31;
-    const int step = gridDim.x * kMarkWarps;
-    for (int i = blockIdx.x * kMarkWarps + (threadIdx.x >> 5); i < p.num_rows; i += step) {
+    for (int i = first; i < p.num_rows; i += step) {
         const Row r = row_of(p, i, lane == 0);
         for (int j = lane; j < r.have; j += 32) {
             const int id = owned_page(p, r, j);
@@ -105,6 +104,11 @@ pages_mark_kernel(const PageParams p) {
             atomicMax(&p.keys[id], page_key(fill, r.writes && j == r.have - 1, i));
         }
     }
+}
+
+__global__ void __launch_bounds__(kMarkWarps * 32)
+pages_mark_kernel(const PageParams p) {
+    mark_rows(p, blockIdx.x * kMarkWarps + (threadIdx.x >> 5), gridDim.x * kMarkWarps);
 }
 
 // ---------------------------------------------------------------- plan
@@ -138,9 +142,8 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, u
     return x - v + (warp ? sh[warp - 1] : 0ull);
 }
 
-__global__ void __launch_bounds__(kPlanThreads)
-fork_plan_kernel(const PageParams p) {
-    __shared__ unsigned long long sh[32];
+// By one block of kPlanThreads.
+__device__ __forceinline__ void fork_plan(const PageParams& p, unsigned long long* sh) {
     unsigned long long base = 0;       // fresh pages wanted | page copies << 32
     for (int i0 = 0; i0 < p.num_rows; i0 += kPlanThreads) {
         const int i = i0 + threadIdx.x;
@@ -181,9 +184,7 @@ fork_plan_kernel(const PageParams p) {
     }
 }
 
-__global__ void __launch_bounds__(kPlanThreads)
-compact_plan_kernel(const PageParams p) {
-    __shared__ unsigned long long sh[32];
+__device__ __forceinline__ void compact_plan(const PageParams& p, unsigned long long* sh) {
     int used = 0;
     for (int q = threadIdx.x; q < p.num_pages; q += kPlanThreads) used += p.keys[q] != 0;
     unsigned long long total;
@@ -212,15 +213,8 @@ compact_plan_kernel(const PageParams p) {
 
 // ---------------------------------------------------------------- apply
 
-constexpr int kApplyThreads = 256;
-constexpr int kChunkVecs = 256;        // 16-byte pieces one warp copies at a time (4 KB, 8 in flight a lane)
-
-// Tables by all threads, then the copies: one warp per 4 KB piece of a page of
-// one cache.
-__global__ void __launch_bounds__(kApplyThreads)
-pages_apply_kernel(const PageParams p, bool fork) {
-    const long long threads = static_cast<long long>(gridDim.x) * kApplyThreads;
-    const long long tid = static_cast<long long>(blockIdx.x) * kApplyThreads + threadIdx.x;
+// Entries tid, tid + threads, ... of the result's table.
+__device__ __forceinline__ void write_table(const PageParams& p, bool fork, long long tid, long long threads) {
     const int fresh = p.counts[1];
     for (long long e = tid; e < static_cast<long long>(p.num_rows) * p.max_pages; e += threads) {
         const int i = static_cast<int>(e / p.max_pages), j = static_cast<int>(e % p.max_pages);
@@ -241,11 +235,18 @@ pages_apply_kernel(const PageParams p, bool fork) {
         }
         p.table_out[e] = id;
     }
-    const int lane = threadIdx.x & 31;
+}
+
+constexpr int kApplyThreads = 256;
+constexpr int kChunkVecs = 256;        // 16-byte pieces one warp copies at a time (4 KB, 8 in flight a lane)
+
+// The copies: one warp per 4 KB piece of a page of one cache.
+__device__ __forceinline__ void copy_pages(const PageParams& p, bool fork, long long warp, long long warps) {
+    const int fresh = p.counts[1], lane = threadIdx.x & 31;
     const int vecs = static_cast<int>(p.page_bytes / 16);
     const int chunks = (vecs + kChunkVecs - 1) / kChunkVecs;
     const long long units = static_cast<long long>(p.counts[0]) * p.num_caches * chunks;
-    for (long long u = tid / 32; u < units; u += threads / 32) {
+    for (long long u = warp; u < units; u += warps) {
         const int chunk = static_cast<int>(u % chunks);
         const int cache = static_cast<int>(u / chunks % p.num_caches);
         const int k = static_cast<int>(u / chunks / p.num_caches);
@@ -266,6 +267,52 @@ pages_apply_kernel(const PageParams p, bool fork) {
         for (int c = 0; c < kChunkVecs / 32; ++c)
             if (v0 + 32 * c < vecs) d[v0 + 32 * c] = x[c];
     }
+}
+
+template <bool kFork>
+__global__ void __launch_bounds__(kPlanThreads)
+pages_plan_kernel(const PageParams p) {
+    __shared__ unsigned long long sh[32];
+    if constexpr (kFork) fork_plan(p, sh);
+    else compact_plan(p, sh);
+}
+
+template <bool kFork>
+__global__ void __launch_bounds__(kApplyThreads)
+pages_apply_kernel(const PageParams p) {
+    const long long threads = static_cast<long long>(gridDim.x) * kApplyThreads;
+    const long long tid = static_cast<long long>(blockIdx.x) * kApplyThreads + threadIdx.x;
+    write_table(p, kFork, tid, threads);
+    copy_pages(p, kFork, tid / 32, threads / 32);
+}
+
+// Small tables and pools: keys in shared memory, everything but the copies by
+// one block, the copies' launch under it.
+constexpr int kSmallPages = 32768, kSmallEntries = 32768;
+
+template <bool kFork>
+__global__ void __launch_bounds__(kPlanThreads)
+pages_small_kernel(PageParams p) {
+    extern __shared__ __align__(16) uint32_t keys_s[];
+    __shared__ unsigned long long sh[32];
+    grid_dependents_launch();
+    p.keys = keys_s;
+    for (int q = threadIdx.x; q < p.num_pages; q += kPlanThreads) keys_s[q] = 0;
+    __syncthreads();
+    mark_rows(p, threadIdx.x >> 5, kPlanThreads / 32);
+    __syncthreads();
+    if constexpr (kFork) fork_plan(p, sh);
+    else compact_plan(p, sh);
+    __syncthreads();
+    write_table(p, kFork, threadIdx.x, kPlanThreads);
+}
+
+template <bool kFork>
+__global__ void __launch_bounds__(kApplyThreads)
+pages_copy_kernel(const PageParams p) {
+    grid_dependency_wait();
+    const long long tid = static_cast<long long>(blockIdx.x) * kApplyThreads + threadIdx.x;
+    copy_pages(p, kFork, tid / 32, static_cast<long long>(gridDim.x) * kApplyThreads / 32);
 }
 
 // ---------------------------------------------------------------- host
@@ -309,7 +356,8 @@ moe_status_t check_common(const void* caches, size_t cache_stride, int num_cache
     return MOE_OK;
 }
 
-moe_status_t run_pages(PageParams& p, void* workspace, bool fork, cudaStream_t st) {
+template <bool kFork>
+moe_status_t run_pages(PageParams& p, void* workspace, cudaStream_t st) {
     const Layout l = layout(p.num_pages, p.num_rows);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     p.keys = reinterpret_cast<uint32_t*>(ws + l.keys);
@@ -318,15 +366,23 @@ moe_status_t run_pages(PageParams& p, void* workspace, bool fork, cudaStream_t s
     p.move_dst = reinterpret_cast<int32_t*>(ws + l.dst);
     p.first_req = reinterpret_cast<int32_t*>(ws + l.first_req);
     p.counts = reinterpret_cast<int32_t*>(ws + l.counts);
+    const int copy_blocks = 148 * 4;
+    if (p.num_pages <= kSmallPages && static_cast<long long>(p.num_rows) * p.max_pages <= kSmallEntries) {
+        static bool attr[kMaxDevices] = {};
+        if (smem_optin_once(pages_small_kernel<kFork>, kSmallPages * 4, attr) != cudaSuccess) return MOE_ERR_CUDA;
+        pages_small_kernel<kFork><<<1, kPlanThreads, static_cast<size_t>(p.num_pages) * 4, st>>>(p);
+        const moe_status_t s = launch_status();
+        if (s != MOE_OK || p.num_caches == 0) return s;
+        return launch_dependent(pages_copy_kernel<kFork>, copy_blocks, kApplyThreads, st, p) == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
+    }
     if (cudaMemsetAsync(p.keys, 0, static_cast<size_t>(p.num_pages) * 4, st) != cudaSuccess) return MOE_ERR_CUDA;
     const int mark_blocks = (p.num_rows + kMarkWarps - 1) / kMarkWarps;
     pages_mark_kernel<<<mark_blocks < 1184 ? mark_blocks : 1184, kMarkWarps * 32, 0, st>>>(p);
     moe_status_t s = launch_status();
     if (s != MOE_OK) return s;
-    if (fork) fork_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
-    else compact_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
+    pages_plan_kernel<kFork><<<1, kPlanThreads, 0, st>>>(p);
     if ((s = launch_status()) != MOE_OK) return s;
-    pages_apply_kernel<<<148 * 4, kApplyThreads, 0, st>>>(p, fork);
+    pages_apply_kernel<kFork><<<copy_blocks, kApplyThreads, 0, st>>>(p);
     return launch_status();
 }
 
@@ -373,7 +429,7 @@ moe_status_t kv_pages_fork(void* caches, size_t cache_stride, int num_caches, in
     p.table_out = table_out;
     p.lens_out = lens_out;
     p.error_word = error_word;
-    return run_pages(p, workspace, true, static_cast<cudaStream_t>(stream));
+    return run_pages<true>(p, workspace, static_cast<cudaStream_t>(stream));
 }
 
 moe_status_t kv_pages_compact(void* caches, size_t cache_stride, int num_caches, int num_pages, size_t page_bytes,
@@ -402,7 +458,7 @@ moe_status_t kv_pages_compact(void* caches, size_t cache_stride, int num_caches,
     p.table_out = table_out;
     p.num_used = num_used;
     p.error_word = error_word;
-    return run_pages(p, workspace, false, static_cast<cudaStream_t>(stream));
+    return run_pages<false>(p, workspace, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
