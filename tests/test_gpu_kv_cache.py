@@ -375,7 +375,8 @@ def fork_case(rng, seqs, rows, longest, pool_extra, caches=3, words=36):
 
 
 @pytest.mark.parametrize("seqs,rows,longest,extra", [(1, 1, 1, 1), (4, 8, 100, 40), (3, 1, 50, 4), (40, 120, 300, 600),
-                                                     (5, 5, 16, 20), (7, 30, 33, 5), (2, 40, 20, 0), (600, 1500, 40, 6000)])
+                                                     (5, 5, 16, 20), (7, 30, 33, 5), (2, 40, 20, 0), (600, 1500, 40, 6000),
+                                                     (300, 1500, 400, 9000), (9, 20, 100, 40000)])
 def test_fork(gpu, seqs, rows, longest, extra):
     for seed in range(3):
         rng = np.random.default_rng(seed * 1000 + seqs)
@@ -439,7 +440,8 @@ def test_fork_no_caches_and_replay(gpu):
     assert t.tolist() == [[4, 0, -1, -1], [4, 1, -1, -1]] and n.tolist() == [16, 16]
 
 
-@pytest.mark.parametrize("seqs,longest,extra", [(1, 1, 3), (4, 100, 40), (40, 300, 500), (3, 16, 0), (600, 40, 6000)])
+@pytest.mark.parametrize("seqs,longest,extra", [(1, 1, 3), (4, 100, 40), (40, 300, 500), (3, 16, 0), (600, 40, 6000),
+                                                  (1100, 400, 4000), (9, 100, 40000)])
 def test_compact(gpu, seqs, longest, extra):
     for seed in range(3):
         rng = np.random.default_rng(seed * 77 + seqs)

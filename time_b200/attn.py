@@ -10,7 +10,6 @@ those stay exported unchanged as drop-ins.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from ctypes import c_float, c_int, c_longlong, c_size_t, c_void_p
 
@@ -21,7 +20,7 @@ from . import moe as M
 HEAD_DIM = 128
 PAGE = 16
 
-_bound = False
+_lib = None
 
 
 class BlockConfig(ctypes.Structure):
@@ -35,9 +34,9 @@ class BlockWeights(ctypes.Structure):
 
 
 def lib():
-    global _bound
-    k = M.libs()["libkernels.so"]
-    if not _bound:
+    global _lib
+    if _lib is None:
+        k = M.libs()["libkernels.so"]
         k.attn_rope_kv_write.argtypes = [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                          c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                          c_void_p]
@@ -77,8 +76,8 @@ def lib():
         k.fp8_gemm_small_workspace_bytes.restype = c_size_t
         k.fp8_gemm_small.argtypes = [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p,
                                      c_void_p, c_size_t, c_void_p]
-        _bound = True
-    return k
+        _lib = k
+    return _lib
 
 
 def rope_inv_freq(rot: int, theta: float) -> np.ndarray:
@@ -159,25 +158,24 @@ def paged_rows(q, k_cache, v_cache, page_table, row_seq, seq_lens, nq: int, nkv:
     return out, out_q, out_s
 
 
-@contextlib.contextmanager
-def on_stream(t, stream=None):
-    """The handle of `stream` (None: the current one) with torch's allocations on it.  The tensor `t` must lie on the
-    current device: a launch goes to that one."""
+def on_stream(t, stream, call, *args):
+    """call(handle of `stream`, *args) with torch's allocations on that stream (None: the current one).  The tensor `t`
+    must lie on the current device: a launch goes to that one."""
     import torch
     if t.device.index != torch.cuda.current_device():
         raise ValueError(f"tensors on {t.device}, current device {torch.cuda.current_device()}")
     if stream is None:
-        yield torch.cuda.current_stream().cuda_stream
-    else:
-        with torch.cuda.stream(stream):
-            yield stream.cuda_stream
+        return call(torch.cuda.current_stream().cuda_stream, *args)
+    with torch.cuda.stream(stream):
+        return call(stream.cuda_stream, *args)
 
 
-def check_i32(**tensors):
+def check_i32(*tensors):
     """Index tensors (or None): contiguous int32."""
-    for name, t in tensors.items():
-        if t is not None and (str(t.dtype) != "torch.int32" or not t.is_contiguous()):
-            raise ValueError(f"{name} is a contiguous int32 tensor")
+    import torch
+    for t in tensors:
+        if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()):
+            raise ValueError("positions, lengths, sequence rows, page tables and bounds are contiguous int32 tensors")
 
 
 def check_rows(name, t, dtype, width):
@@ -200,24 +198,30 @@ def prompt_packed(q, k, v, cu_seqlens, scale: float, quant: bool = False, out=No
     import torch
     for name, t in (("q", q), ("k", k), ("v", v)):
         check_heads(name, t, torch.bfloat16)
-    check_i32(cu_seqlens=cu_seqlens)
+    check_i32(cu_seqlens)
     T, nq = q.shape[:2]
     nkv = k.shape[1]
     if k.shape[0] != T or v.shape != k.shape:
         raise ValueError("q, k and v have the same rows, k and v the same heads")
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
         raise ValueError("out is a contiguous tensor like q")
-    with on_stream(q, stream) as s:
-        out = torch.empty(T, nq, HEAD_DIM, dtype=q.dtype, device=q.device) if out is None else out
-        out_q = out_s = None
-        ld = (T + 3) // 4 * 4
-        if quant:
-            out_q = torch.empty(T, nq * HEAD_DIM, dtype=torch.uint8, device=q.device)
-            out_s = torch.empty(nq, ld, dtype=torch.float32, device=q.device)
-        M.check("attn_prompt_packed", lib().attn_prompt_packed(
-            q.data_ptr(), _row_stride(q), k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v),
-            cu_seqlens.data_ptr(), max(cu_seqlens.numel() - 1, 0), T, nq, nkv, HEAD_DIM, scale, out.data_ptr(),
-            M.ptr(out_q), M.ptr(out_s), ld, M.ptr(error_word), s))
+    return on_stream(q, stream, _prompt_packed, q, k, v, cu_seqlens, scale, quant, out, error_word)
+
+
+def _prompt_packed(stream, q, k, v, cu_seqlens, scale, quant, out, error_word):
+    import torch
+    T, nq = q.shape[:2]
+    if out is None:
+        out = torch.empty(T, nq, HEAD_DIM, dtype=q.dtype, device=q.device)
+    out_q = out_s = None
+    ld = (T + 3) // 4 * 4
+    if quant:
+        out_q = torch.empty(T, nq * HEAD_DIM, dtype=torch.uint8, device=q.device)
+        out_s = torch.empty(nq, ld, dtype=torch.float32, device=q.device)
+    M.check("attn_prompt_packed", lib().attn_prompt_packed(
+        q.data_ptr(), _row_stride(q), k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v), cu_seqlens.data_ptr(),
+        max(cu_seqlens.numel() - 1, 0), T, nq, k.shape[1], HEAD_DIM, scale, out.data_ptr(), M.ptr(out_q), M.ptr(out_s), ld,
+        M.ptr(error_word), stream))
     return out, out_q, out_s
 
 

@@ -11,6 +11,7 @@ next fork.
 """
 from __future__ import annotations
 
+import functools
 from ctypes import c_float, c_int, c_size_t, c_void_p
 
 from . import attn as A
@@ -20,13 +21,13 @@ HEAD_DIM, PAGE, GROUP = A.HEAD_DIM, A.PAGE, 32
 CODE_BYTES = PAGE * HEAD_DIM // 2
 PAGE4_BYTES = CODE_BYTES + PAGE * (HEAD_DIM // GROUP) * 2      # one page of one kv head
 
-_bound = False
+_lib = None
 
 
 def lib():
-    global _bound
-    k = M.libs()["libkernels.so"]
-    if not _bound:
+    global _lib
+    if _lib is None:
+        k = M.libs()["libkernels.so"]
         k.attn_kv4_page_bytes.argtypes = [c_int]
         k.attn_kv4_page_bytes.restype = c_size_t
         k.attn_kv4_rope_write_rows.argtypes = [c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p,
@@ -47,8 +48,8 @@ def lib():
                                     c_void_p]
         k.kv_pages_compact.argtypes = [c_void_p, c_size_t, c_int, c_int, c_size_t, c_int, c_void_p, c_int, c_void_p,
                                        c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]
-        _bound = True
-    return k
+        _lib = k
+    return _lib
 
 
 def kv4_cache(num_pages: int, nkv: int, device):
@@ -58,12 +59,16 @@ def kv4_cache(num_pages: int, nkv: int, device):
 
 
 def _check_kv4(k_cache, v_cache):
-    for c in (k_cache, v_cache):
-        if c.dim() != 3 or c.shape[2] != PAGE4_BYTES or c.element_size() != 1 or not c.is_contiguous():
-            raise ValueError(f"a 4-bit cache is a contiguous uint8 tensor [pages][nkv][{PAGE4_BYTES}]")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError("k_cache and v_cache differ in shape")
-    return k_cache.shape[0], k_cache.shape[1]
+    shape = k_cache.shape
+    if len(shape) != 3 or shape[2] != PAGE4_BYTES or k_cache.element_size() != 1 or v_cache.element_size() != 1 or \
+            not k_cache.is_contiguous() or not v_cache.is_contiguous() or v_cache.shape != shape:
+        raise ValueError(f"k_cache and v_cache are contiguous uint8 tensors [pages][nkv][{PAGE4_BYTES}]")
+
+
+@functools.lru_cache(maxsize=None)
+def _splits(B: int, nkv: int, max_context: int, split_tokens: int | None, max_splits: int | None):
+    split = lib().attn_kv4_split_tokens(B, nkv, max_context) if split_tokens is None else split_tokens
+    return split, -(-max_context // split) if max_splits is None else max_splits
 
 
 def kv4_rope_write(qkv, positions, row_seq, page_table, k_cache, v_cache, nq: int, rot: int, inv_freq,
@@ -72,9 +77,9 @@ def kv4_rope_write(qkv, positions, row_seq, page_table, k_cache, v_cache, nq: in
     rotated keys bf16 [B][nkv][128] before quantisation, else None); k and v into their page slots.  row_seq None:
     row b uses page-table row b."""
     import torch
-    pages, nkv = _check_kv4(k_cache, v_cache)
-    A.check_rows("qkv", qkv, torch.bfloat16, (nq + 2 * nkv) * HEAD_DIM)
-    A.check_i32(positions=positions, row_seq=row_seq, page_table=page_table, seq_lens_out=seq_lens_out)
+    _check_kv4(k_cache, v_cache)
+    A.check_rows("qkv", qkv, torch.bfloat16, (nq + 2 * k_cache.shape[1]) * HEAD_DIM)
+    A.check_i32(positions, row_seq, page_table, seq_lens_out)
     B = qkv.shape[0]
     if positions.numel() != B or (B if row_seq is None else row_seq.numel()) != B:
         raise ValueError("positions and row_seq have one entry per row")
@@ -82,31 +87,43 @@ def kv4_rope_write(qkv, positions, row_seq, page_table, k_cache, v_cache, nq: in
         raise ValueError("inv_freq has rot / 2 entries")
     if row_seq is None and page_table.shape[0] < B:
         raise ValueError("the page table has a row per row of qkv when row_seq is None")
-    with A.on_stream(qkv, stream) as s:
-        q = torch.empty(B, nq, HEAD_DIM, dtype=torch.bfloat16, device=qkv.device)
-        k = torch.empty(B, nkv, HEAD_DIM, dtype=torch.bfloat16, device=qkv.device) if keys else None
-        M.check("attn_kv4_rope_write_rows", lib().attn_kv4_rope_write_rows(
-            M.ptr(qkv), B, nq, nkv, HEAD_DIM, rot, M.ptr(inv_freq), M.ptr(positions), M.ptr(row_seq),
-            page_table.shape[0], M.ptr(page_table), page_table.shape[1], PAGE, pages, M.ptr(q), M.ptr(k),
-            M.ptr(k_cache), M.ptr(v_cache), M.ptr(seq_lens_out), M.ptr(error_word), s))
+    return A.on_stream(qkv, stream, _rope_write, qkv, positions, row_seq, page_table, k_cache, v_cache, nq, rot, inv_freq,
+                       keys, seq_lens_out, error_word)
+
+
+def _rope_write(stream, qkv, positions, row_seq, page_table, k_cache, v_cache, nq, rot, inv_freq, keys, seq_lens_out,
+                error_word):
+    import torch
+    B, (pages, nkv, _) = qkv.shape[0], k_cache.shape
+    q = torch.empty(B, nq, HEAD_DIM, dtype=torch.bfloat16, device=qkv.device)
+    k = torch.empty(B, nkv, HEAD_DIM, dtype=torch.bfloat16, device=qkv.device) if keys else None
+    M.check("attn_kv4_rope_write_rows", lib().attn_kv4_rope_write_rows(
+        qkv.data_ptr(), B, nq, nkv, HEAD_DIM, rot, M.ptr(inv_freq), positions.data_ptr(), M.ptr(row_seq),
+        page_table.shape[0], page_table.data_ptr(), page_table.shape[1], PAGE, pages, q.data_ptr(), M.ptr(k),
+        k_cache.data_ptr(), v_cache.data_ptr(), M.ptr(seq_lens_out), M.ptr(error_word), stream))
     return q, k
 
 
 def kv4_read_rows(k_cache, v_cache, positions, row_seq, page_table, error_word=None, stream=None):
     """attn_kv4_read_rows: the tokens at `positions` of page-table rows `row_seq` as the bf16 values the cache holds:
     (k, v), each [B][nkv][128]."""
-    import torch
-    pages, nkv = _check_kv4(k_cache, v_cache)
-    A.check_i32(positions=positions, row_seq=row_seq, page_table=page_table)
+    _check_kv4(k_cache, v_cache)
+    A.check_i32(positions, row_seq, page_table)
     B = positions.numel()
     if (B if row_seq is None else row_seq.numel()) != B or (row_seq is None and page_table.shape[0] < B):
         raise ValueError("row_seq has one entry per position")
-    with A.on_stream(k_cache, stream) as s:
-        k = torch.empty(B, nkv, HEAD_DIM, dtype=torch.bfloat16, device=k_cache.device)
-        v = torch.empty_like(k)
-        M.check("attn_kv4_read_rows", lib().attn_kv4_read_rows(
-            M.ptr(k_cache), M.ptr(v_cache), pages, M.ptr(positions), M.ptr(row_seq), page_table.shape[0],
-            M.ptr(page_table), page_table.shape[1], PAGE, B, nkv, HEAD_DIM, M.ptr(k), M.ptr(v), M.ptr(error_word), s))
+    return A.on_stream(k_cache, stream, _read_rows, k_cache, v_cache, positions, row_seq, page_table, error_word)
+
+
+def _read_rows(stream, k_cache, v_cache, positions, row_seq, page_table, error_word):
+    import torch
+    B, (pages, nkv, _) = positions.numel(), k_cache.shape
+    k = torch.empty(B, nkv, HEAD_DIM, dtype=torch.bfloat16, device=k_cache.device)
+    v = torch.empty_like(k)
+    M.check("attn_kv4_read_rows", lib().attn_kv4_read_rows(
+        k_cache.data_ptr(), v_cache.data_ptr(), pages, positions.data_ptr(), M.ptr(row_seq), page_table.shape[0],
+        page_table.data_ptr(), page_table.shape[1], PAGE, B, nkv, HEAD_DIM, k.data_ptr(), v.data_ptr(), M.ptr(error_word),
+        stream))
     return k, v
 
 
@@ -116,37 +133,39 @@ def kv4_decode(q, k_cache, v_cache, page_table, seq_lens, scale: float, row_seq=
     row_seq[b] (None: b).  split_tokens None: the split that fills the GPU.  Returns (out bf16 [B][nq][128], out_q e4m3
     [B][nq * 128] or None, out_s [nq][ld] or None)."""
     import torch
-    pages, nkv = _check_kv4(k_cache, v_cache)
+    _check_kv4(k_cache, v_cache)
     A.check_heads("q", q, torch.bfloat16)
-    A.check_i32(page_table=page_table, seq_lens=seq_lens, row_seq=row_seq)
+    A.check_i32(page_table, seq_lens, row_seq)
     if not q.is_contiguous():
         raise ValueError("q is contiguous")
-    B, nq = q.shape[:2]
+    B = q.shape[0]
     if seq_lens.numel() != B or (B if row_seq is None else row_seq.numel()) != B:
         raise ValueError("seq_lens and row_seq have one entry per row of q")
     if row_seq is None and page_table.shape[0] < B:
         raise ValueError("the page table has a row per row of q when row_seq is None")
-    num_seqs, max_pages = page_table.shape
-    k = lib()
-    if split_tokens is None:
-        split_tokens = k.attn_kv4_split_tokens(B, nkv, max_pages * PAGE)
-    if max_splits is None:
-        max_splits = -(-max_pages * PAGE // split_tokens)
-    with A.on_stream(q, stream) as s:
-        if workspace is None:
-            workspace = torch.empty(max(k.attn_kv4_decode_workspace_bytes(B, nq, max_splits), 16), dtype=torch.uint8,
-                                    device=q.device)
-        out = torch.empty_like(q)
-        out_q = out_s = None
-        ld = (B + 3) // 4 * 4
-        if quant:
-            out_q = torch.empty(B, nq * HEAD_DIM, dtype=torch.uint8, device=q.device)
-            out_s = torch.empty(nq, ld, dtype=torch.float32, device=q.device)
-        M.check("attn_kv4_decode_rows", k.attn_kv4_decode_rows(
-            M.ptr(q), M.ptr(k_cache), M.ptr(v_cache), pages, M.ptr(page_table), max_pages, M.ptr(row_seq), num_seqs,
-            M.ptr(seq_lens), B, nq, nkv, HEAD_DIM, PAGE, scale, split_tokens, max_splits, M.ptr(workspace),
-            workspace.numel() * workspace.element_size(), M.ptr(out), M.ptr(out_q), M.ptr(out_s), ld,
-            M.ptr(error_word), s))
+    return A.on_stream(q, stream, _decode, q, k_cache, v_cache, page_table, seq_lens, scale, row_seq, split_tokens,
+                       max_splits, quant, workspace, error_word)
+
+
+def _decode(stream, q, k_cache, v_cache, page_table, seq_lens, scale, row_seq, split_tokens, max_splits, quant, workspace,
+            error_word):
+    import torch
+    (B, nq, _), (pages, nkv, _), (num_seqs, max_pages) = q.shape, k_cache.shape, page_table.shape
+    split_tokens, max_splits = _splits(B, nkv, max_pages * PAGE, split_tokens, max_splits)
+    if workspace is None:
+        need = max(lib().attn_kv4_decode_workspace_bytes(B, nq, max_splits), 16)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    out = torch.empty_like(q)
+    out_q = out_s = None
+    ld = (B + 3) // 4 * 4
+    if quant:
+        out_q = torch.empty(B, nq * HEAD_DIM, dtype=torch.uint8, device=q.device)
+        out_s = torch.empty(nq, ld, dtype=torch.float32, device=q.device)
+    M.check("attn_kv4_decode_rows", lib().attn_kv4_decode_rows(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), pages, page_table.data_ptr(), max_pages, M.ptr(row_seq),
+        num_seqs, seq_lens.data_ptr(), B, nq, nkv, HEAD_DIM, PAGE, scale, split_tokens, max_splits, workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), out.data_ptr(), M.ptr(out_q), M.ptr(out_s), ld, M.ptr(error_word),
+        stream))
     return out, out_q, out_s
 
 
@@ -154,10 +173,15 @@ def kv4_decode(q, k_cache, v_cache, page_table, seq_lens, scale: float, row_seq=
 
 def _cache_args(caches):
     """(pointer, bytes between caches, caches, pages, bytes of a page) of a tensor [caches][pages][...]."""
-    if caches.dim() < 3 or not caches[0].is_contiguous():
+    shape, stride, e = caches.shape, caches.stride(), caches.element_size()
+    inner = 1
+    for n, st in zip(reversed(shape[1:]), reversed(stride[1:])):
+        if n != 1 and st != inner:
+            raise ValueError("caches is a tensor [caches][pages][...] with every cache contiguous")
+        inner *= n
+    if len(shape) < 3:
         raise ValueError("caches is a tensor [caches][pages][...] with every cache contiguous")
-    e = caches.element_size()
-    return M.ptr(caches), caches.stride(0) * e, caches.shape[0], caches.shape[1], caches.stride(1) * e
+    return caches.data_ptr(), stride[0] * e, shape[0], shape[1], inner // max(shape[1], 1) * e
 
 
 def _check_table(table, lens):
@@ -169,43 +193,47 @@ def fork_pages(caches, table, lens, parents, reserve=None, workspace=None, error
     """kv_pages_fork: row i of the result is row parents[i] (-1: empty) with room for reserve[i] more tokens; full
     pages are shared, a page in part filled is copied for all appending rows but one.  Returns (table, lens) int32,
     new tensors."""
-    import torch
-    A.check_i32(table=table, lens=lens, parents=parents, reserve=reserve)
+    A.check_i32(table, lens, parents, reserve)
     _check_table(table, lens)
     if reserve is not None and reserve.numel() != parents.numel():
         raise ValueError("reserve has one entry per parent")
+    return A.on_stream(caches, stream, _fork, caches, table, lens, parents, reserve, workspace, error_word)
+
+
+def _fork(stream, caches, table, lens, parents, reserve, workspace, error_word):
+    import torch
     ptr, stride, n, pages, page_bytes = _cache_args(caches)
-    rows, k = parents.numel(), lib()
-    with A.on_stream(caches, stream) as s:
-        if workspace is None:
-            workspace = torch.empty(k.kv_pages_workspace_bytes(pages, rows), dtype=torch.uint8, device=caches.device)
-        out = torch.empty(rows, table.shape[1], dtype=torch.int32, device=caches.device)
-        lens_out = torch.empty(rows, dtype=torch.int32, device=caches.device)
-        M.check("kv_pages_fork", k.kv_pages_fork(
-            ptr, stride, n, pages, page_bytes, PAGE, M.ptr(table), table.shape[1], M.ptr(lens), table.shape[0],
-            M.ptr(parents), M.ptr(reserve), rows, M.ptr(out), M.ptr(lens_out), M.ptr(workspace),
-            workspace.numel() * workspace.element_size(), M.ptr(error_word), s))
+    rows, max_pages = parents.numel(), table.shape[1]
+    if workspace is None:
+        workspace = torch.empty(lib().kv_pages_workspace_bytes(pages, rows), dtype=torch.uint8, device=caches.device)
+    out = torch.empty(rows, max_pages, dtype=torch.int32, device=caches.device)
+    lens_out = torch.empty(rows, dtype=torch.int32, device=caches.device)
+    M.check("kv_pages_fork", lib().kv_pages_fork(
+        ptr, stride, n, pages, page_bytes, PAGE, table.data_ptr(), max_pages, lens.data_ptr(), table.shape[0],
+        parents.data_ptr(), M.ptr(reserve), rows, out.data_ptr(), lens_out.data_ptr(), workspace.data_ptr(),
+        workspace.numel() * workspace.element_size(), M.ptr(error_word), stream))
     return out, lens_out
 
 
 def compact_pages(caches, table, lens, out=None, workspace=None, error_word=None, stream=None):
     """kv_pages_compact: moves the pages in use to the lowest ids.  Returns (table, pages in use int32 [1]); `out` may
     be `table` itself."""
-    import torch
-    A.check_i32(table=table, lens=lens, out=out)
+    A.check_i32(table, lens, out)
     _check_table(table, lens)
     if out is not None and out.shape != table.shape:
         raise ValueError("out has the page table's shape")
+    return A.on_stream(caches, stream, _compact, caches, table, lens, out, workspace, error_word)
+
+
+def _compact(stream, caches, table, lens, out, workspace, error_word):
+    import torch
     ptr, stride, n, pages, page_bytes = _cache_args(caches)
-    k = lib()
-    with A.on_stream(caches, stream) as s:
-        if workspace is None:
-            workspace = torch.empty(k.kv_pages_workspace_bytes(pages, table.shape[0]), dtype=torch.uint8,
-                                    device=caches.device)
-        out = torch.empty_like(table) if out is None else out
-        used = torch.empty(1, dtype=torch.int32, device=caches.device)
-        M.check("kv_pages_compact", k.kv_pages_compact(
-            ptr, stride, n, pages, page_bytes, PAGE, M.ptr(table), table.shape[1], M.ptr(lens), table.shape[0],
-            M.ptr(out), M.ptr(used), M.ptr(workspace), workspace.numel() * workspace.element_size(),
-            M.ptr(error_word), s))
+    seqs, max_pages = table.shape
+    if workspace is None:
+        workspace = torch.empty(lib().kv_pages_workspace_bytes(pages, seqs), dtype=torch.uint8, device=caches.device)
+    out = torch.empty_like(table) if out is None else out
+    used = torch.empty(1, dtype=torch.int32, device=caches.device)
+    M.check("kv_pages_compact", lib().kv_pages_compact(
+        ptr, stride, n, pages, page_bytes, PAGE, table.data_ptr(), max_pages, lens.data_ptr(), seqs, out.data_ptr(),
+        used.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(), M.ptr(error_word), stream))
     return out, used
