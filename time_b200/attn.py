@@ -162,10 +162,12 @@ def on_stream(t, stream, call, *args):
     """call(handle of `stream`, *args) with torch's allocations on that stream (None: the current one).  The tensor `t`
     must lie on the current device: a launch goes to that one."""
     import torch
-    if t.device.index != torch.cuda.current_device():
+    device = t.device.index
+    if device != torch.cuda.current_device():
         raise ValueError(f"tensors on {t.device}, current device {torch.cuda.current_device()}")
     if stream is None:
-        return call(torch.cuda.current_stream().cuda_stream, *args)
+        # the handle of torch.cuda.current_stream() without the object, which takes longer than the launch's arguments
+        return call(torch._C._cuda_getCurrentRawStream(device), *args)
     with torch.cuda.stream(stream):
         return call(stream.cuda_stream, *args)
 
