@@ -804,8 +804,9 @@ int attn_kv4_split_tokens(int B, int nkv, int max_context) {
     if (max_context <= 512) return (max_context + kPage - 1) / kPage * kPage;
     long long split = static_cast<long long>(B) * nkv * max_context / (2 * 444);
     if (split > 1536) split = split / 2 < 2048 ? split / 2 : 2048;
-    split = (split + kPage - 1) / kPage * kPage;
-    return static_cast<int>(split < 256 ? 256 : split);
+    constexpr int kTurn = 2 * kPage * kWarps;      // a page pair for every warp
+    split = (split + kTurn / 2) / kTurn * kTurn;
+    return static_cast<int>(split < 2 * kTurn ? 2 * kTurn : split);
 }
 
 size_t attn_kv4_decode_workspace_bytes(int B, int nq, int max_splits) {
