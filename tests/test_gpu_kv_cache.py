@@ -272,6 +272,34 @@ def test_decode_first_split_all_minus_infinity(gpu):
     assert (np.abs(f64(out)[0] - ref) <= tol + 1e-6).all()
 
 
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 0.02, 2.0])
+def test_decode_scales(gpu, scale):
+    rng = np.random.default_rng(13)
+    kc, vc = random_cache(rng, 30, 2)
+    pt, lens = table_of(rng, [250, 100], 30), [250, 100]
+    q = normal_bf16(rng, 2, 8, D)
+    out = f64(KV.kv4_decode(q.to(gpu), torch.from_numpy(kc).to(gpu), torch.from_numpy(vc).to(gpu), i32(pt, gpu),
+                            i32(lens, gpu), scale, split_tokens=64)[0])
+    for b, n in enumerate(lens):
+        ref, tol = R.attend(f64(-q[b:b + 1] if scale < 0 else q[b:b + 1]), seq_values(kc, "k", pt[b], n),
+                            seq_values(vc, "v", pt[b], n), [n], abs(scale))
+        assert (np.abs(out[b] - ref[0]) <= tol[0]).all()
+
+
+def test_empty_batches(gpu):
+    kc = KV.kv4_cache(2, 1, gpu)
+    none = i32([], gpu)
+    table = torch.zeros(0, 3, dtype=torch.int32, device=gpu)
+    q = torch.zeros(0, 4, D, dtype=torch.bfloat16, device=gpu)
+    assert KV.kv4_decode(q, kc, kc, table, none, 0.1)[0].shape == (0, 4, D)
+    x = torch.zeros(0, 6 * D, dtype=torch.bfloat16, device=gpu)
+    f = torch.zeros(32, device=gpu)
+    assert KV.kv4_rope_write(x, none, None, table, kc, kc, 4, 64, f)[0].shape == (0, 4, D)
+    assert KV.kv4_read_rows(kc, kc, none, None, table)[0].shape == (0, 1, D)
+    t, n = KV.fork_pages(kc[None], i32([[0]], gpu), i32([1], gpu), none)
+    assert t.shape == (0, 1) and n.numel() == 0
+
+
 def test_decode_bounds(gpu):
     rng = np.random.default_rng(9)
     kc, vc = random_cache(rng, 4, 1)

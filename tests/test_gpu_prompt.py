@@ -27,6 +27,8 @@ def cu_of(lens, gpu, first=0):
 def check(out, q, k, v, lens, scale, first=0):
     at = first
     for n in lens:
+        if n == 0:
+            continue
         s = slice(at, at + n)
         ref, tol = R.attend(f64(q[s]), f64(k[s]), f64(v[s]), np.arange(1, n + 1), scale)
         got = f64(out[s])
@@ -234,3 +236,34 @@ def test_many_uneven_prompts(gpu):
             assert (np.abs(f64(out[s]) - ref) <= tol).all()
         at += n
     assert torch.equal(out, A.prompt_packed(q, k, v, cu_of(lens, gpu), 0.1)[0])
+
+
+def test_more_sequences_than_a_warp(gpu):
+    """Sequences of none, one and several tiles in an order that mixes them, past the 32 that are counted in registers."""
+    rng = np.random.default_rng(12)
+    nq, nkv = 4, 2
+    lens = [int(x) for x in rng.choice([0, 1, 3, 17, 127, 128, 129, 300], 150)]
+    T = sum(lens)
+    q, k, v = rows(rng, T, nq, D).to(gpu), rows(rng, T, nkv, D).to(gpu), rows(rng, T, nkv, D).to(gpu)
+    out = torch.full((T + 5, nq, D), 7.0, dtype=torch.bfloat16, device=gpu)[:T]
+    A.prompt_packed(q, k, v, cu_of(lens, gpu), 0.1, out=out)
+    check(out, q, k, v, lens, 0.1)
+    # 5000 one-token prompts: every row is its value
+    q, k, v = rows(rng, 5000, nq, D).to(gpu), rows(rng, 5000, nkv, D).to(gpu), rows(rng, 5000, nkv, D).to(gpu)
+    out = A.prompt_packed(q, k, v, torch.arange(5001, dtype=torch.int32, device=gpu), 0.1)[0]
+    assert torch.equal(out, v.repeat_interleave(nq // nkv, dim=1))
+
+
+def test_two_calls_at_once(gpu):
+    """The same buffers attended on two streams at the same time."""
+    rng = np.random.default_rng(13)
+    lens = [900, 40, 300]
+    T = sum(lens)
+    q, k, v = rows(rng, T, 16, D).to(gpu), rows(rng, T, 4, D).to(gpu), rows(rng, T, 4, D).to(gpu)
+    want = A.prompt_packed(q, k, v, cu_of(lens, gpu), 0.1)[0]
+    cu = cu_of(lens, gpu)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[A.prompt_packed(q, k, v, cu, 0.1, stream=s)[0] for s in streams] for _ in range(5)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for pair in outs for o in pair)

@@ -741,9 +741,9 @@ moe_status_t attn_kv4_rope_write_rows(const void* qkv_bf16, int B, int nq, int n
                                       int num_cache_pages, void* q_out_bf16, void* k_out_bf16, void* k_cache,
                                       void* v_cache, int32_t* seq_lens_out, int* error_word, cwStream_t stream) {
     if (B < 0 || nq <= 0 || nkv <= 0 || nq % nkv || head_dim != kD || page_size != kPage) return MOE_ERR_INVALID_ARGUMENT;
-    if (num_cache_pages <= 0 || num_seqs <= 0) return MOE_ERR_INVALID_ARGUMENT;
-    if (rot < 0 || rot > kD || rot % 2 || max_pages <= 0) return MOE_ERR_INVALID_ARGUMENT;
+    if (num_cache_pages <= 0 || rot < 0 || rot > kD || rot % 2 || max_pages <= 0) return MOE_ERR_INVALID_ARGUMENT;
     if (B == 0) return MOE_OK;
+    if (num_seqs <= 0) return MOE_ERR_INVALID_ARGUMENT;
     if (!qkv_bf16 || (rot > 0 && !inv_freq) || !positions || !page_table || !q_out_bf16 || !k_cache || !v_cache)
         return MOE_ERR_INVALID_ARGUMENT;
     if (!a16(qkv_bf16) || !a16(q_out_bf16) || !a16(k_out_bf16) || !a16(k_cache) || !a16(v_cache))
@@ -780,10 +780,10 @@ moe_status_t attn_kv4_read_rows(const void* k_cache, const void* v_cache, int nu
                                 const int32_t* positions, const int32_t* row_seq, int num_seqs,
                                 const int32_t* page_table, int max_pages, int page_size, int B, int nkv, int head_dim,
                                 void* k_out_bf16, void* v_out_bf16, int* error_word, cwStream_t stream) {
-    if (B < 0 || nkv <= 0 || head_dim != kD || page_size != kPage || num_cache_pages <= 0 || num_seqs <= 0 ||
-        max_pages <= 0)
+    if (B < 0 || nkv <= 0 || head_dim != kD || page_size != kPage || num_cache_pages <= 0 || max_pages <= 0)
         return MOE_ERR_INVALID_ARGUMENT;
     if (B == 0 || (!k_out_bf16 && !v_out_bf16)) return MOE_OK;
+    if (num_seqs <= 0) return MOE_ERR_INVALID_ARGUMENT;
     if (!positions || !page_table || (k_out_bf16 && !k_cache) || (v_out_bf16 && !v_cache)) return MOE_ERR_INVALID_ARGUMENT;
     if (!a16(k_cache) || !a16(v_cache) || !a16(k_out_bf16) || !a16(v_out_bf16)) return MOE_ERR_INVALID_ARGUMENT;
     const long long warps = static_cast<long long>(B) * ((2ll * nkv + 2 * kReadUnroll - 1) / (2 * kReadUnroll));
@@ -820,7 +820,7 @@ moe_status_t attn_kv4_decode_rows(const void* q_bf16, const void* k_cache, const
                                   float scale, int split_tokens, int max_splits, void* workspace,
                                   size_t workspace_bytes, void* out_bf16, void* out_q, float* out_s, int out_ld,
                                   int* error_word, cwStream_t stream) {
-    if (B < 0 || num_seqs <= 0 || nq <= 0 || nkv <= 0 || nq % nkv || nq / nkv > kGPad || head_dim != kD ||
+    if (B < 0 || nq <= 0 || nkv <= 0 || nq % nkv || nq / nkv > kGPad || head_dim != kD ||
         page_size != kPage)
         return MOE_ERR_INVALID_ARGUMENT;
     if (split_tokens <= 0 || split_tokens % kPage || split_tokens > kMaxSplitPages * kPage || max_splits <= 0 ||
@@ -828,6 +828,7 @@ moe_status_t attn_kv4_decode_rows(const void* q_bf16, const void* k_cache, const
         return MOE_ERR_INVALID_ARGUMENT;
     if (static_cast<long long>(B) * nkv > 65535 || static_cast<long long>(B) * nq > 0x7FFFFFFF) return MOE_ERR_UNSUPPORTED;
     if (B == 0) return MOE_OK;
+    if (num_seqs <= 0) return MOE_ERR_INVALID_ARGUMENT;
     if (!q_bf16 || !k_cache || !v_cache || !page_table || !seq_lens || !workspace || !out_bf16)
         return MOE_ERR_INVALID_ARGUMENT;
     if (!a16(q_bf16) || !a16(k_cache) || !a16(v_cache) || !a16(workspace)) return MOE_ERR_INVALID_ARGUMENT;

@@ -47,65 +47,79 @@ struct Tile {
     bool some;
 };
 
-// Tiles of `span` positions in the order of (tile index, descending; sequence).  From
-// the first bound that is out of order or range on there are no sequences, so
-// no two overlap.  Used by one warp.
+// Tiles of `span` positions in the order of (tile index, descending; sequence),
+// asked for in ascending numbers by one warp.  From the first bound that is out
+// of order or range on there are no sequences, so no two overlap.  Up to 32
+// sequences are counted in registers and a tile is found by bisection over the
+// indices; more are walked 32 at a time from the last tile found, so that the
+// whole run walks each index's sequences once.
 struct TileOrder {
     const PromptParams& p;
-    int span, lane, seqs, most;    // positions of a tile; sequences, tiles of the longest
-    int own;                       // tiles of sequence `lane`: the first 32 stay in a register
+    int span, lane, seqs;          // positions of a tile; sequences
+    int own;                       // tiles of sequence `lane`
+    int most;                      // tiles of the longest sequence
+    int level, s0;                 // walk: tile index and first of the 32 sequences looked at,
+    unsigned int before;           // and the tiles that come before them
 
-    __device__ __forceinline__ int count(int s) const {
+    __device__ __forceinline__ int tiles(int s) const {
         return s < seqs ? (p.cu_seqlens[s + 1] - p.cu_seqlens[s] + span - 1) / span : 0;
     }
-    __device__ __forceinline__ int tiles(int s0) const { return s0 == 0 ? own : count(s0 + lane); }
 
     __device__ __forceinline__ TileOrder(const PromptParams& params, int positions, bool report)
-        : p(params), span(positions), lane(threadIdx.x & 31), seqs(params.num_seqs), most(0) {
+        : p(params), span(positions), lane(threadIdx.x & 31), seqs(params.num_seqs), most(0), s0(0), before(0) {
         for (int s = lane; s < p.num_seqs; s += 32) {
             const int a = p.cu_seqlens[s], b = p.cu_seqlens[s + 1];
             if (a < 0 || b < a || b > p.T) seqs = min(seqs, s);
         }
         seqs = __reduce_min_sync(0xffffffffu, seqs);
         if (seqs < p.num_seqs && report && lane == 0 && p.error_word) atomicExch(p.error_word, 5);
-        own = count(lane);
-        for (int s0 = 0; s0 < seqs; s0 += 32) most = max(most, tiles(s0));
+        own = tiles(lane);
+        most = own;
+        for (int s = lane + 32; s < seqs; s += 32) most = max(most, tiles(s));
         most = __reduce_max_sync(0xffffffffu, most);
+        level = most - 1;
     }
 
-    // tiles with an index of at least x; all together are below 2^31
-    __device__ __forceinline__ unsigned int at_least(int x) const {
-        unsigned int sum = 0;
-        for (int s0 = 0; s0 < seqs; s0 += 32) sum += max(tiles(s0) - x, 0);
-        return __reduce_add_sync(0xffffffffu, sum);
+    // Sequence number `skip` of those in `m`, the sequences from s on with a tile `index`.
+    __device__ __forceinline__ Tile pick(uint32_t m, int skip, int s, int index) const {
+        const uint32_t hit = __ballot_sync(0xffffffffu, (m >> lane & 1) && __popc(m & ((1u << lane) - 1u)) == skip);
+        s += __ffs(hit) - 1;
+        Tile t;
+        t.first = p.cu_seqlens[s];
+        t.len = p.cu_seqlens[s + 1] - t.first;
+        t.index = index;
+        t.some = true;
+        return t;
     }
 
     // Tile number c, the same in every lane.
-    __device__ __forceinline__ Tile find(unsigned int c) const {
-        Tile t = {0, 0, 0, false};
-        if (c >= at_least(0)) return t;
-        int lo = 0, hi = most;         // at_least(lo) > c, at_least(hi) <= c
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (at_least(mid) > c) lo = mid;
-            else hi = mid;
-        }
-        int skip = static_cast<int>(c - at_least(lo + 1));
-        for (int s0 = 0; s0 < seqs; s0 += 32) {
-            const bool has = tiles(s0) > lo;
-            const uint32_t m = __ballot_sync(0xffffffffu, has);
-            const uint32_t hit = __ballot_sync(0xffffffffu, has && __popc(m & ((1u << lane) - 1u)) == skip);
-            if (hit) {
-                const int s = s0 + __ffs(hit) - 1;
-                t.first = p.cu_seqlens[s];
-                t.len = p.cu_seqlens[s + 1] - t.first;
-                t.index = lo;
-                t.some = true;
-                return t;
+    __device__ __forceinline__ Tile find(unsigned int c) {
+        const Tile none = {0, 0, 0, false};
+        if (seqs <= 32) {
+            // tiles with an index of at least x; all together are below 2^31
+            auto at_least = [&](int x) { return __reduce_add_sync(0xffffffffu, static_cast<unsigned int>(max(own - x, 0))); };
+            if (c >= at_least(0)) return none;
+            int lo = 0, hi = most;     // at_least(lo) > c, at_least(hi) <= c
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (at_least(mid) > c) lo = mid;
+                else hi = mid;
             }
-            skip -= __popc(m);
+            const uint32_t m = __ballot_sync(0xffffffffu, own > lo);
+            return pick(m, static_cast<int>(c - at_least(lo + 1)), 0, lo);
         }
-        return t;
+        while (level >= 0) {
+            const uint32_t m = __ballot_sync(0xffffffffu, tiles(s0 + lane) > level);
+            const unsigned int n = __popc(m);
+            if (c - before < n) return pick(m, static_cast<int>(c - before), s0, level);
+            before += n;
+            s0 += 32;
+            if (s0 >= seqs) {
+                s0 = 0;
+                --level;
+            }
+        }
+        return none;
     }
 };
 
@@ -596,7 +610,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         }
     } else if (warp == 14) {
         // ---- tiles; Q, and K and V of keys 0.., 128.. of every tile
-        const TileOrder order(p, tile_pos, blockIdx.x == 0);
+        TileOrder order(p, tile_pos, blockIdx.x == 0);
         int item = 0, q_n = 0;
         bool ok = true;
         for (int n = 0; ok; ++n) {

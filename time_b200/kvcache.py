@@ -65,7 +65,7 @@ def _check_kv4(k_cache, v_cache):
         raise ValueError(f"k_cache and v_cache are contiguous uint8 tensors [pages][nkv][{PAGE4_BYTES}]")
 
 
-@functools.lru_cache(maxsize=None)
+@functools.lru_cache(maxsize=1024)
 def _splits(B: int, nkv: int, max_context: int, split_tokens: int | None, max_splits: int | None):
     split = lib().attn_kv4_split_tokens(B, nkv, max_context) if split_tokens is None else split_tokens
     return split, -(-max_context // split) if max_splits is None else max_splits
