@@ -107,7 +107,7 @@ moe_status_t attn_paged_rows(const void* q_bf16, const void* k_cache, const void
  * [T][nq][128] and k, v bf16 rows of nkv heads; consecutive rows lie q_stride,
  * k_stride, v_stride elements apart (multiples of 8, so v may stay inside the
  * qkv projection's rows); 16-byte aligned.  out_bf16 [T][nq][128], out_q and
- * out_s as in attn_decode_paged, both outputs 32-byte aligned.  Rows in no sequence are left as they were.
+ * out_s as in attn_decode_paged, out_q 32-byte aligned.  Rows in no sequence are left as they were.
  * From the first bound that is out of order or outside 0..T on, sequences are
  * skipped (*error_word = 5).  A NaN or infinity in k or v reaches the rows that attend
  * it and no others. */

@@ -123,16 +123,14 @@ struct TileOrder {
     }
 };
 
-// Zeroes the NaN and infinite elements of eight bf16 values; true if any.
-__device__ __forceinline__ bool zero_nonfinite(uint4& v) {
+// Zeroes the NaN and infinite elements of eight bf16 values.
+__device__ __forceinline__ void zero_nonfinite(uint4& v) {
     uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-    bool any = false;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        if ((w[i] & 0x7F80u) == 0x7F80u) { w[i] &= 0xFFFF0000u; any = true; }
-        if ((w[i] & 0x7F800000u) == 0x7F800000u) { w[i] &= 0x0000FFFFu; any = true; }
+        if ((w[i] & 0x7F80u) == 0x7F80u) w[i] &= 0xFFFF0000u;
+        if ((w[i] & 0x7F800000u) == 0x7F800000u) w[i] &= 0x0000FFFFu;
     }
-    return any;
 }
 
 // ---------------------------------------------------------------- kernel
@@ -164,9 +162,13 @@ constexpr int kStages = 4;                              // K and V tiles in flig
 constexpr int kThreads = 512;
 constexpr uint32_t kHalf = kKeys * 128;                 // 64 dims of a 128-row tile: rows of 128 bytes, swizzled
 constexpr uint32_t kTileBytes = 2 * kHalf;
-constexpr size_t kSmem = 2 * kTileBytes + kStages * kTileBytes + 1024;
+constexpr uint32_t kOutBytes = 128 * kD * 2;            // output rows of an M tile
+constexpr size_t kSmem = 2 * kTileBytes + kStages * kTileBytes + kOutBytes + 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kTileReaders = 8 + 4 + 2 + 1;             // softmax, epilogue, MMA warps and the cleaner
+
+// A tile is at most 256 positions (one head a group): masked steps, and ring stages with V of them.
+constexpr int kMaskedSteps = 5, kMaskedItems = 3;
 
 // A tile as the load warp hands it to the others.
 struct TileWork {
@@ -187,7 +189,9 @@ struct Bars {
     uint64_t full[kStages], empty[kStages];             // ring of K0 V0 K1 V1 ...
     uint64_t s_full[2][2], p_full[2][2];                // [M tile][score buffer]
     uint64_t pv_done[2], o_full[2], o_free[2];
-    uint64_t tile_full[2], tile_empty[2], q_full, q_empty, go, clean, drain[2];
+    uint64_t tile_full[2], tile_empty[2], q_full, q_empty, drain[2];
+    // V with masked positions, by the tile's slot; every one of them completes once a tile, so its phase is the slot's
+    uint64_t v_full[2][kMaskedItems], clean[2][kMaskedSteps];
 };
 
 // Bounded wait that reads the clock and the abort flag every 256 tries only: a
@@ -286,6 +290,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* q_s = sm;                                  // [2 halves][256 rows][128 B]
     uint8_t* kv_s = sm + 2 * kTileBytes;                // [stages][2 halves][128][128 B]
+    uint8_t* out_sm = kv_s + kStages * kTileBytes;      // [128][256 B], chunks of 16 swizzled by row
     __shared__ Bars bars;
     __shared__ TileWork tile_s[2];
     __shared__ float l_s[kRows];                        // row sums
@@ -312,8 +317,10 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         }
         mbar_init(&bars.q_full, 1);
         mbar_init(&bars.q_empty, 2);
-        mbar_init(&bars.go, 2);
-        mbar_init(&bars.clean, 32);
+        for (int t = 0; t < 2; ++t) {
+            for (int i = 0; i < kMaskedItems; ++i) mbar_init(&bars.v_full[t][i], 1);
+            for (int i = 0; i < kMaskedSteps; ++i) mbar_init(&bars.clean[t][i], 1);
+        }
         abort_s = 0;
         fence_mbar_init();
         prefetch_tmap(&qmap);
@@ -492,21 +499,33 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     }
                     if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
                 }
-                uint32_t wt[4][16];
+                // Rows go through shared memory, a warp's own 32, so that a store instruction covers two whole rows and not
+                // a sector of each of 32.
+                uint8_t* mine = out_sm + (threadIdx.x & 127) * 256;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float x[32];
                     columns(c, x);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) wt[c][e] = pack_bf16(x[2 * e], x[2 * e + 1]);
+                    for (int e = 0; e < 4; ++e)
+                        *reinterpret_cast<uint4*>(mine + (((4 * c + e) ^ (lane & 15)) << 4)) =
+                            make_uint4(pack_bf16(x[8 * e], x[8 * e + 1]), pack_bf16(x[8 * e + 2], x[8 * e + 3]),
+                                       pack_bf16(x[8 * e + 4], x[8 * e + 5]), pack_bf16(x[8 * e + 6], x[8 * e + 7]));
                 }
                 tc_fence_before();
                 mbar_arrive(&bars.o_free[t]);           // the next tile may write its output
-                if (store)                              // whole 32-byte sectors
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) st_global_32(p.out + out_row * kD + 32 * c + 16 * e, wt[c] + 8 * e);
+                __syncwarp();
+                const int in_warp = (warp & 3) * 32;    // the warp's first row of the M tile
+#pragma unroll 4
+                for (int r = lane >> 4; r < 32; r += 2) {
+                    const int i = t * 128 + in_warp + r;
+                    if (i >= rows) break;
+                    const int row_at = group_div(i, g_inv);
+                    const uint4 x = *reinterpret_cast<const uint4*>(out_sm + (in_warp + r) * 256 + (((lane & 15) ^ (r & 15)) << 4));
+                    *reinterpret_cast<uint4*>(p.out + ((first + pos0 + row_at) * p.nq + kvh * p.G + i - row_at * p.G) * kD +
+                                              (lane & 15) * 8) = x;
+                }
+                __syncwarp();                           // before the next M tile's rows
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.tile_empty[n & 1]);
@@ -522,7 +541,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         const uint32_t q_lo = desc_lo_k(smem_u32(q_s)) + t * (kHalf >> 4);
         const uint32_t k_lo = desc_lo_k(smem_u32(kv_s)), v_lo = desc_lo_mn(smem_u32(kv_s), kHalf);
         int item = 0, stage = 0;                        // ring items of the tiles before, and their stage
-        int tiles = 0, masked = 0;                      // tiles of this M tile, masked steps of all tiles
+        int tiles = 0;                                  // tiles of this M tile
         uint32_t p_phase = 0;                           // of p_full[t][b], bit b
         auto stage_of = [&](int ahead) { return (stage + ahead) % kStages; };
         auto wait_item = [&](int ahead) { return all(wait(&bars.full[stage_of(ahead)], ((item + ahead) / kStages) & 1)); };
@@ -538,16 +557,18 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 for (int i = 0; i < (steps + 1) / 2 * 2 && ok; ++i) {
                     if (!(ok = wait_item(i))) break;
                     if (el) mbar_arrive(&bars.empty[stage_of(i)]);
-                    for (int j = i - 1; (i & 1) && j <= i && ok; ++j)      // the steps of V item i
-                        if (j < steps && j >= first_masked) {
-                            if (el) mbar_arrive(&bars.go);
-                            ok = all(wait(&bars.clean, masked++ & 1));
-                        }
                 }
                 if (ok && !(ok = all(wait(&bars.q_full, n & 1)))) break;
                 if (el) mbar_arrive(&bars.q_empty);
             } else {
                 int k_at = 0;                           // K item of the scores issued next, from the tile's first
+                const uint32_t slot_phase = (n >> 1) & 1;
+                // V of step j, cleaned where it has to be
+                auto wait_v = [&](int j, int ahead) {
+                    if (j >= first_masked) return all(wait(&bars.clean[n & 1][j - first_masked], slot_phase));
+                    if (j / 2 >= first_masked / 2) return all(wait(&bars.v_full[n & 1][j / 2 - first_masked / 2], slot_phase));
+                    return wait_item(ahead);
+                };
                 auto scores = [&](int j) {              // S of step j into buffer j % 2
                     const int st = stage_of(k_at);
                     const uint32_t id_s = idesc_bf16_f32(128, j + 1 == steps ? last : kStep, false) | negate;
@@ -568,15 +589,16 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 tc_fence_after();
                 scores(0);
                 if (steps > 1) scores(1);
-                if (!(ok = wait_item(1) && all(wait(&bars.o_free[t], (tiles++ & 1) ^ 1)))) break;
+                if (!(ok = all(wait(&bars.o_free[t], (tiles++ & 1) ^ 1)))) break;
                 bool ready = false;                     // what a test for the next weights gave, under the MMAs before
                 for (int j = 0; j < steps; ++j) {
-                    const int st = stage_of(j / 2 * 2 + 1);
-                    const bool clean = j >= first_masked;
-                    if (clean && el) mbar_arrive(&bars.go);
+                    const int v_at = j / 2 * 2 + 1, st = stage_of(v_at);
+                    if (!wait_v(j, v_at)) {
+                        ok = false;
+                        break;
+                    }
                     if (!all(ready) && !(ok = all(wait(&bars.p_full[t][j & 1], (p_phase >> (j & 1)) & 1)))) break;
                     p_phase ^= 1u << (j & 1);
-                    if (clean && !(ok = all(wait(&bars.clean, masked++ & 1)))) break;
                     tc_fence_after();
                     const uint32_t v = v_lo + st * (kTileBytes >> 4) + (j & 1) * (kStep * 128 >> 4);
                     const uint32_t pa = tm + (j & 1) * kStep;
@@ -591,7 +613,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     }
                     if ((j & 1) || j + 1 == steps) umma_commit_warp(&bars.empty[st]);
                     if (j + 2 < steps) {
-                        if (!(j & 1) && !(ok = wait_item(k_at) && wait_item(k_at + 1))) break;     // K of step j + 2, V for its product
+                        if (!(j & 1) && !(ok = wait_item(k_at))) break;     // K of step j + 2
                         ready = mbar_test(&bars.p_full[t][(j + 1) & 1], (p_phase >> ((j + 1) & 1)) & 1);
                         scores(j + 2);
                     } else {
@@ -620,7 +642,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             const int kvh = static_cast<int>(c % p.nkv);
             if (lane == 0) {
                 ok = wait(&bars.tile_empty[n & 1], ((n >> 1) & 1) ^ 1);
-                int loads = 0, pos0 = 0;
+                int loads = 0, pos0 = 0, masked0 = 0, armed = 0;
                 if (ok) {
                     TileWork w;
                     w.some = tl.some;
@@ -633,6 +655,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     w.steps = tl.some ? pos1 / kStep + 1 : 0;
                     w.last = (pos1 % kStep + 16) / 16 * 16;
                     w.first_masked = (w.pos0 + 1) / kStep;
+                    masked0 = w.first_masked / 2;
                     w.dirty = 0;
                     loads = (w.steps + 1) / 2 * 2;
                     tile_s[n & 1] = w;
@@ -651,12 +674,19 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     if (!(ok = wait(&bars.empty[st], ((item / kStages) & 1) ^ 1))) break;
                     uint8_t* dst = kv_s + st * kTileBytes;
                     const int y = tl.first + j / 2 * kKeys;
-                    mbar_arrive_expect_tx(&bars.full[st], kTileBytes);
+                    // V that has to be cleaned lands at a barrier of its own; the ring's only keeps its phase
+                    const bool to_clean = (j & 1) && j / 2 >= masked0;
+                    uint64_t* bar = to_clean ? &bars.v_full[n & 1][j / 2 - masked0] : &bars.full[st];
+                    if (to_clean) mbar_arrive(&bars.full[st]);
+                    mbar_arrive_expect_tx(bar, kTileBytes);
                     const CUtensorMap* map = (j & 1) ? &vmap : &kmap;
-                    tma_load_2d(map, &bars.full[st], dst, x, y);
-                    tma_load_2d(map, &bars.full[st], dst + kHalf, x + 64, y);
+                    tma_load_2d(map, bar, dst, x, y);
+                    tma_load_2d(map, bar, dst + kHalf, x + 64, y);
                     ++item;
+                    if (to_clean) armed = j / 2 - masked0 + 1;
                 }
+                if (ok)
+                    for (int i = armed; i < kMaskedItems; ++i) mbar_arrive(&bars.v_full[n & 1][i]);
                 if (ok && n && loads == 2) {            // no item behind the first K and V
                     if ((ok = wait(&bars.q_empty, (n & 1) ^ 1))) {
                         mbar_arrive_expect_tx(&bars.q_full, tile_pos * p.G * 256);
@@ -667,6 +697,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 }
                 if (!ok) {   // loads in flight land before the block leaves
                     for (int i = max(item - kStages, 0); i < item; ++i) mbar_drain(&bars.full[i % kStages], (i / kStages) & 1);
+                    for (int i = 0; i < armed; ++i) mbar_drain(&bars.v_full[n & 1][i], (n >> 1) & 1);
                     if (q_n) mbar_drain(&bars.q_full, (q_n - 1) & 1);
                 }
             }
@@ -674,34 +705,44 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         }
     } else {
         // ---- a weight of 0 must meet a finite value: V of positions that not every row attends
-        int masked = 0, item = 0;
+        int item = 0;
         bool ok = true;
         for (int n = 0; ok; ++n) {
             if (!(ok = all(wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
             TileWork& w = tile_s[n & 1];
             if (!w.some) break;
-            const int steps = w.steps;
-            for (int i = w.first_masked; i < steps; ++i) {
-                const int vi = item + i / 2 * 2 + 1;
-                ok = wait(&bars.go, masked++ & 1) && wait(&bars.full[vi % kStages], (vi / kStages) & 1);
-                if (!(ok = all(ok))) break;
-                uint8_t* v = kv_s + vi % kStages * kTileBytes + (i & 1) * (kStep * 128);
+            const int steps = w.steps, first_masked = w.first_masked, masked0 = first_masked / 2;
+            for (int i = first_masked; i < steps; ++i) {
+                if (!(ok = all(wait(&bars.v_full[n & 1][i / 2 - masked0], (n >> 1) & 1)))) break;
+                uint8_t* v = kv_s + (item + i / 2 * 2 + 1) % kStages * kTileBytes + (i & 1) * (kStep * 128);
                 const int j0 = max(w.pos0 + 1 - i * kStep, 0);       // first such row of the step
                 const int j1 = i + 1 == steps ? w.last : kStep;
-                bool dirty = false;
+                auto at = [&](int c) {
+                    return reinterpret_cast<uint4*>(v + (c & 1) * kHalf + (j0 + (c >> 4)) * 128 + ((c >> 1) & 7) * 16);
+                };
+                // an exponent of all ones carries into the sign's place
+                uint32_t found = 0;
 #pragma unroll 8
                 for (int c = lane; c < (j1 - j0) * 16; c += 32) {
-                    uint4* at = reinterpret_cast<uint4*>(v + (c & 1) * kHalf + (j0 + (c >> 4)) * 128 + ((c >> 1) & 7) * 16);
-                    uint4 x = *at;
-                    if (zero_nonfinite(x)) {
-                        *at = x;
-                        dirty = true;
+                    const uint4 x = *at(c);
+                    found |= ((x.x & 0x7F807F80u) + 0x00800080u) | ((x.y & 0x7F807F80u) + 0x00800080u) |
+                             ((x.z & 0x7F807F80u) + 0x00800080u) | ((x.w & 0x7F807F80u) + 0x00800080u);
+                }
+                if (found & 0x80008000u) {
+                    w.dirty = 1;
+                    for (int c = lane; c < (j1 - j0) * 16; c += 32) {
+                        uint4 x = *at(c);
+                        zero_nonfinite(x);
+                        *at(c) = x;
                     }
                 }
-                if (dirty) w.dirty = 1;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&bars.clean);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars.clean[n & 1][i - first_masked]);
             }
+            if (!ok) break;
+            if (lane == 0)
+                for (int i = max(steps - first_masked, 0); i < kMaskedSteps; ++i) mbar_arrive(&bars.clean[n & 1][i]);
             item += (steps + 1) / 2 * 2;
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.tile_empty[n & 1]);
@@ -771,9 +812,8 @@ moe_status_t attn_prompt_packed(const void* q_bf16, long long q_stride, const vo
         return MOE_ERR_INVALID_ARGUMENT;
     if (T == 0 || num_seqs == 0) return MOE_OK;
     if (!q_bf16 || !k_bf16 || !v_bf16 || !cu_seqlens || !out_bf16) return MOE_ERR_INVALID_ARGUMENT;
-    auto a32 = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 31) == 0; };
-    if (!a16(q_bf16) || !a16(k_bf16) || !a16(v_bf16) || !a32(out_bf16)) return MOE_ERR_INVALID_ARGUMENT;
-    if (out_q && (!out_s || out_ld < T || !a32(out_q))) return MOE_ERR_INVALID_ARGUMENT;
+    if (!a16(q_bf16) || !a16(k_bf16) || !a16(v_bf16) || !a16(out_bf16)) return MOE_ERR_INVALID_ARGUMENT;
+    if (out_q && (!out_s || out_ld < T || (reinterpret_cast<uintptr_t>(out_q) & 31))) return MOE_ERR_INVALID_ARGUMENT;
     PromptParams p;
     p.q = static_cast<const __nv_bfloat16*>(q_bf16);
     p.k = static_cast<const __nv_bfloat16*>(k_bf16);
