@@ -150,25 +150,31 @@ __device__ __forceinline__ void zero_nonfinite(uint4& v) {
 // of scores and 2 x 128 of output.  The running maximum is left behind by up to
 // 2^8 before the output is rescaled, so a rescale is rare and the softmax threads
 // do it themselves.  An M tile's MMAs have a warp of their own, so that what one
-// spends between MMAs (barriers, descriptors) is covered by the other's.  The
-// next tile's loads, scores and softmax run under a tile's epilogue.
+// spends between MMAs (barriers, descriptors) is covered by the other's.  Steps
+// run on from tile to tile: with Q in two buffers, the next tile's first scores
+// are issued under the last weights of a tile, and its output rows leave through
+// the buffer of the queries that are done with.
 
 constexpr int kSms = 148;
 constexpr int kRows = 256;
-constexpr int kKeys = 128;                              // of a ring stage
-constexpr int kStep = 64;                               // of a softmax step
+constexpr int kStep = 64;                               // keys of a softmax step and of a ring stage
 constexpr int kFmaPairs = 2;                            // pairs of eight whose exponentials go to the FMA pipe
-constexpr int kStages = 4;                              // K and V tiles in flight, 32 KB each
+constexpr int kStages = 6;                              // K and V tiles in flight, 16 KB each
 constexpr int kThreads = 512;
-constexpr uint32_t kHalf = kKeys * 128;                 // 64 dims of a 128-row tile: rows of 128 bytes, swizzled
+constexpr uint32_t kHalf = kStep * 128;                 // 64 dims of a 64-key tile: rows of 128 bytes, swizzled
 constexpr uint32_t kTileBytes = 2 * kHalf;
-constexpr uint32_t kOutBytes = 128 * kD * 2;            // output rows of an M tile
-constexpr size_t kSmem = 2 * kTileBytes + kStages * kTileBytes + kOutBytes + 1024;
+constexpr uint32_t kQHalf = kRows * 128;                // 64 dims of the queries
+constexpr uint32_t kQBytes = 2 * kQHalf;
+constexpr size_t kSmem = 2 * kQBytes + kStages * kTileBytes + 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
 constexpr int kTileReaders = 8 + 4 + 2 + 1;             // softmax, epilogue, MMA warps and the cleaner
 
-// A tile is at most 256 positions (one head a group): masked steps, and ring stages with V of them.
-constexpr int kMaskedSteps = 5, kMaskedItems = 3;
+// A tile is at most 256 positions (one head a group): steps with masked ones.
+constexpr int kMaskedSteps = 5;
+
+// Ring items of a tile: K0 K1 V0 K2 V1 .. in the order of their MMAs.
+__device__ __forceinline__ int k_item(int j) { return j ? 2 * j - 1 : 0; }
+__device__ __forceinline__ int v_item(int j, int steps) { return min(2 * j + 2, 2 * steps - 1); }
 
 // A tile as the load warp hands it to the others.
 struct TileWork {
@@ -186,12 +192,12 @@ struct TileWork {
 __device__ __forceinline__ int group_div(int x, uint32_t g_inv) { return static_cast<int>(static_cast<uint32_t>(x) * g_inv >> 16); }
 
 struct Bars {
-    uint64_t full[kStages], empty[kStages];             // ring of K0 V0 K1 V1 ...
+    uint64_t full[kStages], empty[kStages];             // ring of K and V
     uint64_t s_full[2][2], p_full[2][2];                // [M tile][score buffer]
     uint64_t pv_done[2], o_full[2], o_free[2];
-    uint64_t tile_full[2], tile_empty[2], q_full, q_empty, drain[2];
+    uint64_t tile_full[2], tile_empty[2], q_full[2], drain[2];      // by the tile's slot; an empty slot's Q is empty
     // V with masked positions, by the tile's slot; every one of them completes once a tile, so its phase is the slot's
-    uint64_t v_full[2][kMaskedItems], clean[2][kMaskedSteps];
+    uint64_t v_full[2][kMaskedSteps], clean[2][kMaskedSteps];
 };
 
 // Bounded wait that reads the clock and the abort flag every 256 tries only: a
@@ -288,9 +294,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
               const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ uint8_t sm_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint8_t* q_s = sm;                                  // [2 halves][256 rows][128 B]
-    uint8_t* kv_s = sm + 2 * kTileBytes;                // [stages][2 halves][128][128 B]
-    uint8_t* out_sm = kv_s + kStages * kTileBytes;      // [128][256 B], chunks of 16 swizzled by row
+    uint8_t* q_s = sm;                                  // [2 slots][2 halves][256 rows][128 B]
+    uint8_t* kv_s = sm + 2 * kQBytes;                   // [stages][2 halves][64][128 B]
     __shared__ Bars bars;
     __shared__ TileWork tile_s[2];
     __shared__ float l_s[kRows];                        // row sums
@@ -315,11 +320,12 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             mbar_init(&bars.tile_empty[t], kTileReaders);
             mbar_init(&bars.drain[t], 1);
         }
-        mbar_init(&bars.q_full, 1);
-        mbar_init(&bars.q_empty, 2);
         for (int t = 0; t < 2; ++t) {
-            for (int i = 0; i < kMaskedItems; ++i) mbar_init(&bars.v_full[t][i], 1);
-            for (int i = 0; i < kMaskedSteps; ++i) mbar_init(&bars.clean[t][i], 1);
+            mbar_init(&bars.q_full[t], 1);
+            for (int i = 0; i < kMaskedSteps; ++i) {
+                mbar_init(&bars.v_full[t][i], 1);
+                mbar_init(&bars.clean[t][i], 1);
+            }
         }
         abort_s = 0;
         fence_mbar_init();
@@ -345,8 +351,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         const uint32_t ts = tmem + (static_cast<uint32_t>(warp & 3) << 21) + t * 128;   // this warp's 32 lanes
         const uint32_t to = ts + 256;
         const float sl2 = p.scale_log2;
-        uint32_t s_phase = 0;                           // of s_full[t][b], bit b
-        int pv_n = 0, tiles = 0;                        // steps and tiles of this M tile so far
+        int g = 0, tiles = 0;                           // steps and tiles of this M tile so far
         bool ok = true;
         for (int n = 0; ok; ++n) {
             if (!(ok = all(wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
@@ -355,11 +360,11 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             if (t < w.mt) {
                 const int steps = w.steps, first_masked = w.first_masked;
                 const int pos = w.pos0 + group_div(min(i_row, w.rows - 1), g_inv);
+                const bool used = i_row < w.rows;
                 float m = -INFINITY, l = 0.0f;
-                for (int j = 0; j < steps; ++j, ++pv_n) {
-                    const uint32_t sb = ts + (j & 1) * kStep;
-                    if (!(ok = all(wait(&bars.s_full[t][j & 1], (s_phase >> (j & 1)) & 1)))) break;
-                    s_phase ^= 1u << (j & 1);
+                for (int j = 0; j < steps; ++j, ++g) {
+                    const uint32_t sb = ts + (g & 1) * kStep;
+                    if (!(ok = all(wait(&bars.s_full[t][g & 1], (g >> 1) & 1)))) break;
                     tc_fence_after();
                     uint32_t s[2][32];
 #pragma unroll
@@ -384,13 +389,13 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     if (j == 0) {
                         m = mt;
                     } else {
-                        const bool need = !((mt - m) * sl2 <= 8.0f) && mt != m;
+                        const bool need = !((mt - m) * sl2 <= 8.0f) && mt != m && used;
                         if (__any_sync(0xffffffffu, need)) {
                             const float f = need ? ex2((m - mt) * sl2) : 1.0f;
                             l *= f;
                             if (need) m = mt;
                             // the product of the step before has to be in
-                            if (!(ok = all(wait(&bars.pv_done[t], (pv_n - 1) & 1)))) break;
+                            if (!(ok = all(wait(&bars.pv_done[t], (g - 1) & 1)))) break;
                             tc_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < 8; ++c) {
@@ -431,7 +436,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     }
                     tmem_wait_st();
                     tc_fence_before();
-                    mbar_arrive(&bars.p_full[t][j & 1]);
+                    mbar_arrive(&bars.p_full[t][g & 1]);
                 }
                 ++tiles;
             }
@@ -499,34 +504,34 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     }
                     if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
                 }
-                // Rows go through shared memory, a warp's own 32, so that a store instruction covers two whole rows and not
-                // a sector of each of 32.
-                uint8_t* mine = out_sm + (threadIdx.x & 127) * 256;
+                // Rows go through shared memory, in place of the warp's own 32 queries, so that a store instruction covers
+                // two whole rows and not a sector of each of 32.
+                uint8_t* rows_sm = q_s + (n & 1) * kQBytes;         // 16-byte chunk c of row i
+                auto chunk = [&](int i, int c) {
+                    return reinterpret_cast<uint4*>(rows_sm + (c >> 3) * kQHalf + i * 128 + (((c ^ i) & 7) << 4));
+                };
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float x[32];
                     columns(c, x);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        *reinterpret_cast<uint4*>(mine + (((4 * c + e) ^ (lane & 15)) << 4)) =
+                        *chunk(i_row, 4 * c + e) =
                             make_uint4(pack_bf16(x[8 * e], x[8 * e + 1]), pack_bf16(x[8 * e + 2], x[8 * e + 3]),
                                        pack_bf16(x[8 * e + 4], x[8 * e + 5]), pack_bf16(x[8 * e + 6], x[8 * e + 7]));
                 }
                 tc_fence_before();
                 mbar_arrive(&bars.o_free[t]);           // the next tile may write its output
                 __syncwarp();
-                const int in_warp = (warp & 3) * 32;    // the warp's first row of the M tile
+                const int row0 = t * 128 + (warp & 3) * 32;
 #pragma unroll 4
-                for (int r = lane >> 4; r < 32; r += 2) {
-                    const int i = t * 128 + in_warp + r;
-                    if (i >= rows) break;
+                for (int i = row0 + (lane >> 4); i < min(rows, row0 + 32); i += 2) {
                     const int row_at = group_div(i, g_inv);
-                    const uint4 x = *reinterpret_cast<const uint4*>(out_sm + (in_warp + r) * 256 + (((lane & 15) ^ (r & 15)) << 4));
                     *reinterpret_cast<uint4*>(p.out + ((first + pos0 + row_at) * p.nq + kvh * p.G + i - row_at * p.G) * kD +
-                                              (lane & 15) * 8) = x;
+                                              (lane & 15) * 8) = *chunk(i, lane & 15);
                 }
-                __syncwarp();                           // before the next M tile's rows
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // before the slot's next queries
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.tile_empty[n & 1]);
         }
@@ -538,70 +543,67 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         const uint32_t negate = p.flip_q ? 1u << 13 : 0u;      // of A
         constexpr uint32_t id_o = idesc_bf16_f32(128, kD, true);
         const uint32_t tm = uni(tmem) + t * 128;
-        const uint32_t q_lo = desc_lo_k(smem_u32(q_s)) + t * (kHalf >> 4);
+        const uint32_t q_lo = desc_lo_k(smem_u32(q_s)) + t * (128 * 128 >> 4);
         const uint32_t k_lo = desc_lo_k(smem_u32(kv_s)), v_lo = desc_lo_mn(smem_u32(kv_s), kHalf);
-        int item = 0, stage = 0;                        // ring items of the tiles before, and their stage
-        int tiles = 0;                                  // tiles of this M tile
-        uint32_t p_phase = 0;                           // of p_full[t][b], bit b
-        auto stage_of = [&](int ahead) { return (stage + ahead) % kStages; };
-        auto wait_item = [&](int ahead) { return all(wait(&bars.full[stage_of(ahead)], ((item + ahead) / kStages) & 1)); };
+        auto wait_item = [&](int x) { return all(wait(&bars.full[x % kStages], (x / kStages) & 1)); };
+        int n = 0, base = 0, tiles = 0, g = 0;          // tile, its first ring item; tiles and products of this M tile so far
+        // scores, up to two steps before the products and at most one tile
+        int sn = -1, sj = 0, s_steps = 0, s_last = 0, s_base = 0, sg = 0;
+        auto scores = [&](int next, int next_base) {    // `next`: the tile that comes after this run of scores
+            while (sg - g < 2) {
+                if (sj == s_steps) {
+                    if (sn >= next) return true;
+                    if (!all(wait(&bars.tile_full[next & 1], (next >> 1) & 1))) return false;
+                    const TileWork& w = tile_s[next & 1];
+                    if (!uni(w.some) || t >= uni(w.mt)) return true;
+                    if (!all(wait(&bars.q_full[next & 1], (next >> 1) & 1))) return false;
+                    sn = next;
+                    sj = 0;
+                    s_steps = uni(w.steps);
+                    s_last = uni(w.last);
+                    s_base = next_base;
+                }
+                const int x = s_base + k_item(sj), st = x % kStages;
+                if (!wait_item(x)) return false;
+                tc_fence_after();
+                const uint32_t id_s = idesc_bf16_f32(128, sj + 1 == s_steps ? s_last : kStep, false) | negate;
+                const uint32_t q = q_lo + (sn & 1) * (kQBytes >> 4), k = k_lo + st * (kTileBytes >> 4);
+                const uint32_t d = tm + (sg & 1) * kStep;
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks)
+                    umma_f16_warp(d, q + (ks >> 2) * (kQHalf >> 4) + (ks & 3) * 2, k + (ks >> 2) * (kHalf >> 4) + (ks & 3) * 2,
+                                  id_s, ks > 0);
+                umma_commit_warp(&bars.s_full[t][sg & 1]);
+                umma_commit_warp(&bars.empty[st]);
+                ++sj;
+                ++sg;
+            }
+            return true;
+        };
         bool ok = true;
-        for (int n = 0; ok; ++n) {
+        for (; ok; ++n) {
             if (!(ok = all(wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
             const TileWork& slot = tile_s[n & 1];
             if (!uni(slot.some)) break;
             const int steps = uni(slot.steps), last = uni(slot.last), first_masked = uni(slot.first_masked);
-            const bool active = t < uni(slot.mt);
-            if (!active) {
-                // the other M tile has it alone: this warp only keeps the counts of the barriers that both arrive on
-                for (int i = 0; i < (steps + 1) / 2 * 2 && ok; ++i) {
-                    if (!(ok = wait_item(i))) break;
-                    if (el) mbar_arrive(&bars.empty[stage_of(i)]);
-                }
-                if (ok && !(ok = all(wait(&bars.q_full, n & 1)))) break;
-                if (el) mbar_arrive(&bars.q_empty);
+            if (t >= uni(slot.mt)) {
+                // the other M tile has it alone: this warp only keeps the counts of the ring
+                for (int x = base; x < base + 2 * steps && ok; ++x)
+                    if ((ok = wait_item(x)) && el) mbar_arrive(&bars.empty[x % kStages]);
+                if (!ok) break;
             } else {
-                int k_at = 0;                           // K item of the scores issued next, from the tile's first
                 const uint32_t slot_phase = (n >> 1) & 1;
-                // V of step j, cleaned where it has to be
-                auto wait_v = [&](int j, int ahead) {
-                    if (j >= first_masked) return all(wait(&bars.clean[n & 1][j - first_masked], slot_phase));
-                    if (j / 2 >= first_masked / 2) return all(wait(&bars.v_full[n & 1][j / 2 - first_masked / 2], slot_phase));
-                    return wait_item(ahead);
-                };
-                auto scores = [&](int j) {              // S of step j into buffer j % 2
-                    const int st = stage_of(k_at);
-                    const uint32_t id_s = idesc_bf16_f32(128, j + 1 == steps ? last : kStep, false) | negate;
-                    const uint32_t k = k_lo + st * (kTileBytes >> 4) + (j & 1) * (kStep * 128 >> 4);
-                    const uint32_t d = tm + (j & 1) * kStep;
-#pragma unroll
-                    for (int ks = 0; ks < 8; ++ks)
-                        umma_f16_warp(d, q_lo + (ks >> 2) * (2 * kHalf >> 4) + (ks & 3) * 2,
-                                      k + (ks >> 2) * (kHalf >> 4) + (ks & 3) * 2, id_s, ks > 0);
-                    umma_commit_warp(&bars.s_full[t][j & 1]);
-                    if ((j & 1) || j + 1 == steps) {
-                        umma_commit_warp(&bars.empty[st]);
-                        k_at += 2;
-                        if (j + 1 == steps) umma_commit_warp(&bars.q_empty);
-                    }
-                };
-                if (!(ok = all(wait(&bars.q_full, n & 1)) && wait_item(0))) break;
-                tc_fence_after();
-                scores(0);
-                if (steps > 1) scores(1);
-                if (!(ok = all(wait(&bars.o_free[t], (tiles++ & 1) ^ 1)))) break;
+                if (!(ok = scores(n, base) && all(wait(&bars.o_free[t], (tiles++ & 1) ^ 1)))) break;
                 bool ready = false;                     // what a test for the next weights gave, under the MMAs before
                 for (int j = 0; j < steps; ++j) {
-                    const int v_at = j / 2 * 2 + 1, st = stage_of(v_at);
-                    if (!wait_v(j, v_at)) {
-                        ok = false;
-                        break;
-                    }
-                    if (!all(ready) && !(ok = all(wait(&bars.p_full[t][j & 1], (p_phase >> (j & 1)) & 1)))) break;
-                    p_phase ^= 1u << (j & 1);
+                    const int x = base + v_item(j, steps), st = x % kStages;
+                    // V, cleaned where it has to be
+                    ok = j < first_masked ? wait_item(x) : all(wait(&bars.clean[n & 1][j - first_masked], slot_phase));
+                    if (!ok) break;
+                    if (!all(ready) && !(ok = all(wait(&bars.p_full[t][g & 1], (g >> 1) & 1)))) break;
                     tc_fence_after();
-                    const uint32_t v = v_lo + st * (kTileBytes >> 4) + (j & 1) * (kStep * 128 >> 4);
-                    const uint32_t pa = tm + (j & 1) * kStep;
+                    const uint32_t v = v_lo + st * (kTileBytes >> 4);
+                    const uint32_t pa = tm + (g & 1) * kStep;
                     const int ksteps = j + 1 == steps ? last / 16 : kStep / 16;
 #pragma unroll
                     for (int ks = 0; ks < kStep / 16; ++ks)     // 16 keys: 16 rows of 128 bytes
@@ -611,19 +613,13 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                         if (el) mbar_arrive(&bars.o_full[t]);   // the cleaner's word on the tile and the row sums go with it
                         umma_commit_warp(&bars.o_full[t]);
                     }
-                    if ((j & 1) || j + 1 == steps) umma_commit_warp(&bars.empty[st]);
-                    if (j + 2 < steps) {
-                        if (!(j & 1) && !(ok = wait_item(k_at))) break;     // K of step j + 2
-                        ready = mbar_test(&bars.p_full[t][(j + 1) & 1], (p_phase >> ((j + 1) & 1)) & 1);
-                        scores(j + 2);
-                    } else {
-                        ready = false;
-                    }
+                    umma_commit_warp(&bars.empty[st]);
+                    ++g;
+                    ready = j + 1 < steps && mbar_test(&bars.p_full[t][g & 1], (g >> 1) & 1);
+                    if (!(ok = scores(n + 1, base + 2 * steps))) break;
                 }
             }
-            const int used = (steps + 1) / 2 * 2;
-            item += used;
-            stage = (stage + used) % kStages;
+            base += 2 * steps;
             if (el) mbar_arrive(&bars.tile_empty[n & 1]);
         }
         if (!ok) {
@@ -633,7 +629,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
     } else if (warp == 14) {
         // ---- tiles; Q, and K and V of keys 0.., 128.. of every tile
         TileOrder order(p, tile_pos, blockIdx.x == 0);
-        int item = 0, q_n = 0;
+        int item = 0;
+        int armed[2] = {0, 0}, q_tiles = 0;             // V barriers with a copy, by slot; tiles whose Q is loaded
         bool ok = true;
         for (int n = 0; ok; ++n) {
             // every other round backwards: a CTA's tiles even out
@@ -642,63 +639,57 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             const int kvh = static_cast<int>(c % p.nkv);
             if (lane == 0) {
                 ok = wait(&bars.tile_empty[n & 1], ((n >> 1) & 1) ^ 1);
-                int loads = 0, pos0 = 0, masked0 = 0, armed = 0;
                 if (ok) {
                     TileWork w;
                     w.some = tl.some;
                     w.kvh = kvh;
                     w.first = tl.first;
-                    w.pos0 = pos0 = tl.index * tile_pos;
+                    w.pos0 = tl.index * tile_pos;
                     w.rows = min(tile_pos, tl.len - w.pos0) * p.G;
                     w.mt = w.rows > 128 ? 2 : 1;
                     const int pos1 = min(w.pos0 + tile_pos, tl.len) - 1;
                     w.steps = tl.some ? pos1 / kStep + 1 : 0;
                     w.last = (pos1 % kStep + 16) / 16 * 16;
                     w.first_masked = (w.pos0 + 1) / kStep;
-                    masked0 = w.first_masked / 2;
                     w.dirty = 0;
-                    loads = (w.steps + 1) / 2 * 2;
                     tile_s[n & 1] = w;
                     mbar_arrive(&bars.tile_full[n & 1]);
-                }
-                const int x = kvh * kD;
-                for (int j = 0; j < loads && ok; ++j) {
-                    if (j == (n ? 2 : 0)) {             // behind the first K and V, which need not wait for the last tile's Q
-                        if (!(ok = wait(&bars.q_empty, (n & 1) ^ 1))) break;
-                        mbar_arrive_expect_tx(&bars.q_full, tile_pos * p.G * 256);
-                        tma_load_3d(&qmap, &bars.q_full, q_s, 0, kvh * p.G, tl.first + pos0);
-                        tma_load_3d(&qmap, &bars.q_full, q_s + 2 * kHalf, 64, kvh * p.G, tl.first + pos0);
-                        ++q_n;
-                    }
-                    const int st = item % kStages;
-                    if (!(ok = wait(&bars.empty[st], ((item / kStages) & 1) ^ 1))) break;
-                    uint8_t* dst = kv_s + st * kTileBytes;
-                    const int y = tl.first + j / 2 * kKeys;
-                    // V that has to be cleaned lands at a barrier of its own; the ring's only keeps its phase
-                    const bool to_clean = (j & 1) && j / 2 >= masked0;
-                    uint64_t* bar = to_clean ? &bars.v_full[n & 1][j / 2 - masked0] : &bars.full[st];
-                    if (to_clean) mbar_arrive(&bars.full[st]);
-                    mbar_arrive_expect_tx(bar, kTileBytes);
-                    const CUtensorMap* map = (j & 1) ? &vmap : &kmap;
-                    tma_load_2d(map, bar, dst, x, y);
-                    tma_load_2d(map, bar, dst + kHalf, x + 64, y);
-                    ++item;
-                    if (to_clean) armed = j / 2 - masked0 + 1;
-                }
-                if (ok)
-                    for (int i = armed; i < kMaskedItems; ++i) mbar_arrive(&bars.v_full[n & 1][i]);
-                if (ok && n && loads == 2) {            // no item behind the first K and V
-                    if ((ok = wait(&bars.q_empty, (n & 1) ^ 1))) {
-                        mbar_arrive_expect_tx(&bars.q_full, tile_pos * p.G * 256);
-                        tma_load_3d(&qmap, &bars.q_full, q_s, 0, kvh * p.G, tl.first + pos0);
-                        tma_load_3d(&qmap, &bars.q_full, q_s + 2 * kHalf, 64, kvh * p.G, tl.first + pos0);
-                        ++q_n;
+                    armed[n & 1] = 0;
+                    if (w.some) {
+                        const int x = kvh * kD;
+                        auto load = [&](const CUtensorMap* map, int j, uint64_t* own_bar) {
+                            const int st = item % kStages;
+                            if (!(ok = wait(&bars.empty[st], ((item / kStages) & 1) ^ 1))) return;
+                            // V that has to be cleaned lands at a barrier of its own; the ring's only keeps its phase
+                            uint64_t* bar = own_bar ? own_bar : &bars.full[st];
+                            if (own_bar) mbar_arrive(&bars.full[st]);
+                            mbar_arrive_expect_tx(bar, kTileBytes);
+                            uint8_t* dst = kv_s + st * kTileBytes;
+                            tma_load_2d(map, bar, dst, x, w.first + j * kStep);
+                            tma_load_2d(map, bar, dst + kHalf, x + 64, w.first + j * kStep);
+                            ++item;
+                            if (own_bar) ++armed[n & 1];
+                        };
+                        uint8_t* q = q_s + (n & 1) * kQBytes;
+                        mbar_arrive_expect_tx(&bars.q_full[n & 1], tile_pos * p.G * 256);
+                        tma_load_3d(&qmap, &bars.q_full[n & 1], q, 0, kvh * p.G, w.first + w.pos0);
+                        tma_load_3d(&qmap, &bars.q_full[n & 1], q + kQHalf, 64, kvh * p.G, w.first + w.pos0);
+                        q_tiles = n + 1;
+                        load(&kmap, 0, nullptr);
+                        for (int j = 0; j < w.steps && ok; ++j) {
+                            if (j + 1 < w.steps) load(&kmap, j + 1, nullptr);
+                            if (ok) load(&vmap, j, j < w.first_masked ? nullptr : &bars.v_full[n & 1][j - w.first_masked]);
+                        }
+                        if (ok)
+                            for (int i = armed[n & 1]; i < kMaskedSteps; ++i) mbar_arrive(&bars.v_full[n & 1][i]);
                     }
                 }
                 if (!ok) {   // loads in flight land before the block leaves
                     for (int i = max(item - kStages, 0); i < item; ++i) mbar_drain(&bars.full[i % kStages], (i / kStages) & 1);
-                    for (int i = 0; i < armed; ++i) mbar_drain(&bars.v_full[n & 1][i], (n >> 1) & 1);
-                    if (q_n) mbar_drain(&bars.q_full, (q_n - 1) & 1);
+                    for (int m = max(q_tiles - 2, 0); m < q_tiles; ++m) {
+                        mbar_drain(&bars.q_full[m & 1], (m >> 1) & 1);
+                        for (int i = 0; i < armed[m & 1]; ++i) mbar_drain(&bars.v_full[m & 1][i], (m >> 1) & 1);
+                    }
                 }
             }
             ok = __shfl_sync(0xffffffffu, ok, 0) && tl.some;
@@ -711,10 +702,10 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             if (!(ok = all(wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
             TileWork& w = tile_s[n & 1];
             if (!w.some) break;
-            const int steps = w.steps, first_masked = w.first_masked, masked0 = first_masked / 2;
+            const int steps = w.steps, first_masked = w.first_masked;
             for (int i = first_masked; i < steps; ++i) {
-                if (!(ok = all(wait(&bars.v_full[n & 1][i / 2 - masked0], (n >> 1) & 1)))) break;
-                uint8_t* v = kv_s + (item + i / 2 * 2 + 1) % kStages * kTileBytes + (i & 1) * (kStep * 128);
+                if (!(ok = all(wait(&bars.v_full[n & 1][i - first_masked], (n >> 1) & 1)))) break;
+                uint8_t* v = kv_s + (item + v_item(i, steps)) % kStages * kTileBytes;
                 const int j0 = max(w.pos0 + 1 - i * kStep, 0);       // first such row of the step
                 const int j1 = i + 1 == steps ? w.last : kStep;
                 auto at = [&](int c) {
@@ -743,7 +734,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             if (!ok) break;
             if (lane == 0)
                 for (int i = max(steps - first_masked, 0); i < kMaskedSteps; ++i) mbar_arrive(&bars.clean[n & 1][i]);
-            item += (steps + 1) / 2 * 2;
+            item += 2 * steps;
             __syncwarp();
             if (lane == 0) mbar_arrive(&bars.tile_empty[n & 1]);
         }
@@ -771,13 +762,13 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// bf16 rows [T][cols], `stride` elements apart, boxes of 64 columns x 128 rows.
+// bf16 rows [T][cols], `stride` elements apart, boxes of 64 columns x 64 rows.
 bool encode_rows(CUtensorMap* map, const void* base, int T, int cols, long long stride) {
     auto fn = encode_fn();
     if (!fn) return false;
     cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(T)};
     cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride) * 2};
-    cuuint32_t box[2] = {64, kKeys};
+    cuuint32_t box[2] = {64, kStep};
     cuuint32_t estr[2] = {1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
