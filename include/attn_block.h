@@ -107,10 +107,12 @@ moe_status_t attn_paged_rows(const void* q_bf16, const void* k_cache, const void
  * [T][nq][128] and k, v bf16 rows of nkv heads; consecutive rows lie q_stride,
  * k_stride, v_stride elements apart (multiples of 8, so v may stay inside the
  * qkv projection's rows); 16-byte aligned.  out_bf16 [T][nq][128], out_q and
- * out_s as in attn_decode_paged, out_q 32-byte aligned.  Rows in no sequence are left as they were.
- * From the first bound that is out of order or outside 0..T on, sequences are
- * skipped (*error_word = 5).  A NaN or infinity in k or v reaches the rows that attend
- * it and no others. */
+ * out_s as in attn_decode_paged, out_q 32-byte aligned; no output overlaps an
+ * input.  scale is finite, of any sign.  Rows in no sequence are left as they
+ * were.  From the first bound that is out of order or outside 0..T on, sequences
+ * are skipped (*error_word = 5).  A NaN or infinity in k or v reaches the rows
+ * that attend it and no others.  *error_word = 1: a wait inside the kernel gave
+ * up after two seconds and rows are missing. */
 moe_status_t attn_prompt_packed(const void* q_bf16, long long q_stride, const void* k_bf16, long long k_stride,
                                 const void* v_bf16, long long v_stride, const int32_t* cu_seqlens, int num_seqs, int T,
                                 int nq, int nkv, int head_dim, float scale, void* out_bf16, void* out_q, float* out_s,

@@ -23,7 +23,8 @@
  * which is the order the decode kernel's tensor-core fragments read with
  * 16-byte loads.
  *
- * Error words (device int32, optional, set, never cleared): 4 a position
+ * Error words (device int32, optional, set, never cleared): 1 a wait inside the
+ * decode kernel gave up after two seconds and its rows are wrong, 4 a position
  * outside the page table, 5 a length that was cut, 6 a page id outside the
  * cache, 7 a sequence row outside the table, 8 no free page left.
  */
@@ -77,7 +78,9 @@ size_t attn_kv4_decode_workspace_bytes(int B, int nq, int max_splits);
  * and, when out_q is given, their e4m3 1x128 quantisation) and checks.  Rows
  * with seq_lens[b] <= 0 or row_seq outside [0, num_seqs) get zeros; slots past
  * a sequence's length are not read into the result whatever they hold.  A
- * row's bits depend on split_tokens and on nothing else of the call. */
+ * row's bits depend on split_tokens and on nothing else of the call.  scale is
+ * finite, of any sign.  The workspace is the call's own until it has run: calls
+ * that may run at the same time take one each. */
 moe_status_t attn_kv4_decode_rows(const void* q_bf16, const void* k_cache, const void* v_cache, int num_cache_pages,
                                   const int32_t* page_table, int max_pages, const int32_t* row_seq, int num_seqs,
                                   const int32_t* seq_lens, int B, int nq, int nkv, int head_dim, int page_size,
@@ -91,7 +94,8 @@ moe_status_t attn_kv4_decode_rows(const void* q_bf16, const void* k_cache, const
  * p * page_bytes (bytes, multiples of 16).  A sequence of len tokens owns the
  * first ceil(len / 16) entries of its page-table row; a page that no row owns
  * is free, so nothing is counted between calls and a row is freed by leaving
- * it out.  An owned entry outside [0, num_pages) is carried as -1 (error 6). */
+ * it out.  An owned entry outside [0, num_pages) is carried as -1 (error 6).
+ * The workspace is the call's own until it has run, as for decode. */
 size_t kv_pages_workspace_bytes(int num_pages, int num_rows);
 
 /* New rows from old ones: table_out[i], lens_out[i] = row parents[i] of

@@ -112,6 +112,17 @@ def test_prompt_refusals(k, change, code):
     assert k.attn_prompt_packed(*{**PROMPT, **change}.values()) == code
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3e38])
+def test_scales_that_are_not_finite(k, scale):
+    """3e38 is a float whose product with log2(e) is not."""
+    assert k.attn_prompt_packed(*{**PROMPT, "scale": scale}.values()) == INVALID
+    assert k.attn_kv4_decode_rows(*{**DECODE, "scale": scale}.values()) == INVALID
+
+
+def test_prompt_quantised_rows_32_byte_aligned(k):
+    assert k.attn_prompt_packed(*{**PROMPT, "out_q": 32 * P + 16, "out_s": P}.values()) == INVALID
+
+
 @pytest.mark.parametrize("change,code", [
     (dict(n=-1), INVALID), (dict(pages=0), INVALID), (dict(page=8), INVALID), (dict(max_pages=0), INVALID),
     (dict(seqs=0), INVALID), (dict(rows=-1), INVALID), (dict(caches=None), INVALID), (dict(caches=P + 8), INVALID),

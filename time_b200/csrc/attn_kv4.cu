@@ -824,7 +824,7 @@ moe_status_t attn_kv4_decode_rows(const void* q_bf16, const void* k_cache, const
         page_size != kPage)
         return MOE_ERR_INVALID_ARGUMENT;
     if (split_tokens <= 0 || split_tokens % kPage || split_tokens > kMaxSplitPages * kPage || max_splits <= 0 ||
-        max_pages <= 0 || num_cache_pages <= 0)
+        max_pages <= 0 || num_cache_pages <= 0 || !std::isfinite(scale * kLog2e))
         return MOE_ERR_INVALID_ARGUMENT;
     if (static_cast<long long>(B) * nkv > 65535 || static_cast<long long>(B) * nq > 0x7FFFFFFF) return MOE_ERR_UNSUPPORTED;
     if (B == 0) return MOE_OK;

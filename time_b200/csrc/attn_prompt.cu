@@ -798,6 +798,7 @@ moe_status_t attn_prompt_packed(const void* q_bf16, long long q_stride, const vo
                                 int out_ld, int* error_word, cwStream_t stream) {
     if (T < 0 || num_seqs < 0 || nq <= 0 || nkv <= 0 || nq % nkv || nq / nkv > kMaxGroup || head_dim != kD)
         return MOE_ERR_INVALID_ARGUMENT;
+    if (!std::isfinite(scale * kLog2e)) return MOE_ERR_INVALID_ARGUMENT;
     if (nkv > 65535 || nq > (1 << 20)) return MOE_ERR_UNSUPPORTED;
     if (q_stride < nq * kD || k_stride < nkv * kD || v_stride < nkv * kD || q_stride % 8 || k_stride % 8 || v_stride % 8)
         return MOE_ERR_INVALID_ARGUMENT;
