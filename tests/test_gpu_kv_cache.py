@@ -136,6 +136,31 @@ def test_write_extreme_magnitudes(gpu):
     assert torch.isnan(vr[0, 0, 64:96]).all() and torch.isfinite(vr[0, 0, 32:64]).all()
 
 
+@pytest.mark.parametrize("exp", [-132, -126, -122, -118, -59, -58, -57, -56, 0, 60, 117])
+def test_write_rounds_every_quotient(gpu, exp):
+    """Groups whose largest value is 2^exp times 1 to 2: every scale of four bits there with every bf16 value of both
+    signs down to 2^-7 of the largest, halves between two codes among them.  Codes are exact, so nothing is tolerated."""
+    tops = 2.0 ** exp * (1 + np.arange(128) / 128)
+    tops = torch.from_numpy(tops).to(torch.bfloat16)           # subnormal below 2^-126
+    _, s = R.quantise(tops.double().numpy().repeat(D).reshape(-1, D))
+    groups = []
+    for v in np.unique(s[:, 0]):
+        top = tops[s[:, 0] == v].max()                         # the largest group of that scale
+        x = (top.view(torch.int16).to(torch.int32) - torch.arange(7 * 128)).clamp(min=0).to(torch.int16).view(torch.bfloat16)
+        x = torch.cat([x, -x, torch.zeros(-2 * len(x) % 31, dtype=torch.bfloat16)]).reshape(-1, 31)
+        groups.append(torch.cat([top.repeat(len(x), 1), x], dim=1))
+    x = torch.cat(groups)
+    x = torch.cat([x, x[:-len(x) % 4]]).reshape(-1, D)
+    rows = len(x)
+    qkv = torch.cat([torch.zeros_like(x), x, -x], dim=1).to(gpu)
+    pages = -(-rows // PAGE)
+    kc, vc = KV.kv4_cache(pages, 1, gpu), KV.kv4_cache(pages, 1, gpu)
+    pt, pos, seq = i32([list(range(pages))], gpu), i32(list(range(rows)), gpu), i32([0] * rows, gpu)
+    KV.kv4_rope_write(qkv, pos, seq, pt, kc, vc, 1, 0, None)
+    for got, want in zip(KV.kv4_read_rows(kc, vc, pos, seq, pt), (x, -x)):
+        np.testing.assert_array_equal(f64(got)[:, 0], R.values(*R.quantise(want.double().numpy())))
+
+
 def test_write_and_read_bounds(gpu):
     rng = np.random.default_rng(3)
     nq, nkv = 4, 1

@@ -68,23 +68,45 @@ struct WriteParams {
     int nq, nkv, rot, num_seqs, max_pages, num_cache_pages;
 };
 
+__device__ __forceinline__ float2 bf16_pair(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+
 // Eight dims 8 l .. 8 l + 7 of a head, by lane l of a half-warp, quantised into
 // token t of the (page, head) tile; the whole warp comes here, `store` says
 // which half has a tile.
-__device__ __forceinline__ void quantise_store(const __nv_bfloat16 (&x)[8], uint8_t* page, int t, int l, bool is_k, bool store) {
+//
+// rint(x / s) without a division: q = x * r with r near 1 / s is corrected by its
+// own residual (Newton), q + (x - q s) r, within 2^-45 of x / s before it is
+// rounded.  With x of 8 bits and s of 4, x / s is a half integer or at least 2^-12
+// away from one, so only half integers need care, and those are floats: the
+// corrected q is x / s itself.  Scales below 2^-60 are worked at 2^64 times
+// their size, where the residual is no subnormal.
+__device__ __forceinline__ void quantise_store(const uint4& xv, uint8_t* page, int t, int l, bool is_k, bool store) {
+    const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
     uint32_t amax = 0;                               // as bits: a NaN is above every number
 #pragma unroll
-    for (int e = 0; e < 8; ++e) amax = max(amax, __float_as_uint(__bfloat162float(x[e])) & 0x7FFFFFFFu);
+    for (int i = 0; i < 4; ++i) amax = max(amax, max(xw[i] << 16 & 0x7FFF0000u, xw[i] & 0x7FFF0000u));
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));       // a group of 32 dims is four lanes
     if (!store) return;
     const float s = group_scale(amax);
-    uint32_t codes = 0;
+    const float up = s < 8.67361737988403547e-19f ? 18446744073709551616.0f : 1.0f;
+    const float su = s * up, r = __frcp_rn(su);
+    constexpr float kMagic = 12582912.0f + 8.0f;     // 1.5 * 2^23: the sum's low bits are rint(q) + 8
+    uint32_t codes = 0;                              // the sums' other bits go by their total
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float n = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(__bfloat162float(x[e]), s)), -8.0f), 7.0f) : 0.0f;
-        codes |= static_cast<uint32_t>(static_cast<int>(n) + 8) << (4 * e);
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = bf16_pair(xw[i]);
+        const float xe[2] = {x.x * up, x.y * up};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float q = xe[e] * r;
+            q = fmaf(fmaf(-q, su, xe[e]), r, q);
+            codes += __float_as_uint(fminf(q, 7.0f) + kMagic) << (4 * (2 * i + e));
+        }
     }
+    constexpr uint32_t kOnes = 0x11111111u;
+    codes -= 0x4B400000u * kOnes;
+    if (s == 0.0f) codes = 8u * kOnes;
     if (is_k) {
         *reinterpret_cast<uint32_t*>(page + k_code_byte(t, 8 * l)) = codes;
     } else {
@@ -140,13 +162,14 @@ kv4_rope_write_kernel(const WriteParams p) {
     const int t = pos % kPage;
     // this lane's dims: below half, above it, or not rotated
     const bool rotated = 8 * l < p.rot, lo = 8 * l < half;
-    float cs[8], sn[8];
+    float2 cs[4], sn[4];                             // sn with the sign that it has in this lane's sum
     if constexpr (kLanes) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int i = rotated ? 8 * l + e - (lo ? 0 : half) : 0;
-            cs[e] = rotated ? cs_s[i] : 1.0f;
-            sn[e] = rotated ? sn_s[i] : 0.0f;
+        for (int i = 0; i < 4; ++i) {
+            const int d = rotated ? 8 * l + 2 * i - (lo ? 0 : half) : 0;
+            cs[i] = rotated ? make_float2(cs_s[d], cs_s[d + 1]) : make_float2(1.0f, 1.0f);
+            sn[i] = rotated ? make_float2(sn_s[d], sn_s[d + 1]) : make_float2(0.0f, 0.0f);
+            if (lo) sn[i] = make_float2(-sn[i].x, -sn[i].y);
         }
     }
     const int partner = lo ? lane + half / 8 : lane - half / 8;
@@ -156,26 +179,25 @@ kv4_rope_write_kernel(const WriteParams p) {
             const int h = h0 + u * stride;
             if (h - (lane >> 4) >= heads) break;     // for the whole warp: what follows shuffles
             const bool some = h < heads;
-            const __nv_bfloat16* ib = reinterpret_cast<const __nv_bfloat16*>(&in[u]);
-            __nv_bfloat16 x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = ib[e];
+            uint4 xv = in[u];
             if constexpr (kLanes) {
                 uint4 other;
                 other.x = __shfl_sync(0xffffffffu, in[u].x, partner & 31);
                 other.y = __shfl_sync(0xffffffffu, in[u].y, partner & 31);
                 other.z = __shfl_sync(0xffffffffu, in[u].z, partner & 31);
                 other.w = __shfl_sync(0xffffffffu, in[u].w, partner & 31);
-                const __nv_bfloat16* ob = reinterpret_cast<const __nv_bfloat16*>(&other);
                 if (rotated && h < p.nq + p.nkv) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float mine = __bfloat162float(ib[e]), theirs = __bfloat162float(ob[e]);
-                        x[e] = __float2bfloat16_rn(lo ? rotate_lo(mine, theirs, cs[e], sn[e]) : rotate_hi(theirs, mine, cs[e], sn[e]));
-                    }
+                    auto rotate = [&](uint32_t mine, uint32_t theirs, int i) {
+                        const float2 x = fadd2(fmul2(bf16_pair(mine), cs[i]), fmul2(bf16_pair(theirs), sn[i]));
+                        return pack_bf16(x.x, x.y);
+                    };
+                    xv = make_uint4(rotate(xv.x, other.x, 0), rotate(xv.y, other.y, 1), rotate(xv.z, other.z, 2),
+                                    rotate(xv.w, other.w, 3));
                 }
             } else if (some && h < p.nq + p.nkv) {
                 const __nv_bfloat16* src = row + static_cast<size_t>(h) * kD;
+                const __nv_bfloat16* ib = reinterpret_cast<const __nv_bfloat16*>(&in[u]);
+                __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(&xv);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int d = 8 * l + e;
@@ -183,7 +205,6 @@ kv4_rope_write_kernel(const WriteParams p) {
                     else if (d < p.rot) x[e] = __float2bfloat16_rn(rotate_hi(__bfloat162float(src[d - half]), __bfloat162float(ib[e]), cs_s[d - half], sn_s[d - half]));
                 }
             }
-            const uint4 xv = *reinterpret_cast<const uint4*>(x);
             if (some && h < p.nq) *reinterpret_cast<uint4*>(p.q_out + (static_cast<size_t>(b) * p.nq + h) * kD + 8 * l) = xv;
             if (h - (lane >> 4) + 1 < p.nq) continue;        // both heads of the warp are queries
             const bool is_k = h < p.nq + p.nkv;
@@ -191,7 +212,7 @@ kv4_rope_write_kernel(const WriteParams p) {
             const bool kv = some && h >= p.nq;
             if (kv && is_k && p.k_out) *reinterpret_cast<uint4*>(p.k_out + (static_cast<size_t>(b) * p.nkv + kvh) * kD + 8 * l) = xv;
             uint8_t* page = (is_k ? p.k_cache : p.v_cache) + (static_cast<size_t>(phys) * p.nkv + (kv ? kvh : 0)) * kPage4;
-            quantise_store(x, page, t, l, is_k, kv);
+            quantise_store(xv, page, t, l, is_k, kv);
         }
         h0 += stride * kWriteUnroll;
         load();
