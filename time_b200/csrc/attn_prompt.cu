@@ -167,7 +167,7 @@ constexpr uint32_t kQHalf = kRows * 128;                // 64 dims of the querie
 constexpr uint32_t kQBytes = 2 * kQHalf;
 constexpr size_t kSmem = 2 * kQBytes + kStages * kTileBytes + 1024;
 constexpr uint64_t kWaitNs = 2000000000ull;
-constexpr int kTileReaders = 8 + 4 + 2 + 1;             // softmax, epilogue, MMA warps and the cleaner
+constexpr int kTileReaders = 8 + 1 + 2 + 1;             // softmax warps, the epilogue, MMA warps and the cleaner
 
 // A tile is at most 256 positions (one head a group): steps with masked ones.
 constexpr int kMaskedSteps = 5;
@@ -194,7 +194,7 @@ __device__ __forceinline__ int group_div(int x, uint32_t g_inv) { return static_
 struct Bars {
     uint64_t full[kStages], empty[kStages];             // ring of K and V
     uint64_t s_full[2][2], p_full[2][2];                // [M tile][score buffer]
-    uint64_t pv_done[2], o_full[2], o_free[2];
+    uint64_t pv_done[2], o_full[2], o_free[2], staged;
     uint64_t tile_full[2], tile_empty[2], q_full[2], drain[2];      // by the tile's slot; an empty slot's Q is empty
     // V with masked positions, by the tile's slot; every one of them completes once a tile, so its phase is the slot's
     uint64_t v_full[2][kMaskedSteps], clean[2][kMaskedSteps];
@@ -291,7 +291,7 @@ __device__ __noinline__ void epilogue_dirty(const PromptParams& p, uint32_t to, 
 
 __global__ void __launch_bounds__(kThreads, 1)
 prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-              const __grid_constant__ CUtensorMap vmap) {
+              const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap omap) {
     extern __shared__ uint8_t sm_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* q_s = sm;                                  // [2 slots][2 halves][256 rows][128 B]
@@ -327,11 +327,13 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 mbar_init(&bars.clean[t][i], 1);
             }
         }
+        mbar_init(&bars.staged, 4);
         abort_s = 0;
         fence_mbar_init();
         prefetch_tmap(&qmap);
         prefetch_tmap(&kmap);
         prefetch_tmap(&vmap);
+        prefetch_tmap(&omap);
     } else if (warp == 12) {
         tmem_alloc(&tmem_s, 512);
         tc_fence_before();
@@ -445,20 +447,27 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         }
     } else if (warp < 12) {
         // ---- epilogue
-        int tiles[2] = {0, 0};
+        uint32_t o_phase = 0;                           // of o_full[t], bit t
         bool ok = true;
         for (int n = 0; ok; ++n) {
             if (!(ok = all(wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
             const TileWork& w = tile_s[n & 1];
             if (!w.some) break;
-            const int rows = w.rows, pos0 = w.pos0, kvh = w.kvh;
+            const int rows = w.rows, pos0 = w.pos0, kvh = w.kvh, mt = w.mt;
             const long long first = w.first;
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                if (t >= w.mt || !ok) break;
+            // Rows go through shared memory in place of the queries, in their layout: a full tile leaves as one box, and of
+            // one in part filled a store instruction covers two rows and not a sector of each of 32.
+            uint8_t* rows_sm = q_s + (n & 1) * kQBytes;             // 16-byte chunk c of row i
+            auto chunk = [&](int i, int c) {
+                return reinterpret_cast<uint4*>(rows_sm + (c >> 3) * kQHalf + i * 128 + (((c ^ i) & 7) << 4));
+            };
+            bool box = rows == tile_pos * p.G;
+#pragma unroll 1
+            for (int t = 0; t < mt; ++t) {
                 const int i_row = t * 128 + (threadIdx.x & 127);
                 const uint32_t to = tmem + (static_cast<uint32_t>(warp & 3) << 21) + 256 + t * 128;
-                if (!(ok = all(wait(&bars.o_full[t], tiles[t]++ & 1)))) break;
+                if (!(ok = all(wait(&bars.o_full[t], (o_phase >> t) & 1)))) break;
+                o_phase ^= 1u << t;
                 tc_fence_after();
                 const float inv = 1.0f / l_s[i_row];
                 const bool dirty = *static_cast<volatile const int*>(&w.dirty) != 0;
@@ -468,6 +477,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 const bool store = i_row < rows;
                 const long long out_row = (first + pos) * p.nq + head;
                 if (dirty) {
+                    box = false;
                     epilogue_dirty(p, to, inv, first, pos0, pos, kvh, head, store);
                     tc_fence_before();
                     mbar_arrive(&bars.o_free[t]);
@@ -504,13 +514,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     }
                     if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
                 }
-                // Rows go through shared memory, in place of the warp's own 32 queries, so that a store instruction covers
-                // two whole rows and not a sector of each of 32.
-                uint8_t* rows_sm = q_s + (n & 1) * kQBytes;         // 16-byte chunk c of row i
-                auto chunk = [&](int i, int c) {
-                    return reinterpret_cast<uint4*>(rows_sm + (c >> 3) * kQHalf + i * 128 + (((c ^ i) & 7) << 4));
-                };
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     float x[32];
                     columns(c, x);
@@ -522,6 +526,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 }
                 tc_fence_before();
                 mbar_arrive(&bars.o_free[t]);           // the next tile may write its output
+                if (box) continue;
                 __syncwarp();
                 const int row0 = t * 128 + (warp & 3) * 32;
 #pragma unroll 4
@@ -531,9 +536,22 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                                               (lane & 15) * 8) = *chunk(i, lane & 15);
                 }
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // before the slot's next queries
+            if (!ok) break;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // before the box, and the slot's next queries
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.tile_empty[n & 1]);
+            if (lane == 0) mbar_arrive(&bars.staged);
+            if (warp == 8) {
+                if (!(ok = all(wait(&bars.staged, n & 1)))) break;
+                if (lane == 0) {
+                    if (box) {
+                        tma_store_3d(&omap, rows_sm, 0, kvh * p.G, static_cast<int>(first) + pos0);
+                        tma_store_3d(&omap, rows_sm + kQHalf, 64, kvh * p.G, static_cast<int>(first) + pos0);
+                        bulk_store_wait_read();
+                    }
+                    mbar_arrive(&bars.tile_empty[n & 1]);
+                }
+                __syncwarp();
+            }
         }
     } else if (warp < 14) {
         // ---- MMA issue, by a whole warp for M tile t
@@ -547,16 +565,22 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         const uint32_t k_lo = desc_lo_k(smem_u32(kv_s)), v_lo = desc_lo_mn(smem_u32(kv_s), kHalf);
         auto wait_item = [&](int x) { return all(wait(&bars.full[x % kStages], (x / kStages) & 1)); };
         int n = 0, base = 0, tiles = 0, g = 0;          // tile, its first ring item; tiles and products of this M tile so far
-        // scores, up to two steps before the products and at most one tile
+        bool ok = true;
+        // Scores, up to two steps before the products and at most one tile: as far as tile `next` they are issued where
+        // their operands are there, and waited for with `block`.
         int sn = -1, sj = 0, s_steps = 0, s_last = 0, s_base = 0, sg = 0;
-        auto scores = [&](int next, int next_base) {    // `next`: the tile that comes after this run of scores
+        auto scores = [&](int next, int next_base, bool block) {
+            auto got = [&](uint64_t* bar, uint32_t phase) {
+                if (!block) return all(mbar_test(bar, phase)) != 0;
+                return ok = all(wait(bar, phase));
+            };
             while (sg - g < 2) {
                 if (sj == s_steps) {
-                    if (sn >= next) return true;
-                    if (!all(wait(&bars.tile_full[next & 1], (next >> 1) & 1))) return false;
+                    if (sn >= next) return;
+                    if (!got(&bars.tile_full[next & 1], (next >> 1) & 1)) return;
                     const TileWork& w = tile_s[next & 1];
-                    if (!uni(w.some) || t >= uni(w.mt)) return true;
-                    if (!all(wait(&bars.q_full[next & 1], (next >> 1) & 1))) return false;
+                    if (!uni(w.some) || t >= uni(w.mt)) return;
+                    if (!got(&bars.q_full[next & 1], (next >> 1) & 1)) return;
                     sn = next;
                     sj = 0;
                     s_steps = uni(w.steps);
@@ -564,7 +588,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     s_base = next_base;
                 }
                 const int x = s_base + k_item(sj), st = x % kStages;
-                if (!wait_item(x)) return false;
+                if (!got(&bars.full[st], (x / kStages) & 1)) return;
                 tc_fence_after();
                 const uint32_t id_s = idesc_bf16_f32(128, sj + 1 == s_steps ? s_last : kStep, false) | negate;
                 const uint32_t q = q_lo + (sn & 1) * (kQBytes >> 4), k = k_lo + st * (kTileBytes >> 4);
@@ -578,9 +602,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 ++sj;
                 ++sg;
             }
-            return true;
         };
-        bool ok = true;
         for (; ok; ++n) {
             if (!(ok = all(wait(&bars.tile_full[n & 1], (n >> 1) & 1)))) break;
             const TileWork& slot = tile_s[n & 1];
@@ -593,14 +615,21 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 if (!ok) break;
             } else {
                 const uint32_t slot_phase = (n >> 1) & 1;
-                if (!(ok = scores(n, base) && all(wait(&bars.o_free[t], (tiles++ & 1) ^ 1)))) break;
-                bool ready = false;                     // what a test for the next weights gave, under the MMAs before
                 for (int j = 0; j < steps; ++j) {
-                    const int x = base + v_item(j, steps), st = x % kStages;
+                    // scores and these weights, whichever comes first; the next tile may be handed out only once these are used
+                    bool ready = false;
+                    for (int i = 0; i < 512 && !ready && sg - g < 2; ++i) {
+                        const bool own = sg == g;       // those that the weights are made of
+                        scores(own ? n : n + 1, own ? base : base + 2 * steps, own);
+                        if (!ok) break;
+                        ready = all(mbar_test(&bars.p_full[t][g & 1], (g >> 1) & 1));
+                    }
+                    if (!ok || !(ready || (ok = all(wait(&bars.p_full[t][g & 1], (g >> 1) & 1))))) break;
+                    if (j == 0 && !(ok = all(wait(&bars.o_free[t], (tiles++ & 1) ^ 1)))) break;
                     // V, cleaned where it has to be
+                    const int x = base + v_item(j, steps), st = x % kStages;
                     ok = j < first_masked ? wait_item(x) : all(wait(&bars.clean[n & 1][j - first_masked], slot_phase));
                     if (!ok) break;
-                    if (!all(ready) && !(ok = all(wait(&bars.p_full[t][g & 1], (g >> 1) & 1)))) break;
                     tc_fence_after();
                     const uint32_t v = v_lo + st * (kTileBytes >> 4);
                     const uint32_t pa = tm + (g & 1) * kStep;
@@ -615,8 +644,6 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     }
                     umma_commit_warp(&bars.empty[st]);
                     ++g;
-                    ready = j + 1 < steps && mbar_test(&bars.p_full[t][g & 1], (g >> 1) & 1);
-                    if (!(ok = scores(n + 1, base + 2 * steps))) break;
                 }
             }
             base += 2 * steps;
@@ -628,62 +655,79 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         }
     } else if (warp == 14) {
         // ---- tiles; Q, and K and V of keys 0.., 128.. of every tile
+        // A tile is handed out, and its Q on the way, as soon as its slot is free, between the loads of the tile before; it
+        // is found under those of that tile's first steps.
         TileOrder order(p, tile_pos, blockIdx.x == 0);
-        int item = 0;
-        int armed[2] = {0, 0}, q_tiles = 0;             // V barriers with a copy, by slot; tiles whose Q is loaded
+        int item = 0, q_tiles = 0;                      // ring items so far, tiles whose Q is loaded
+        int armed[2] = {0, 0};                          // V barriers with a copy, by slot
         bool ok = true;
-        for (int n = 0; ok; ++n) {
+        auto find = [&](int n) {
             // every other round backwards: a CTA's tiles even out
             const unsigned int c = n * gridDim.x + ((n & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
             const Tile tl = order.find(c / p.nkv);
-            const int kvh = static_cast<int>(c % p.nkv);
+            TileWork w;
+            w.some = tl.some;
+            w.kvh = static_cast<int>(c % p.nkv);
+            w.first = tl.first;
+            w.pos0 = tl.index * tile_pos;
+            w.rows = min(tile_pos, tl.len - w.pos0) * p.G;
+            w.mt = w.rows > 128 ? 2 : 1;
+            const int pos1 = min(w.pos0 + tile_pos, tl.len) - 1;
+            w.steps = tl.some ? pos1 / kStep + 1 : 0;
+            w.last = (pos1 % kStep + 16) / 16 * 16;
+            w.first_masked = (w.pos0 + 1) / kStep;
+            w.dirty = 0;
+            return w;
+        };
+        auto hand_out = [&](int n, const TileWork& w) {         // into a free slot
+            tile_s[n & 1] = w;
+            mbar_arrive(&bars.tile_full[n & 1]);
+            armed[n & 1] = 0;
+            if (!w.some) return;
+            uint8_t* q = q_s + (n & 1) * kQBytes;
+            mbar_arrive_expect_tx(&bars.q_full[n & 1], tile_pos * p.G * 256);
+            tma_load_3d(&qmap, &bars.q_full[n & 1], q, 0, w.kvh * p.G, w.first + w.pos0);
+            tma_load_3d(&qmap, &bars.q_full[n & 1], q + kQHalf, 64, w.kvh * p.G, w.first + w.pos0);
+            q_tiles = n + 1;
+        };
+        // own_bar: V that has to be cleaned lands at a barrier of its own; the ring's only keeps its phase
+        auto load = [&](const CUtensorMap* map, int x, int y, int n, uint64_t* own_bar) {
+            const int st = item % kStages;
+            if (!(ok = wait(&bars.empty[st], ((item / kStages) & 1) ^ 1))) return;
+            uint64_t* bar = own_bar ? own_bar : &bars.full[st];
+            if (own_bar) mbar_arrive(&bars.full[st]);
+            mbar_arrive_expect_tx(bar, kTileBytes);
+            uint8_t* dst = kv_s + st * kTileBytes;
+            tma_load_2d(map, bar, dst, x, y);
+            tma_load_2d(map, bar, dst + kHalf, x + 64, y);
+            ++item;
+            if (own_bar) ++armed[n & 1];
+        };
+        auto load_step = [&](int n, const TileWork& w, int j) { // K of the step behind, V of this one; the first K with it
+            const int x = w.kvh * kD, y = w.first + j * kStep;
+            if (j == 0) load(&kmap, x, y, n, nullptr);
+            if (ok && j + 1 < w.steps) load(&kmap, x, y + kStep, n, nullptr);
+            if (ok) load(&vmap, x, y, n, j < w.first_masked ? nullptr : &bars.v_full[n & 1][j - w.first_masked]);
+        };
+        TileWork w = find(0);
+        if (lane == 0) hand_out(0, w);
+        for (int n = 0; w.some; ++n) {
+            const int early = min(w.steps, 2);
+            if (lane == 0)
+                for (int j = 0; j < early && ok; ++j) load_step(n, w, j);
+            __syncwarp();
+            const TileWork next = find(n + 1);
             if (lane == 0) {
-                ok = wait(&bars.tile_empty[n & 1], ((n >> 1) & 1) ^ 1);
-                if (ok) {
-                    TileWork w;
-                    w.some = tl.some;
-                    w.kvh = kvh;
-                    w.first = tl.first;
-                    w.pos0 = tl.index * tile_pos;
-                    w.rows = min(tile_pos, tl.len - w.pos0) * p.G;
-                    w.mt = w.rows > 128 ? 2 : 1;
-                    const int pos1 = min(w.pos0 + tile_pos, tl.len) - 1;
-                    w.steps = tl.some ? pos1 / kStep + 1 : 0;
-                    w.last = (pos1 % kStep + 16) / 16 * 16;
-                    w.first_masked = (w.pos0 + 1) / kStep;
-                    w.dirty = 0;
-                    tile_s[n & 1] = w;
-                    mbar_arrive(&bars.tile_full[n & 1]);
-                    armed[n & 1] = 0;
-                    if (w.some) {
-                        const int x = kvh * kD;
-                        auto load = [&](const CUtensorMap* map, int j, uint64_t* own_bar) {
-                            const int st = item % kStages;
-                            if (!(ok = wait(&bars.empty[st], ((item / kStages) & 1) ^ 1))) return;
-                            // V that has to be cleaned lands at a barrier of its own; the ring's only keeps its phase
-                            uint64_t* bar = own_bar ? own_bar : &bars.full[st];
-                            if (own_bar) mbar_arrive(&bars.full[st]);
-                            mbar_arrive_expect_tx(bar, kTileBytes);
-                            uint8_t* dst = kv_s + st * kTileBytes;
-                            tma_load_2d(map, bar, dst, x, w.first + j * kStep);
-                            tma_load_2d(map, bar, dst + kHalf, x + 64, w.first + j * kStep);
-                            ++item;
-                            if (own_bar) ++armed[n & 1];
-                        };
-                        uint8_t* q = q_s + (n & 1) * kQBytes;
-                        mbar_arrive_expect_tx(&bars.q_full[n & 1], tile_pos * p.G * 256);
-                        tma_load_3d(&qmap, &bars.q_full[n & 1], q, 0, kvh * p.G, w.first + w.pos0);
-                        tma_load_3d(&qmap, &bars.q_full[n & 1], q + kQHalf, 64, kvh * p.G, w.first + w.pos0);
-                        q_tiles = n + 1;
-                        load(&kmap, 0, nullptr);
-                        for (int j = 0; j < w.steps && ok; ++j) {
-                            if (j + 1 < w.steps) load(&kmap, j + 1, nullptr);
-                            if (ok) load(&vmap, j, j < w.first_masked ? nullptr : &bars.v_full[n & 1][j - w.first_masked]);
-                        }
-                        if (ok)
-                            for (int i = armed[n & 1]; i < kMaskedSteps; ++i) mbar_arrive(&bars.v_full[n & 1][i]);
-                    }
+                uint64_t* slot = &bars.tile_empty[(n + 1) & 1];
+                const uint32_t slot_phase = (((n + 1) >> 1) & 1) ^ 1;
+                bool out = false;
+                for (int j = early; j < w.steps && ok; ++j) {
+                    if (!out && (out = mbar_test(slot, slot_phase))) hand_out(n + 1, next);
+                    load_step(n, w, j);
                 }
+                if (ok)
+                    for (int i = armed[n & 1]; i < kMaskedSteps; ++i) mbar_arrive(&bars.v_full[n & 1][i]);
+                if (ok && !out && (ok = wait(slot, slot_phase))) hand_out(n + 1, next);
                 if (!ok) {   // loads in flight land before the block leaves
                     for (int i = max(item - kStages, 0); i < item; ++i) mbar_drain(&bars.full[i % kStages], (i / kStages) & 1);
                     for (int m = max(q_tiles - 2, 0); m < q_tiles; ++m) {
@@ -692,7 +736,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     }
                 }
             }
-            ok = __shfl_sync(0xffffffffu, ok, 0) && tl.some;
+            if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+            w = next;
         }
     } else {
         // ---- a weight of 0 must meet a finite value: V of positions that not every row attends
@@ -831,14 +876,14 @@ moe_status_t attn_prompt_packed(const void* q_bf16, long long q_stride, const vo
     const int tile_pos = kRows / p.G;
     const long long tiles = ((T + tile_pos - 1ll) / tile_pos + num_seqs) * nkv;
     if (tiles > 0x7FFFFFFF - 1024) return MOE_ERR_UNSUPPORTED;
-    CUtensorMap qmap, kmap, vmap;
+    CUtensorMap qmap, kmap, vmap, omap;
     if (!encode_q(&qmap, q_bf16, T, nq, p.G, q_stride) || !encode_rows(&kmap, k_bf16, T, nkv * kD, k_stride) ||
-        !encode_rows(&vmap, v_bf16, T, nkv * kD, v_stride))
+        !encode_rows(&vmap, v_bf16, T, nkv * kD, v_stride) || !encode_q(&omap, out_bf16, T, nq, p.G, nq * kD))
         return MOE_ERR_CUDA;
     static bool attr[kMaxDevices] = {};
     if (smem_optin_once(prompt_kernel, static_cast<int>(kSmem), attr) != cudaSuccess) return MOE_ERR_CUDA;
     prompt_kernel<<<static_cast<int>(tiles < kSms ? tiles : kSms), kThreads, kSmem, static_cast<cudaStream_t>(stream)>>>(
-        p, qmap, kmap, vmap);
+        p, qmap, kmap, vmap, omap);
     return launch_status();
 }
 
