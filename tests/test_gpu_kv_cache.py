@@ -136,6 +136,28 @@ def test_write_extreme_magnitudes(gpu):
     assert torch.isnan(vr[0, 0, 64:96]).all() and torch.isfinite(vr[0, 0, 32:64]).all()
 
 
+@pytest.mark.parametrize("rot", [64, 36])
+def test_write_rounds_each_product(gpu, rot):
+    """Both products and their sum are rounded to fp32, whatever a compiler would contract: the bits of the same steps in
+    torch, one operation at a time.  (The same cosf and sinf give the angles there.)"""
+    rng = np.random.default_rng(rot)
+    rows, nq, nkv = 300, 12, 1
+    qkv = normal_bf16(rng, rows, nq + 2 * nkv, D).to(gpu)
+    pos = i32(rng.permutation(rows), gpu)
+    f = torch.from_numpy(A.rope_inv_freq(rot, 1e6)).to(gpu)
+    pages = -(-rows // PAGE)
+    kc, vc = KV.kv4_cache(pages, nkv, gpu), KV.kv4_cache(pages, nkv, gpu)
+    q, k = KV.kv4_rope_write(qkv.flatten(1), pos, i32([0] * rows, gpu), i32([list(range(pages))], gpu), kc, vc, nq, rot, f,
+                             keys=True)
+    ang = (pos.float()[:, None] * f)[:, None]
+    c, s = ang.cos(), ang.sin()
+    x = qkv[:, :nq + nkv].float()
+    a, b = x[..., :rot // 2], x[..., rot // 2:rot]
+    ac, bs, as_, bc = a * c, b * s, a * s, b * c
+    want = torch.cat([ac - bs, as_ + bc, x[..., rot:]], dim=-1).bfloat16()
+    assert torch.equal(torch.cat([q, k], dim=1), want)
+
+
 @pytest.mark.parametrize("exp", [-132, -126, -122, -118, -59, -58, -57, -56, 0, 60, 117])
 def test_write_rounds_every_quotient(gpu, exp):
     """Groups whose largest value is 2^exp times 1 to 2: every scale of four bits there with every bf16 value of both

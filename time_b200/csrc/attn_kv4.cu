@@ -188,8 +188,9 @@ kv4_rope_write_kernel(const WriteParams p) {
                 other.w = __shfl_sync(0xffffffffu, in[u].w, partner & 31);
                 if (rotated && h < p.nq + p.nkv) {
                     auto rotate = [&](uint32_t mine, uint32_t theirs, int i) {
-                        const float2 x = fadd2(fmul2(bf16_pair(mine), cs[i]), fmul2(bf16_pair(theirs), sn[i]));
-                        return pack_bf16(x.x, x.y);
+                        const float2 a = bf16_pair(mine), b = bf16_pair(theirs);
+                        return pack_bf16(__fadd_rn(__fmul_rn(a.x, cs[i].x), __fmul_rn(b.x, sn[i].x)),
+                                         __fadd_rn(__fmul_rn(a.y, cs[i].y), __fmul_rn(b.y, sn[i].y)));
                     };
                     xv = make_uint4(rotate(xv.x, other.x, 0), rotate(xv.y, other.y, 1), rotate(xv.z, other.z, 2),
                                     rotate(xv.w, other.w, 3));

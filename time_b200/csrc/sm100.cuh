@@ -425,11 +425,6 @@ __device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(ar), "l"(br));
     return *reinterpret_cast<float2*>(&d);
 }
-__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
-    uint64_t ar = *reinterpret_cast<uint64_t*>(&a), br = *reinterpret_cast<uint64_t*>(&b), d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(ar), "l"(br));
-    return *reinterpret_cast<float2*>(&d);
-}
 
 // 2^x, one MUFU operation (results below 2^-126 are 0).
 __device__ __forceinline__ float ex2(float x) {
