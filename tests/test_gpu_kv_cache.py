@@ -595,3 +595,27 @@ def test_prompt_fork_decode_compact(gpu):
     for b in range(3):
         np.testing.assert_array_equal(f64(kr[b]), held[b][0][-1])
         np.testing.assert_array_equal(f64(vr[b]), held[b][1][-1])
+
+
+def test_tensors_on_the_host_are_refused(gpu):
+    """One tensor that is not on the device, in every place, is refused before anything is launched."""
+    cpu = torch.device("cpu")
+    c = KV.kv4_cache(4, 1, gpu)
+    z = lambda *n: torch.zeros(*n, dtype=torch.int32, device=gpu)
+    q = torch.zeros(2, 4, D, dtype=torch.bfloat16, device=gpu)
+    calls = [
+        (KV.kv4_rope_write, [torch.zeros(2, 6 * D, dtype=torch.bfloat16, device=gpu), z(2), z(2), z(2, 4), c, c, 4, 64,
+                             torch.zeros(32, device=gpu)]),
+        (KV.kv4_read_rows, [c, c, z(2), z(2), z(2, 4)]),
+        (KV.kv4_decode, [q, c, c, z(2, 4), z(2), 0.1, z(2)]),
+        (A.prompt_packed, [q, q, q, z(2), 0.1]),
+        (KV.fork_pages, [c[None], z(2, 4), z(2), z(2), z(2)]),
+        (KV.compact_pages, [c[None], z(2, 4), z(2), z(2, 4)]),
+    ]
+    for call, args in calls:
+        for i, a in enumerate(args):
+            if isinstance(a, torch.Tensor):
+                with pytest.raises(ValueError, match="device|beside"):
+                    call(*args[:i], a.to(cpu), *args[i + 1:])
+        call(*args)
+    torch.cuda.synchronize()

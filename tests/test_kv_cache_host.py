@@ -164,6 +164,20 @@ def test_python_checks_refuse_before_the_call():
         A.prompt_packed(x, x.transpose(1, 2), x, torch.tensor([0, 4], dtype=torch.int32), 0.1)
 
 
+@pytest.mark.parametrize("change", [
+    dict(inv_freq="float64"), dict(inv_freq=31), dict(seq_lens_out=3), dict(positions="int64"), dict(error_word="int64")])
+def test_python_write_checks(change):
+    import torch
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32)
+    c = torch.zeros(4, 1, 1152, dtype=torch.uint8)
+    args = dict(inv_freq=torch.zeros(32), seq_lens_out=i32(2), positions=i32(2), error_word=i32(1))
+    for name, to in change.items():
+        args[name] = args[name].to(getattr(torch, to)) if isinstance(to, str) else torch.zeros(to, dtype=args[name].dtype)
+    with pytest.raises(ValueError, match="inv_freq|one entry per row|int32"):
+        KV.kv4_rope_write(torch.zeros(2, 6 * 128, dtype=torch.bfloat16), args["positions"], None, torch.zeros(2, 4, dtype=torch.int32),
+                          c, c, 4, 64, args["inv_freq"], seq_lens_out=args["seq_lens_out"], error_word=args["error_word"])
+
+
 # ---------------------------------------------------------------- the plain statements themselves
 
 def test_quantiser_by_hand():

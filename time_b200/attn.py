@@ -159,12 +159,15 @@ def paged_rows(q, k_cache, v_cache, page_table, row_seq, seq_lens, nq: int, nkv:
 
 
 def on_stream(t, stream, call, *args):
-    """call(handle of `stream`, *args) with torch's allocations on that stream (None: the current one).  The tensor `t`
-    must lie on the current device: a launch goes to that one."""
+    """call(handle of `stream`, *args) with torch's allocations on that stream (None: the current one).  Every tensor
+    among `args`, `t` one of them, must lie on the current device: a launch goes to that one."""
     import torch
-    device = t.device.index
-    if device != torch.cuda.current_device():
-        raise ValueError(f"tensors on {t.device}, current device {torch.cuda.current_device()}")
+    device = t.get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        raise ValueError(f"tensors on {t.device}, not on the current CUDA device")
+    for a in args:
+        if isinstance(a, torch.Tensor) and a.get_device() != device:
+            raise ValueError(f"a tensor on {a.device} beside others on {t.device}")
     if stream is None:
         # the handle of torch.cuda.current_stream() without the object, which takes longer than the launch's arguments
         return call(torch._C._cuda_getCurrentRawStream(device), *args)
@@ -177,7 +180,7 @@ def check_i32(*tensors):
     import torch
     for t in tensors:
         if t is not None and (t.dtype is not torch.int32 or not t.is_contiguous()):
-            raise ValueError("positions, lengths, sequence rows, page tables and bounds are contiguous int32 tensors")
+            raise ValueError("positions, lengths, sequence rows, page tables, bounds and error words are contiguous int32 tensors")
 
 
 def check_rows(name, t, dtype, width):
@@ -200,7 +203,7 @@ def prompt_packed(q, k, v, cu_seqlens, scale: float, quant: bool = False, out=No
     import torch
     for name, t in (("q", q), ("k", k), ("v", v)):
         check_heads(name, t, torch.bfloat16)
-    check_i32(cu_seqlens)
+    check_i32(cu_seqlens, error_word)
     T, nq = q.shape[:2]
     nkv = k.shape[1]
     if k.shape[0] != T or v.shape != k.shape:

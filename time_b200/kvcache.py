@@ -66,9 +66,18 @@ def _check_kv4(k_cache, v_cache):
 
 
 @functools.lru_cache(maxsize=1024)
-def _splits(B: int, nkv: int, max_context: int, split_tokens: int | None, max_splits: int | None):
+def _splits(B: int, nq: int, nkv: int, max_context: int, split_tokens: int | None, max_splits: int | None):
+    """(tokens of a split, splits, workspace bytes)."""
     split = lib().attn_kv4_split_tokens(B, nkv, max_context) if split_tokens is None else split_tokens
-    return split, -(-max_context // split) if max_splits is None else max_splits
+    if split <= 0:
+        raise ValueError("split_tokens is positive")
+    n = -(-max_context // split) if max_splits is None else max_splits
+    return split, n, max(lib().attn_kv4_decode_workspace_bytes(B, nq, n), 16)
+
+
+@functools.lru_cache(maxsize=1024)
+def _pages_workspace(pages: int, rows: int) -> int:
+    return lib().kv_pages_workspace_bytes(pages, rows)
 
 
 def kv4_rope_write(qkv, positions, row_seq, page_table, k_cache, v_cache, nq: int, rot: int, inv_freq,
@@ -79,12 +88,14 @@ def kv4_rope_write(qkv, positions, row_seq, page_table, k_cache, v_cache, nq: in
     import torch
     _check_kv4(k_cache, v_cache)
     A.check_rows("qkv", qkv, torch.bfloat16, (nq + 2 * k_cache.shape[1]) * HEAD_DIM)
-    A.check_i32(positions, row_seq, page_table, seq_lens_out)
+    A.check_i32(positions, row_seq, page_table, seq_lens_out, error_word)
     B = qkv.shape[0]
-    if positions.numel() != B or (B if row_seq is None else row_seq.numel()) != B:
-        raise ValueError("positions and row_seq have one entry per row")
-    if inv_freq is not None and inv_freq.numel() < rot // 2:
-        raise ValueError("inv_freq has rot / 2 entries")
+    if positions.numel() != B or (B if row_seq is None else row_seq.numel()) != B or \
+            (B if seq_lens_out is None else seq_lens_out.numel()) != B:
+        raise ValueError("positions, row_seq and seq_lens_out have one entry per row")
+    if inv_freq is not None and (inv_freq.numel() < rot // 2 or inv_freq.dtype is not torch.float32 or
+                                 not inv_freq.is_contiguous()):
+        raise ValueError("inv_freq has rot / 2 contiguous float32 entries")
     if row_seq is None and page_table.shape[0] < B:
         raise ValueError("the page table has a row per row of qkv when row_seq is None")
     return A.on_stream(qkv, stream, _rope_write, qkv, positions, row_seq, page_table, k_cache, v_cache, nq, rot, inv_freq,
@@ -108,7 +119,7 @@ def kv4_read_rows(k_cache, v_cache, positions, row_seq, page_table, error_word=N
     """attn_kv4_read_rows: the tokens at `positions` of page-table rows `row_seq` as the bf16 values the cache holds:
     (k, v), each [B][nkv][128]."""
     _check_kv4(k_cache, v_cache)
-    A.check_i32(positions, row_seq, page_table)
+    A.check_i32(positions, row_seq, page_table, error_word)
     B = positions.numel()
     if (B if row_seq is None else row_seq.numel()) != B or (row_seq is None and page_table.shape[0] < B):
         raise ValueError("row_seq has one entry per position")
@@ -135,7 +146,7 @@ def kv4_decode(q, k_cache, v_cache, page_table, seq_lens, scale: float, row_seq=
     import torch
     _check_kv4(k_cache, v_cache)
     A.check_heads("q", q, torch.bfloat16)
-    A.check_i32(page_table, seq_lens, row_seq)
+    A.check_i32(page_table, seq_lens, row_seq, error_word)
     if not q.is_contiguous():
         raise ValueError("q is contiguous")
     B = q.shape[0]
@@ -151,9 +162,8 @@ def _decode(stream, q, k_cache, v_cache, page_table, seq_lens, scale, row_seq, s
             error_word):
     import torch
     (B, nq, _), (pages, nkv, _), (num_seqs, max_pages) = q.shape, k_cache.shape, page_table.shape
-    split_tokens, max_splits = _splits(B, nkv, max_pages * PAGE, split_tokens, max_splits)
+    split_tokens, max_splits, need = _splits(B, nq, nkv, max_pages * PAGE, split_tokens, max_splits)
     if workspace is None:
-        need = max(lib().attn_kv4_decode_workspace_bytes(B, nq, max_splits), 16)
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     out = torch.empty_like(q)
     out_q = out_s = None
@@ -193,7 +203,7 @@ def fork_pages(caches, table, lens, parents, reserve=None, workspace=None, error
     """kv_pages_fork: row i of the result is row parents[i] (-1: empty) with room for reserve[i] more tokens; full
     pages are shared, a page in part filled is copied for all appending rows but one.  Returns (table, lens) int32,
     new tensors."""
-    A.check_i32(table, lens, parents, reserve)
+    A.check_i32(table, lens, parents, reserve, error_word)
     _check_table(table, lens)
     if reserve is not None and reserve.numel() != parents.numel():
         raise ValueError("reserve has one entry per parent")
@@ -205,7 +215,7 @@ def _fork(stream, caches, table, lens, parents, reserve, workspace, error_word):
     ptr, stride, n, pages, page_bytes = _cache_args(caches)
     rows, max_pages = parents.numel(), table.shape[1]
     if workspace is None:
-        workspace = torch.empty(lib().kv_pages_workspace_bytes(pages, rows), dtype=torch.uint8, device=caches.device)
+        workspace = torch.empty(_pages_workspace(pages, rows), dtype=torch.uint8, device=caches.device)
     out = torch.empty(rows, max_pages, dtype=torch.int32, device=caches.device)
     lens_out = torch.empty(rows, dtype=torch.int32, device=caches.device)
     M.check("kv_pages_fork", lib().kv_pages_fork(
@@ -218,7 +228,7 @@ def _fork(stream, caches, table, lens, parents, reserve, workspace, error_word):
 def compact_pages(caches, table, lens, out=None, workspace=None, error_word=None, stream=None):
     """kv_pages_compact: moves the pages in use to the lowest ids.  Returns (table, pages in use int32 [1]); `out` may
     be `table` itself."""
-    A.check_i32(table, lens, out)
+    A.check_i32(table, lens, out, error_word)
     _check_table(table, lens)
     if out is not None and out.shape != table.shape:
         raise ValueError("out has the page table's shape")
@@ -230,7 +240,7 @@ def _compact(stream, caches, table, lens, out, workspace, error_word):
     ptr, stride, n, pages, page_bytes = _cache_args(caches)
     seqs, max_pages = table.shape
     if workspace is None:
-        workspace = torch.empty(lib().kv_pages_workspace_bytes(pages, seqs), dtype=torch.uint8, device=caches.device)
+        workspace = torch.empty(_pages_workspace(pages, seqs), dtype=torch.uint8, device=caches.device)
     out = torch.empty_like(table) if out is None else out
     used = torch.empty(1, dtype=torch.int32, device=caches.device)
     M.check("kv_pages_compact", lib().kv_pages_compact(
