@@ -7,6 +7,10 @@
 // bf16 number 128 + (n + 8), and (136 + n) * s - 136 * s is exact -- 136 * s is
 // 17 * s with at most eight significant bits, n * s has at most eight -- so the
 // tensor cores see exactly the values held and nothing is rounded on the way.
+//
+// Measured (B200, device time).  Write of 4198 rows, 96 query and 8 KV heads:
+// 47 us, 5.1 TB/s of rows in, queries, keys and codes out; 64 rows: 3.2 us.  Rows
+// read back: 8 us for those 4198.  Decode: see there.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -120,7 +124,7 @@ __device__ __forceinline__ void quantise_store(const uint4& xv, uint8_t* page, i
 
 // One block per (row, share of the heads), a half-warp per head with 16 bytes a
 // lane and kWriteUnroll heads in flight; bound by the rows in and the q rows
-// out.  kLanes: the rotated halves are whole lanes, a dim's partner comes from
+// out (0.8 of the copy bandwidth; 2, 3 and 7 heads in flight are within 4 %).  kLanes: the rotated halves are whole lanes, a dim's partner comes from
 // lane l +- half / 8 and a lane's cosines stay in registers; else partners come
 // from memory.
 template <bool kLanes>
@@ -188,6 +192,7 @@ kv4_rope_write_kernel(const WriteParams p) {
                 other.w = __shfl_sync(0xffffffffu, in[u].w, partner & 31);
                 if (rotated && h < p.nq + p.nkv) {
                     auto rotate = [&](uint32_t mine, uint32_t theirs, int i) {
+                        // one by one: packed products and their packed sum come out contracted
                         const float2 a = bf16_pair(mine), b = bf16_pair(theirs);
                         return pack_bf16(__fadd_rn(__fmul_rn(a.x, cs[i].x), __fmul_rn(b.x, sn[i].x)),
                                          __fadd_rn(__fmul_rn(a.y, cs[i].y), __fmul_rn(b.y, sn[i].y)));
@@ -290,6 +295,18 @@ kv4_read_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__
 // a time from bulk-copied rings of their own: codes to fragments with the fma of
 // the file's head, S = Q K^T and O += P V on mma.sync with the group's query
 // heads as M, one online softmax whose maximum is left behind by up to 2^8.
+// mma.sync, because its B fragments are registers: a code goes from the ring to
+// the tensor core without a way back through shared memory, and a group's 16 rows
+// would leave seven eighths of a tcgen05 tile empty.
+//
+// Bound by what a page costs to unpack, not by its bytes: 366 instructions a page
+// and KV head, a third of them shifts and masks; the ALU pipe is 52 % busy, the
+// tensor pipe 38 %, and three CTAs (168 registers) leave a scheduler under three
+// warps.  Measured (B200, device time): 64 contexts of up to 16384, 64 heads on 8
+// KV heads, 189 us or 3.2 TB/s of pages; 64 of up to 32768, 12 heads, 56 us or
+// 2.4 TB/s, the merge and uneven lengths in it; 16 of up to 8191, 96
+// heads, 32 us; one of 32768, 10 us.  Slower: four CTAs of 128 registers, shifts as
+// multiplications, scores of the next pair under this one's softmax.
 
 constexpr int kWarps = 4;
 constexpr int kNst = 3;                                   // page pairs in flight per warp

@@ -7,6 +7,15 @@
 // comes in one TMA box.  Tiles are taken in the order of the keys they attend,
 // most first, by a search over the sequence bounds in each CTA: nothing is
 // planned on the host.
+//
+// Bound: the tensor pipe, 4 * 128 * nq * sum of L (L + 1) / 2 operations over
+// the lengths L.  Measured (B200, device time): one prompt of 16384 tokens, 12 query
+// heads on one KV head, 635-710 us or 1160-1290 TFLOP/s, where the power limit
+// sets the clock; one of 4096 with 96 heads on 8 KV heads, 351 us or 1175; four of
+// 1024, 122 us or 845; seven of up to 1201, 98 us or 770: a CTA has nine tiles
+// there, and first and last steps take longer than those between; 24 of up to 201,
+// 12 heads, 12.7 us: under one wave, launch, first loads, four steps and output in
+// a row.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -147,18 +156,24 @@ __device__ __forceinline__ void zero_nonfinite(uint4& v) {
 // fp32 and written back over itself as the bf16 weights P, which the second MMA
 // takes from TMEM as its A operand with V (MN-major) from shared memory; the
 // scores of the next step are computed meanwhile.  TMEM holds 2 x 2 x 64 columns
-// of scores and 2 x 128 of output.  The running maximum is left behind by up to
+// of scores and 2 x 128 of output.  (128 keys a step with one buffer would read
+// the queries half as often from shared memory, 64 cycles for 64 of products instead
+// of 48 for 32, but leaves the softmax alone with nothing to run under: 141 us
+// instead of 126 for four prompts of 1024 x 96 heads.)  The running maximum is left behind by up to
 // 2^8 before the output is rescaled, so a rescale is rare and the softmax threads
 // do it themselves.  An M tile's MMAs have a warp of their own, so that what one
-// spends between MMAs (barriers, descriptors) is covered by the other's.  Steps
-// run on from tile to tile: with Q in two buffers, the next tile's first scores
-// are issued under the last weights of a tile, and its output rows leave through
-// the buffer of the queries that are done with.
+// spends between MMAs (barriers, descriptors) is covered by the other's; a
+// whole warp issues them, with uniform operands, for a lane of a divergent branch
+// takes longer to issue an MMA than the MMA takes.  Steps run on from tile to
+// tile: with Q in two buffers, the next tile's first scores are issued under the
+// last weights of a tile, and its output rows leave through the buffer of the
+// queries that are done with.  The six ring stages that are left hold three steps
+// of K and V (four stages: 109 us instead of 99 for seven prompts).
 
 constexpr int kSms = 148;
 constexpr int kRows = 256;
 constexpr int kStep = 64;                               // keys of a softmax step and of a ring stage
-constexpr int kFmaPairs = 2;                            // pairs of eight whose exponentials go to the FMA pipe
+constexpr int kFmaPairs = 2;                            // pairs of eight whose exponentials go to the FMA pipe; three or four gain nothing
 constexpr int kStages = 6;                              // K and V tiles in flight, 16 KB each
 constexpr int kThreads = 512;
 constexpr uint32_t kHalf = kStep * 128;                 // 64 dims of a 64-key tile: rows of 128 bytes, swizzled
@@ -654,7 +669,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             mbar_drain(&bars.drain[t], 0);
         }
     } else if (warp == 14) {
-        // ---- tiles; Q, and K and V of keys 0.., 128.. of every tile
+        // ---- tiles, their Q, and K and V of each step
         // A tile is handed out, and its Q on the way, as soon as its slot is free, between the loads of the tile before; it
         // is found under those of that tile's first steps.
         TileOrder order(p, tile_pos, blockIdx.x == 0);
