@@ -530,17 +530,20 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
                 }
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    float x[32];
-                    columns(c, x);
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t o[64];
+                    tmem_ld32(to + 64 * c, *reinterpret_cast<uint32_t(*)[32]>(o));
+                    tmem_ld32(to + 64 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(o + 32));
+                    tmem_wait_ld();
+                    if (c == 1) {
+                        tc_fence_before();
+                        mbar_arrive(&bars.o_free[t]);   // the next tile may write its output
+                    }
+                    auto pack = [&](int e) { return pack_bf16(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv); };
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        *chunk(i_row, 4 * c + e) =
-                            make_uint4(pack_bf16(x[8 * e], x[8 * e + 1]), pack_bf16(x[8 * e + 2], x[8 * e + 3]),
-                                       pack_bf16(x[8 * e + 4], x[8 * e + 5]), pack_bf16(x[8 * e + 6], x[8 * e + 7]));
+                    for (int e = 0; e < 8; ++e)
+                        *chunk(i_row, 8 * c + e) = make_uint4(pack(8 * e), pack(8 * e + 2), pack(8 * e + 4), pack(8 * e + 6));
                 }
-                tc_fence_before();
-                mbar_arrive(&bars.o_free[t]);           // the next tile may write its output
                 if (box) continue;
                 __syncwarp();
                 const int row0 = t * 128 + (warp & 3) * 32;
