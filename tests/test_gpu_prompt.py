@@ -267,3 +267,57 @@ def test_two_calls_at_once(gpu):
     outs = [[A.prompt_packed(q, k, v, cu, 0.1, stream=s)[0] for s in streams] for _ in range(5)]
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for pair in outs for o in pair)
+
+
+@pytest.mark.parametrize("G", range(1, 17))
+def test_every_group_size(gpu, G):
+    """Whole and part-filled tiles of every group size, with rows outside that stay as they were; the same bits with and
+    without the quantised rows."""
+    rng = np.random.default_rng(G)
+    nkv, first, lens = 2, 2, [256 // G * 2 + 3, 1, 70, 256 // G]
+    T = first + sum(lens) + 5
+    q, k, v = rows(rng, T, nkv * G, D).to(gpu), rows(rng, T, nkv, D).to(gpu), rows(rng, T, nkv, D).to(gpu)
+    out = torch.full_like(q, 3.0)
+    A.prompt_packed(q, k, v, cu_of(lens, gpu, first), 0.1, out=out)
+    check(out, q, k, v, lens, 0.1, first)
+    assert (out[:first] == 3).all() and (out[first + sum(lens):] == 3).all()
+    again, _, _ = A.prompt_packed(q, k, v, cu_of(lens, gpu, first), 0.1, quant=True, out=torch.full_like(q, 3.0))
+    assert torch.equal(out, again)
+
+
+def test_element_numbers_past_32_bits(gpu):
+    """q and out of 2.3e9 elements: prompts on both sides of element 2^31 and the last one."""
+    nq, nkv, n = 128, 8, 500
+    seqs = 280
+    T = seqs * n
+    assert T * nq * D > 2 ** 31
+    g = torch.Generator(device=gpu).manual_seed(5)
+    q, k, v = (torch.randn(T, h, D, dtype=torch.bfloat16, device=gpu, generator=g) for h in (nq, nkv, nkv))
+    err = torch.zeros(1, dtype=torch.int32, device=gpu)
+    out, _, _ = A.prompt_packed(q, k, v, cu_of([n] * seqs, gpu), D ** -0.5, error_word=err)
+    assert int(err) == 0
+    for s in (0, 2 ** 31 // (nq * D * n), seqs - 1):
+        r = slice(s * n, (s + 1) * n)
+        for h in (0, nq - 1):
+            kv = h * nkv // nq
+            ref, tol = R.attend(f64(q[r, h:h + 1]), f64(k[r, kv:kv + 1]), f64(v[r, kv:kv + 1]), np.arange(1, n + 1), D ** -0.5)
+            assert (np.abs(f64(out[r, h:h + 1]) - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("G", [1, 12])
+def test_quantised_rows_before_a_nan(gpu, G):
+    """A NaN and an infinity in v, in tiles that are whole and in part filled: the rows before them keep their bits, as bf16
+    and as e4m3 with its scale."""
+    rng = np.random.default_rng(G)
+    n = 300
+    q, k, v = rows(rng, n, G, D).to(gpu), rows(rng, n, 1, D).to(gpu), rows(rng, n, 1, D).to(gpu)
+    clean = A.prompt_packed(q, k, v, cu_of([n], gpu), 0.1, quant=True)
+    for at in (1, 20, 64, 255, 290, 299):
+        bad = v.clone()
+        bad[at, 0, 7], bad[at, 0, 100] = float("nan"), float("-inf")
+        out, oq, os_ = A.prompt_packed(q, k, bad, cu_of([n], gpu), 0.1, quant=True)
+        assert torch.equal(out[:at], clean[0][:at]) and torch.equal(oq[:at], clean[1][:at])
+        assert torch.equal(os_[:, :at], clean[2][:, :at])
+        assert torch.isnan(out[at:, :, 7]).all() and (out[at:, :, 100] == float("-inf")).all()
+        others = [d for d in range(D) if d not in (7, 100)]
+        assert torch.equal(out[at:][..., others], clean[0][at:][..., others])
