@@ -321,3 +321,15 @@ def test_quantised_rows_before_a_nan(gpu, G):
         assert torch.isnan(out[at:, :, 7]).all() and (out[at:, :, 100] == float("-inf")).all()
         others = [d for d in range(D) if d not in (7, 100)]
         assert torch.equal(out[at:][..., others], clean[0][at:][..., others])
+
+
+def test_rows_do_not_depend_on_the_size_of_the_call(gpu):
+    """A prompt alone, which is run in smaller tiles, and among many others."""
+    rng = np.random.default_rng(17)
+    lens, nq = [400] + [300] * 20, 12
+    T = sum(lens)
+    q, k, v = rows(rng, T, nq, D).to(gpu), rows(rng, T, 1, D).to(gpu), rows(rng, T, 1, D).to(gpu)
+    out = A.prompt_packed(q, k, v, cu_of(lens, gpu), 0.1)[0]
+    for first, n in ((0, 400), (400, 300), (T - 300, 300)):
+        s = slice(first, first + n)
+        assert torch.equal(A.prompt_packed(q[s], k[s], v[s], cu_of([n], gpu), 0.1)[0], out[s])

@@ -12,9 +12,9 @@
 // the lengths L.  Measured (B200, device time): one prompt of 16384 tokens, 12 query
 // heads on one KV head, 635-710 us or 1160-1290 TFLOP/s, where the power limit
 // sets the clock; one of 4096 with 96 heads on 8 KV heads, 351 us or 1175; four of
-// 1024, 122 us or 845; seven of up to 1201, 98 us or 770: a CTA has nine tiles
+// 1024, 120 us or 860; seven of up to 1201, 97 us or 780: a CTA has nine tiles
 // there, and first and last steps take longer than those between; 24 of up to 201,
-// 12 heads, 12.7 us: under one wave, launch, first loads, four steps and output in
+// 12 heads, 11.2 us: under one wave, launch, first loads, four steps and output in
 // a row.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -46,6 +46,7 @@ struct PromptParams {
     float* out_s;
     int* error_word;
     int num_seqs, T, nq, nkv, G, out_ld;
+    int tile_pos;                  // positions of a tile
     float scale_log2;
     bool flip_q;                   // a negative scale: its sign is taken by the queries
 };
@@ -354,7 +355,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
         tc_fence_before();
     }
     const uint32_t g_inv = (65536u + p.G - 1) / p.G;
-    const int tile_pos = kRows / p.G;                   // positions of a tile
+    const int tile_pos = p.tile_pos;
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_s;
@@ -839,12 +840,12 @@ bool encode_rows(CUtensorMap* map, const void* base, int T, int cols, long long 
 }
 
 // q rows [T][nq][128], boxes of 64 dims x G heads x the positions of a tile.
-bool encode_q(CUtensorMap* map, const void* base, int T, int nq, int G, long long stride) {
+bool encode_q(CUtensorMap* map, const void* base, int T, int nq, int G, int tile_pos, long long stride) {
     auto fn = encode_fn();
     if (!fn) return false;
     cuuint64_t dims[3] = {kD, static_cast<cuuint64_t>(nq), static_cast<cuuint64_t>(T)};
     cuuint64_t strides[2] = {kD * 2, static_cast<cuuint64_t>(stride) * 2};
-    cuuint32_t box[3] = {64, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(kRows / G)};
+    cuuint32_t box[3] = {64, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(tile_pos)};
     cuuint32_t estr[3] = {1, 1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -891,12 +892,18 @@ moe_status_t attn_prompt_packed(const void* q_bf16, long long q_stride, const vo
     p.flip_q = p.scale_log2 < 0.0f;
     p.scale_log2 = fmaxf(fabsf(p.scale_log2), 1.17549435e-38f);   // 0: every finite score alike, masked ones still -inf
     // every sequence has at most one tile in part filled
-    const int tile_pos = kRows / p.G;
-    const long long tiles = ((T + tile_pos - 1ll) / tile_pos + num_seqs) * nkv;
+    auto tiles_of = [&](int pos) { return ((T + pos - 1ll) / pos + num_seqs) * nkv; };
+    // Where tiles of one M tile find an SM each, twice as many SMs run half as many rows (24 prompts of up to 201 tokens, 12
+    // heads: 11.2 us instead of 12.8; one of 128: 8.8 instead of 10.7).  A step of one M tile takes two thirds of one of
+    // two, so long prompts gain up to two tiles an SM (one of 2000: 31 instead of 35), while for short ones the second
+    // tile costs more (20 of 100: 13.5 instead of 12.0).  A row's bits are the same either way.
+    const long long small = tiles_of(128 / p.G);
+    p.tile_pos = small <= kSms || (small <= 2 * kSms && T >= 500ll * num_seqs) ? 128 / p.G : kRows / p.G;
+    const long long tiles = tiles_of(p.tile_pos);
     if (tiles > 0x7FFFFFFF - 1024) return MOE_ERR_UNSUPPORTED;
     CUtensorMap qmap, kmap, vmap, omap;
-    if (!encode_q(&qmap, q_bf16, T, nq, p.G, q_stride) || !encode_rows(&kmap, k_bf16, T, nkv * kD, k_stride) ||
-        !encode_rows(&vmap, v_bf16, T, nkv * kD, v_stride) || !encode_q(&omap, out_bf16, T, nq, p.G, nq * kD))
+    if (!encode_q(&qmap, q_bf16, T, nq, p.G, p.tile_pos, q_stride) || !encode_rows(&kmap, k_bf16, T, nkv * kD, k_stride) ||
+        !encode_rows(&vmap, v_bf16, T, nkv * kD, v_stride) || !encode_q(&omap, out_bf16, T, nq, p.G, p.tile_pos, nq * kD))
         return MOE_ERR_CUDA;
     static bool attr[kMaxDevices] = {};
     if (smem_optin_once(prompt_kernel, static_cast<int>(kSmem), attr) != cudaSuccess) return MOE_ERR_CUDA;
