@@ -112,8 +112,8 @@ moe_status_t attn_paged_rows(const void* q_bf16, const void* k_cache, const void
  * were.  From the first bound that is out of order or outside 0..T on, sequences
  * are skipped (*error_word = 5).  A NaN or infinity in k or v reaches the rows
  * that attend it and no others; a row's bits depend on its own sequence alone.
- * *error_word = 1: a wait inside the kernel gave
- * up after two seconds and rows are missing. */
+ * *error_word = 1: a wait inside the kernel gave up after two seconds and rows
+ * are missing. */
 moe_status_t attn_prompt_packed(const void* q_bf16, long long q_stride, const void* k_bf16, long long k_stride,
                                 const void* v_bf16, long long v_stride, const int32_t* cu_seqlens, int num_seqs, int T,
                                 int nq, int nkv, int head_dim, float scale, void* out_bf16, void* out_q, float* out_s,
