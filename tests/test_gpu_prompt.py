@@ -333,3 +333,33 @@ def test_rows_do_not_depend_on_the_size_of_the_call(gpu):
     for first, n in ((0, 400), (400, 300), (T - 300, 300)):
         s = slice(first, first + n)
         assert torch.equal(A.prompt_packed(q[s], k[s], v[s], cu_of([n], gpu), 0.1)[0], out[s])
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("long,short", [(13, 4), (16, 1), (21, 5), (19, 10)])
+def test_short_tiles_right_behind_longer_ones(gpu, long, short, quant):
+    """Every CTA's tiles alternate between two M tiles and one, so that a part of the epilogue that is done with the long
+    one can be through the short one before the rest: the bits of each prompt alone, in every one of several runs."""
+    rng = np.random.default_rng(long)
+    nq, sms = 12, torch.cuda.get_device_properties(gpu).multi_processor_count
+    lens = [long if i // sms % 2 == 0 else short for i in range(7 * sms)]
+    T = sum(lens)
+    q, k, v = rows(rng, T, nq, D).to(gpu), rows(rng, T, 1, D).to(gpu), rows(rng, T, 1, D).to(gpu)
+    cu, err = cu_of(lens, gpu), torch.zeros(1, dtype=torch.int32, device=gpu)
+    runs = [A.prompt_packed(q, k, v, cu, 0.1, quant=quant, error_word=err) for _ in range(10)]
+    assert int(err) == 0
+    at = 0
+    want = [torch.empty_like(runs[0][0]), None, None]
+    if quant:
+        want = [want[0], torch.empty_like(runs[0][1]), torch.empty(nq, T, device=gpu)]
+    for n in lens:
+        s = slice(at, at + n)
+        one = A.prompt_packed(q[s], k[s], v[s], cu_of([n], gpu), 0.1, quant=quant)
+        want[0][s] = one[0]
+        if quant:
+            want[1][s], want[2][:, s] = one[1], one[2][:, :n]
+        at += n
+    for out, oq, os_ in runs:
+        assert torch.equal(out, want[0])
+        if quant:
+            assert torch.equal(oq, want[1]) and torch.equal(os_[:, :T], want[2])

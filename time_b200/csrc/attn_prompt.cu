@@ -210,7 +210,10 @@ __device__ __forceinline__ int group_div(int x, uint32_t g_inv) { return static_
 struct Bars {
     uint64_t full[kStages], empty[kStages];             // ring of K and V
     uint64_t s_full[2][2], p_full[2][2];                // [M tile][score buffer]
-    uint64_t pv_done[2], o_full[2], o_free[2], staged;
+    uint64_t pv_done[2], o_full[2], o_free[2];
+    // Output rows in shared memory, by the tile's slot: an epilogue warp may be a tile ahead of the others, and two only
+    // when the slot is free again.
+    uint64_t staged[2];
     uint64_t tile_full[2], tile_empty[2], q_full[2], drain[2];      // by the tile's slot; an empty slot's Q is empty
     // V with masked positions, by the tile's slot; every one of them completes once a tile, so its phase is the slot's
     uint64_t v_full[2][kMaskedSteps], clean[2][kMaskedSteps];
@@ -335,6 +338,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             mbar_init(&bars.tile_full[t], 1);
             mbar_init(&bars.tile_empty[t], kTileReaders);
             mbar_init(&bars.drain[t], 1);
+            mbar_init(&bars.staged[t], 4);
         }
         for (int t = 0; t < 2; ++t) {
             mbar_init(&bars.q_full[t], 1);
@@ -343,7 +347,6 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 mbar_init(&bars.clean[t][i], 1);
             }
         }
-        mbar_init(&bars.staged, 4);
         abort_s = 0;
         fence_mbar_init();
         prefetch_tmap(&qmap);
@@ -558,9 +561,9 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             if (!ok) break;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // before the box, and the slot's next queries
             __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.staged);
+            if (lane == 0) mbar_arrive(&bars.staged[n & 1]);
             if (warp == 8) {
-                if (!(ok = all(wait(&bars.staged, n & 1)))) break;
+                if (!(ok = all(wait(&bars.staged[n & 1], (n >> 1) & 1)))) break;
                 if (lane == 0) {
                     if (box) {
                         tma_store_3d(&omap, rows_sm, 0, kvh * p.G, static_cast<int>(first) + pos0);
