@@ -369,6 +369,29 @@ def test_decode_bounds(gpu):
     assert int(err) == 7 and not out.any()
 
 
+@pytest.mark.parametrize("bad", [[0], [1], [0, 1], [9, 24], [8, 9, 46], list(range(0, 48, 5))])
+def test_decode_bad_ids_among_many_pages(gpu, bad):
+    """One split of 48 pages with ids outside the cache: those pages read as zeros, and the good ones that come into the
+    same places of shared memory after them as themselves."""
+    rng = np.random.default_rng(len(bad))
+    pages = 48
+    kc, vc = random_cache(rng, pages, 1)
+    q = normal_bf16(rng, 1, 12, D).to(gpu)
+    row = rng.permutation(pages)
+    ids = row.copy()
+    ids[bad] = [1000, -1, pages][len(bad) % 3]
+    k, v = seq_values(kc, "k", row, pages * PAGE), seq_values(vc, "v", row, pages * PAGE)
+    for x in (k, v):
+        x.reshape(pages, -1)[bad] = 0
+    ref, tol = R.attend(f64(q), k, v, [pages * PAGE], 0.1)
+    kd, vd = torch.from_numpy(kc).to(gpu), torch.from_numpy(vc).to(gpu)
+    for _ in range(20):
+        err = i32([0], gpu)
+        out = KV.kv4_decode(q, kd, vd, i32(ids[None], gpu), i32([pages * PAGE], gpu), 0.1, split_tokens=pages * PAGE,
+                            error_word=err)[0]
+        assert int(err) == 6 and (np.abs(f64(out) - ref) <= tol).all()
+
+
 def test_decode_row_bits_do_not_depend_on_the_batch(gpu):
     rng = np.random.default_rng(10)
     lens = [200, 1, 77, 130]

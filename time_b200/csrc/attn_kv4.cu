@@ -487,6 +487,8 @@ kv4_decode_kernel(const Kv4Params p) {
             if (!(some >> c & 1))
                 for (int o = lane; o < kPage4 / 16; o += 32)
                     *reinterpret_cast<uint4*>(dst + c * kPage4 + o * 16) = make_uint4(0, 0, 0, 0);
+        // a later pair's bulk copy into this stage comes after the zeros
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (id >= 0) bulk_load(dst + lane * kPage4, cache + static_cast<size_t>(id) * page_stride, kPage4, &full[warp][stage]);
     };
