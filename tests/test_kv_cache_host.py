@@ -101,6 +101,15 @@ def test_decode_refusals(k, change, code):
     assert k.attn_kv4_decode_rows(*{**DECODE, **change}.values()) == code
 
 
+@pytest.mark.parametrize("split,splits,code", [
+    (8192, 262143, UNSUPPORTED), (8192, 262144, UNSUPPORTED), (16, 1 << 27, UNSUPPORTED), (48, 0x7FFFFFFF // 48, UNSUPPORTED),
+    (16, 0x7FFFFFFF, UNSUPPORTED), (8192, 262142, WORKSPACE), (16, (1 << 27) - 600, WORKSPACE)])
+def test_decode_splits_of_more_tokens_than_32_bits_count(k, split, splits, code):
+    """A split's first token and the end of a context are 32-bit numbers; what is refused for its workspace alone is not
+    refused before."""
+    assert k.attn_kv4_decode_rows(*{**DECODE, "split": split, "splits": splits}.values()) == code
+
+
 @pytest.mark.parametrize("change,code", [
     (dict(T=-1), INVALID), (dict(seqs=-1), INVALID), (dict(nq=34), INVALID), (dict(nq=3), INVALID), (dict(nkv=0), INVALID),
     (dict(d=64), INVALID), (dict(qs=511), INVALID), (dict(qs=516), INVALID), (dict(ks=128), INVALID), (dict(vs=250), INVALID),

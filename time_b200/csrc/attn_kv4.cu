@@ -868,6 +868,8 @@ moe_status_t attn_kv4_decode_rows(const void* q_bf16, const void* k_cache, const
         max_pages <= 0 || num_cache_pages <= 0 || !std::isfinite(scale * kLog2e))
         return MOE_ERR_INVALID_ARGUMENT;
     if (static_cast<long long>(B) * nkv > 65535 || static_cast<long long>(B) * nq > 0x7FFFFFFF) return MOE_ERR_UNSUPPORTED;
+    // positions are 32-bit numbers, one split behind the last included
+    if (static_cast<long long>(max_splits) * split_tokens > 0x7FFFFFFF - kMaxSplitPages * kPage) return MOE_ERR_UNSUPPORTED;
     if (B == 0) return MOE_OK;
     if (num_seqs <= 0) return MOE_ERR_INVALID_ARGUMENT;
     if (!q_bf16 || !k_cache || !v_cache || !page_table || !seq_lens || !workspace || !out_bf16)
