@@ -363,3 +363,37 @@ def test_short_tiles_right_behind_longer_ones(gpu, long, short, quant):
         assert torch.equal(out, want[0])
         if quant:
             assert torch.equal(oq, want[1]) and torch.equal(os_[:, :T], want[2])
+
+
+def e4m3_rows(oq, os_, T, nq):
+    """The e4m3 rows times their scales, [T][nq][128] in 64 bits."""
+    return oq.view(torch.float8_e4m3fn).double().reshape(T, nq, D) * os_[:, :T].double().t()[..., None]
+
+
+@pytest.mark.parametrize("G", [1, 12])
+@pytest.mark.parametrize("where", ["q", "k", "v", "v one dim", "v one dim of zeros"])
+def test_nan_reaches_the_quantised_rows(gpu, G, where):
+    """What is NaN in the bf16 rows is NaN in the e4m3 rows, rows that are NaN throughout among them; the rest keeps its
+    codes and scales."""
+    rng = np.random.default_rng(G)
+    n = 300
+    q, k, v = rows(rng, n, G, D).to(gpu), rows(rng, n, 1, D).to(gpu), rows(rng, n, 1, D).to(gpu)
+    if where == "v one dim of zeros":
+        v.zero_()
+    _, clean_q, clean_s = A.prompt_packed(q, k, v, cu_of([n], gpu), 0.1, quant=True)
+    for at in (0, 1, 70, 255, 299):
+        bad = {"q": q, "k": k, "v": v}
+        bad[where[0]] = b = bad[where[0]].clone()
+        b[at, :, 7 if where[0] != "v" or where != "v" else slice(None)] = float("nan")
+        out, oq, os_ = A.prompt_packed(bad["q"], bad["k"], bad["v"], cu_of([n], gpu), 0.1, quant=True)
+        hit = torch.zeros(n, G, D, dtype=torch.bool, device=gpu)
+        if where == "q":
+            hit[at] = True
+        elif where in ("k", "v"):
+            hit[at:] = True
+        else:
+            hit[at:, :, 7] = True
+        assert torch.equal(torch.isnan(out), hit) and torch.equal(torch.isnan(e4m3_rows(oq, os_, n, G)), hit)
+        rows_hit = hit.any(dim=2)
+        assert torch.equal(oq.view(n, G, D)[~rows_hit], clean_q.view(n, G, D)[~rows_hit])
+        assert torch.equal(os_[:, :n].t()[~rows_hit], clean_s[:, :n].t()[~rows_hit])

@@ -300,7 +300,7 @@ __device__ __noinline__ void epilogue_dirty(const PromptParams& p, uint32_t to, 
                     amax = fmaxf(amax, fabsf(x));
                     if (store) p.out[out_row * kD + 16 * c + e] = __float2bfloat16_rn(x);
                 } else if (store) {
-                    p.out_q[out_row * kD + 16 * c + e] = amax > 0.0f ? static_cast<uint8_t>(cvt_e4m3x2(x * qi, 0.0f)) : 0;
+                    p.out_q[out_row * kD + 16 * c + e] = static_cast<uint8_t>(cvt_e4m3x2(x * qi, 0.0f));
                 }
             }
         }
@@ -510,6 +510,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                     for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(o[e]) * inv;
                 };
                 if (p.out_q) {
+                    // The scale goes by the largest number; a NaN gets the code NaN, also where there is no number or only
+                    // zeros (qi = 0).
                     float amax = 0.0f;
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
@@ -526,9 +528,8 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                         uint32_t wt[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            wt[e] = amax > 0.0f ? cvt_e4m3x2(x[4 * e] * qi, x[4 * e + 1] * qi) |
-                                                      static_cast<uint32_t>(cvt_e4m3x2(x[4 * e + 2] * qi, x[4 * e + 3] * qi)) << 16
-                                                : 0u;
+                            wt[e] = cvt_e4m3x2(x[4 * e] * qi, x[4 * e + 1] * qi) |
+                                    static_cast<uint32_t>(cvt_e4m3x2(x[4 * e + 2] * qi, x[4 * e + 3] * qi)) << 16;
                         if (store) st_global_32(p.out_q + out_row * kD + 32 * c, wt);
                     }
                     if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
