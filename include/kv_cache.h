@@ -75,9 +75,10 @@ int attn_kv4_split_tokens(int B, int nkv, int max_context);
 size_t attn_kv4_decode_workspace_bytes(int B, int nq, int max_splits);
 
 /* attn_decode_paged_rows over 4-bit pages: same arguments, outputs (bf16 rows
- * and, when out_q is given, their e4m3 1x128 quantisation) and checks.  Rows
- * with seq_lens[b] <= 0 or row_seq outside [0, num_seqs) get zeros; slots past
- * a sequence's length are not read into the result whatever they hold.
+ * and, when out_q is given, their e4m3 1x128 quantisation) and checks; NaN in a
+ * bf16 row is the e4m3 NaN in out_q, whatever else the row holds.  Rows with
+ * seq_lens[b] <= 0 or row_seq outside [0, num_seqs) get zeros; slots past a
+ * sequence's length are not read into the result whatever they hold.
  * max_splits * split_tokens is at most 2^31 - 8193 (else MOE_ERR_UNSUPPORTED).  A
  * row's bits depend on split_tokens and on nothing else of the call.  scale is
  * finite, of any sign.  The workspace is the call's own until it has run: calls

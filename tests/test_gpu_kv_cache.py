@@ -642,3 +642,43 @@ def test_tensors_on_the_host_are_refused(gpu):
                     call(*args[:i], a.to(cpu), *args[i + 1:])
         call(*args)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("split", [128, 16])
+@pytest.mark.parametrize("where", ["q", "k", "v", "v one group", "v one group of zeros"])
+def test_decode_nan_reaches_the_quantised_rows(gpu, where, split):
+    """What is NaN in the bf16 rows is NaN in the e4m3 rows, rows that are NaN throughout among them, with one split and with
+    several; the rest keeps its codes and scales."""
+    rng = np.random.default_rng(split)
+    nq, n = 6, 100
+    kc, vc = random_cache(rng, 16, 1)
+    if where == "v one group of zeros":
+        vc[...] = 0                                        # scales of 0
+    pt = i32([[0, 1, 2, 3, 4, 5, 6, 15], list(range(7, 15))], gpu)
+    q = normal_bf16(rng, 2, nq, D)
+    run = lambda: KV.kv4_decode(q.to(gpu), torch.from_numpy(kc).to(gpu), torch.from_numpy(vc).to(gpu), pt, i32([n, n], gpu),  # noqa: E731
+                                0.1, split_tokens=split, quant=True)
+    clean = run()
+    hit = np.zeros((2, nq, D), bool)
+    nan = [0xC0, 0x7F]
+    at = R.CODE_BYTES + 8 * 4                              # scales of token 4 of a page
+    if where == "q":
+        q[0, 1, 7] = float("nan")
+        hit[0, 1] = True
+    elif where == "k":
+        kc[3, 0, at + 2:at + 4] = nan
+        hit[0] = True
+    elif where == "v":
+        vc[3, 0, at:at + 8] = nan * 4
+        hit[0] = True
+    else:
+        vc[3, 0, at + 2:at + 4] = nan
+        hit[0, :, 32:64] = True
+    out, oq, os_ = run()
+    hit = torch.from_numpy(hit).to(gpu)
+    assert torch.equal(torch.isnan(out), hit)
+    held = oq.view(torch.float8_e4m3fn).double().reshape(2, nq, D) * os_[:, :2].double().t()[..., None]
+    assert torch.equal(torch.isnan(held), hit)
+    rest = ~hit.any(dim=2)
+    assert torch.equal(oq.view(2, nq, D)[rest], clean[1].view(2, nq, D)[rest])
+    assert torch.equal(os_[:, :2].t()[rest], clean[2][:, :2].t()[rest])
