@@ -682,3 +682,30 @@ def test_decode_nan_reaches_the_quantised_rows(gpu, where, split):
     rest = ~hit.any(dim=2)
     assert torch.equal(oq.view(2, nq, D)[rest], clean[1].view(2, nq, D)[rest])
     assert torch.equal(os_[:, :2].t()[rest], clean[2][:, :2].t()[rest])
+
+
+@pytest.mark.parametrize("nq,nkv,B,split", [(12, 1, 50, 16), (96, 8, 7, 32)])
+def test_decode_row_bits_do_not_depend_on_a_large_batch(gpu, nq, nkv, B, split):
+    """Rows of one to thirty splits alone and in a batch whose rows fill the GPU: the bf16 rows, the e4m3 rows and their
+    fp32 scales."""
+    rng = np.random.default_rng(B)
+    lens = [int(x) for x in rng.integers(1, 30 * split, B)]
+    lens[0], lens[1], lens[2] = 30 * split, 20 * split + 1, 1
+    pool = sum(map(R.pages, lens))
+    kc, vc = random_cache(rng, pool, nkv)
+    kd, vd = torch.from_numpy(kc).to(gpu), torch.from_numpy(vc).to(gpu)
+    pt = i32(table_of(rng, lens, pool), gpu)
+    q = normal_bf16(rng, B, nq, D).to(gpu)
+    assert B * nq > 4 * 148 > 6 * nq
+    out, oq, os_ = KV.kv4_decode(q, kd, vd, pt, i32(lens, gpu), 0.1, split_tokens=split, quant=True)
+    for b in range(B):
+        for rows in ([b], [b] * 5):
+            one, one_q, one_s = KV.kv4_decode(q[rows], kd, vd, pt, i32([lens[i] for i in rows], gpu), 0.1,
+                                              row_seq=i32(rows, gpu), split_tokens=split, quant=True)
+            assert torch.equal(one[-1], out[b]) and torch.equal(one_q[-1], oq[b])
+            assert torch.equal(one_s[:, len(rows) - 1], os_[:, b])
+    # and where one split holds the context, whether there is a second or not
+    short = i32([min(n, split) for n in lens], gpu)
+    a = KV.kv4_decode(q, kd, vd, pt, short, 0.1, split_tokens=split, max_splits=1, quant=True)
+    b = KV.kv4_decode(q, kd, vd, pt, short, 0.1, split_tokens=split, quant=True)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.equal(a[2][:, :B], b[2][:, :B])

@@ -693,7 +693,7 @@ kv4_decode_kernel(const Kv4Params p) {
         const float* mr = mo + r * kMergePad + d;
         const float acc = mr[0] * f.x + mr[kGPad * kMergePad] * f.y + mr[2 * kGPad * kMergePad] * f.z + mr[3 * kGPad * kMergePad] * f.w;
         if (p.max_splits == 1) {
-            write_row(p, b, kvh * p.G + r, acc / fac[kGPad * kWarps + r * 2 + 1], red);
+            write_row(p, b, kvh * p.G + r, (acc + 0.0f) / fac[kGPad * kWarps + r * 2 + 1], red);   // -0 as the merge's sum has it
         } else {
             p.part_o[(base + r) * kD + d] = acc;
             if (d < 2) p.part_ml[(base + r) * 2 + d] = fac[kGPad * kWarps + r * 2 + d];
@@ -701,14 +701,20 @@ kv4_decode_kernel(const Kv4Params p) {
     }
 }
 
-// Merge of a (row, query head)'s splits by 128 threads, one per dim, in kGroups
-// groups that take every kGroups-th split: four where there are few rows, so
-// that many splits are a few loads deep, one where the rows fill the GPU.  Every
-// warp works out the factors of 32 splits by itself, so the partials' loads wait
-// for nothing but the length.
+// Merge of a (row, query head)'s splits: sum g of kSums takes splits g, g + kSums,
+// ... in turns of kMergeTurn, and the sums are added in order.  Where there are few
+// rows, each sum has 128 threads of its own, one per dim, so that many splits are
+// a few loads deep; where the rows fill the GPU, the same threads hold all sums.
+// The steps are the same in both, so a row's bits do not tell which it was.  An
+// octet of lanes works out the factors of a sum's turn, every warp for itself, and
+// the partials' loads wait for nothing but the length.
+constexpr int kSums = 4;
+constexpr int kMergeTurn = 8;
 template <int kGroups>
 __global__ void __launch_bounds__(kGroups * kD)
 kv4_merge_kernel(const Kv4Params p) {
+    static_assert(kGroups == 1 || kGroups == kSums, "a thread holds one sum or all");
+    constexpr int kOwn = kSums / kGroups;
     __shared__ float red[kWarps], sum[kGroups][kD + 2];
     const int b = blockIdx.x / p.nq, h = blockIdx.x % p.nq;
     const int kvh = h / p.G, r = h % p.G;
@@ -717,57 +723,90 @@ kv4_merge_kernel(const Kv4Params p) {
                         ? 0 : clamp_len(p.seq_lens[b], p.max_pages, p.split_tokens, p.max_splits);
     const int ns = (len + p.split_tokens - 1) / p.split_tokens;
     const size_t base = (static_cast<size_t>(b) * p.nkv + kvh) * p.max_splits * p.G + r;
-    const size_t step = static_cast<size_t>(p.G) * kGroups;       // rows of the partials from one of the group's splits to its next
-    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + base + static_cast<size_t>(grp) * p.G;
-    const float* po = p.part_o + (base + static_cast<size_t>(grp) * p.G) * kD + d;
-    const int mine = ns > grp ? (ns - grp + kGroups - 1) / kGroups : 0;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + base;
+    const float* po = p.part_o + base * kD + d;
+    const int lane_sum = kGroups == 1 ? lane / kMergeTurn : grp;
     grid_dependency_wait();                        // the splits
-    float M = -INFINITY, L = 0.0f, acc = 0.0f;
-    for (int s0 = 0; s0 < mine; s0 += 32) {
-        const int n = min(32, mine - s0);
-        const float2 x = lane < n ? ml[static_cast<size_t>(s0 + lane) * step] : make_float2(-INFINITY, 0.0f);
-        float m = x.x;
+    float M = -INFINITY, L = 0.0f, acc[kOwn];      // M and L of lane_sum, acc of sums grp ..
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int u = 0; u < kOwn; ++u) acc[u] = 0.0f;
+    float2 x;
+    float v[kOwn][kMergeTurn];
+    auto load = [&](int s0) {
+        const int mine = s0 + lane_sum + lane % kMergeTurn * kSums;
+        x = mine < ns ? ml[static_cast<size_t>(mine) * p.G] : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+        for (int c = 0; c < kMergeTurn; ++c) {
+            if (kOwn > 1 && s0 + c * kSums >= ns) break;
+#pragma unroll
+            for (int u = 0; u < kOwn; ++u) {
+                const int s = s0 + grp + u + c * kSums;
+                v[u][c] = s < ns ? po[static_cast<size_t>(s) * p.G * kD] : 0.0f;
+            }
+        }
+    };
+    // A lone sum's next turn is on its way under this one (one context of 32768: 10.3 us instead of 10.9); with all sums in a
+    // thread that costs registers, and with them blocks (64 contexts of up to 16384, 64 heads: 171.5 us instead of 169.6).
+    constexpr bool kAhead = kOwn == 1;
+    if (kAhead) load(0);
+    for (int s0 = 0; s0 + grp < ns; s0 += kSums * kMergeTurn) {
+        if (!kAhead) load(s0);
+        const float2 x0 = x;
+        float v0[kOwn][kMergeTurn];
+#pragma unroll
+        for (int u = 0; u < kOwn; ++u)
+#pragma unroll
+            for (int c = 0; c < kMergeTurn; ++c) v0[u][c] = v[u][c];
+        if (kAhead && s0 + kSums * kMergeTurn < ns) load(s0 + kSums * kMergeTurn);
+        float m = x0.x;
+#pragma unroll
+        for (int o = kMergeTurn / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const float mn = fmaxf(M, m);
         const float keep = M == -INFINITY ? 1.0f : ex2(M - mn);
-        const float f = x.x == -INFINITY ? 1.0f : ex2(x.x - mn);   // no weight: l and o are 0 or NaN
-        acc *= keep;
-        float l = lane < n ? x.y * f : 0.0f;
+        const float f = x0.x == -INFINITY ? 1.0f : ex2(x0.x - mn);   // no weight: l and o are 0 or NaN
+        float l = __fmul_rn(x0.y, f);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        L = L * keep + l;
+        for (int o = kMergeTurn / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        L = fmaf(L, keep, l);
         M = mn;
 #pragma unroll
-        for (int c = 0; c < 32; c += 8) {
-            if (c >= n) break;
-            float v[8];
+        for (int u = 0; u < kOwn; ++u) acc[u] *= __shfl_sync(0xffffffffu, keep, u * kMergeTurn);
 #pragma unroll
-            for (int s = 0; s < 8; ++s) v[s] = c + s < n ? po[static_cast<size_t>(s0 + c + s) * step * kD] : 0.0f;
+        for (int c = 0; c < kMergeTurn; ++c) {
+            if (s0 + grp + c * kSums >= ns) break;
 #pragma unroll
-            for (int s = 0; s < 8; ++s) acc += v[s] * __shfl_sync(0xffffffffu, f, c + s);
+            for (int u = 0; u < kOwn; ++u) acc[u] = fmaf(v0[u][c], __shfl_sync(0xffffffffu, f, u * kMergeTurn + c), acc[u]);
         }
     }
     if constexpr (kGroups > 1) {
-        sum[grp][d] = acc;
+        sum[grp][d] = acc[0];
         if (d == 0) {
             sum[grp][kD] = M;
             sum[grp][kD + 1] = L;
         }
         __syncthreads();
         if (grp) return;
-        float top = M;
+    }
+    float Ms[kSums], top = -INFINITY, total = 0.0f;
 #pragma unroll
-        for (int g = 1; g < kGroups; ++g) top = fmaxf(top, sum[g][kD]);
-        acc = L = 0.0f;
+    for (int g = 0; g < kSums; ++g) {
+        if constexpr (kGroups > 1) Ms[g] = sum[g][kD];
+        else Ms[g] = __shfl_sync(0xffffffffu, M, g * kMergeTurn);
+        top = fmaxf(top, Ms[g]);
+    }
+    float Lt = 0.0f;
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            const float f = sum[g][kD] == -INFINITY ? 1.0f : ex2(sum[g][kD] - top);
-            acc += sum[g][d] * f;
-            L += sum[g][kD + 1] * f;
+    for (int g = 0; g < kSums; ++g) {
+        const float f = Ms[g] == -INFINITY ? 1.0f : ex2(Ms[g] - top);
+        if constexpr (kGroups > 1) {
+            total = fmaf(sum[g][d], f, total);
+            Lt = fmaf(sum[g][kD + 1], f, Lt);
+        } else {
+            total = fmaf(acc[g], f, total);
+            Lt = fmaf(__shfl_sync(0xffffffffu, L, g * kMergeTurn), f, Lt);
         }
     }
-    write_row(p, b, h, ns > 0 ? acc / L : 0.0f, red);
+    write_row(p, b, h, ns > 0 ? total / Lt : 0.0f, red);
 }
 
 }  // namespace
@@ -907,7 +946,7 @@ moe_status_t attn_kv4_decode_rows(const void* q_bf16, const void* k_cache, const
     kv4_decode_kernel<<<dim3(max_splits, B * nkv), kWarps * 32, kDecodeSmem, st>>>(p);
     const moe_status_t s = launch_status();
     if (s != MOE_OK || max_splits == 1) return s;
-    const cudaError_t e = B * nq < 4 * 148 ? launch_dependent(kv4_merge_kernel<4>, B * nq, 4 * kD, st, p)
+    const cudaError_t e = B * nq < 4 * 148 ? launch_dependent(kv4_merge_kernel<kSums>, B * nq, kSums * kD, st, p)
                                            : launch_dependent(kv4_merge_kernel<1>, B * nq, kD, st, p);
     return e == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
 }
