@@ -111,8 +111,9 @@ moe_status_t attn_paged_rows(const void* q_bf16, const void* k_cache, const void
  * input.  scale is finite, of any sign.  Rows in no sequence are left as they
  * were.  From the first bound that is out of order or outside 0..T on, sequences
  * are skipped (*error_word = 5).  A NaN or infinity in k or v reaches the rows
- * that attend it and no others, in out_q as the e4m3 NaN; a row's bits depend on
- * its own sequence alone.
+ * that attend it and no others, in out_q as the e4m3 NaN.  A weight counts as
+ * positive however small: an infinity in v is infinite in its dim, two of
+ * opposite signs are NaN.  A row's bits depend on its own sequence alone.
  * *error_word = 1: a wait inside the kernel gave up after two seconds and rows
  * are missing. */
 moe_status_t attn_prompt_packed(const void* q_bf16, long long q_stride, const void* k_bf16, long long k_stride,

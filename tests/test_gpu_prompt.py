@@ -397,3 +397,51 @@ def test_nan_reaches_the_quantised_rows(gpu, G, where):
         rows_hit = hit.any(dim=2)
         assert torch.equal(oq.view(n, G, D)[~rows_hit], clean_q.view(n, G, D)[~rows_hit])
         assert torch.equal(os_[:, :n].t()[~rows_hit], clean_s[:, :n].t()[~rows_hit])
+
+
+def same(a, b):
+    return torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(nan=0.0), b.nan_to_num(nan=0.0))
+
+
+@pytest.mark.parametrize("G", [1, 12])
+@pytest.mark.parametrize("scores", ["far below", "left behind", "alike"])
+def test_an_infinity_does_not_depend_on_the_tile(gpu, G, scores):
+    """A weight that underflows is still positive: an infinity in v is infinite in every row that attends it and two of
+    opposite signs are NaN, wherever the tiles begin; the other dims keep their bits, alone and in a batch."""
+    rng = np.random.default_rng(G)
+    n = 400
+    k, v = torch.zeros(n, 1, D), rows(rng, n, 1, D)
+    q = torch.zeros(n, G, D)
+    q[..., 0] = 1.0
+    c = torch.from_numpy(rng.standard_normal(n).astype(np.float32))
+    # some positions 300 below the rest, or every 64 positions 100 above those before
+    c += -300.0 * (torch.arange(n) % 50 == 3) if scores == "far below" else 100.0 * (torch.arange(n) // 64) if scores == "left behind" else 0
+    k[:, 0, 0] = c
+    q, k, v = q.to(torch.bfloat16).to(gpu), k.to(torch.bfloat16).to(gpu), v.to(gpu)
+    clean = A.prompt_packed(q, k, v, cu_of([n], gpu), 1.0, quant=True)
+    bad, want = v.clone(), clean[0].clone()
+    for dim, at in ((3, [3]), (5, [53, 203]), (70, [203]), (127, [63]), (64, [64])):
+        bad[at, 0, dim] = float("inf")
+        want[at[0]:, :, dim] = float("inf")
+    bad[103, 0, 9] = float("-inf")
+    want[103:, :, 9] = float("-inf")
+    bad[3, 0, 11], bad[253, 0, 11] = float("inf"), float("-inf")
+    want[3:253, :, 11], want[253:, :, 11] = float("inf"), float("nan")
+    bad[153, 0, 80] = float("nan")
+    want[153:, :, 80] = float("nan")
+    alone = A.prompt_packed(q, k, bad, cu_of([n], gpu), 1.0)[0]
+    assert same(alone, want)
+    # among many others the tiles are of another size
+    r = 40
+    batch = A.prompt_packed(q.repeat(r, 1, 1), k.repeat(r, 1, 1), bad.repeat(r, 1, 1), cu_of([n] * r, gpu), 1.0, quant=True)
+    one = A.prompt_packed(q, k, bad, cu_of([n], gpu), 1.0, quant=True)
+    assert same(one[0], want)
+    for i in (0, 17, r - 1):
+        s = slice(i * n, (i + 1) * n)
+        assert same(batch[0][s], want)
+        assert torch.equal(batch[1][s], one[1]) and same(batch[2][:, s], one[2][:, :n])
+    hit = ~torch.isfinite(want)
+    held = one[1].view(torch.float8_e4m3fn).double().reshape(n, G, D) * one[2][:, :n].double().t()[..., None]
+    assert not torch.isfinite(held[hit]).any()
+    rest = ~hit.any(dim=2)
+    assert torch.equal(one[1].view(n, G, D)[rest], clean[1].view(n, G, D)[rest])

@@ -275,42 +275,150 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     return d;
 }
 
-// Epilogue of a row of a tile with NaN or infinite values in V that not every
-// row attends: they were zeroed for the MMA, so a row that attends them adds
-// them here (a positive weight times one of them is the same again).
-__device__ __noinline__ void epilogue_dirty(const PromptParams& p, uint32_t to, float inv, long long first, int pos0, int pos,
-                                            int kvh, int head, bool store) {
-    const __nv_bfloat16* vrow = p.v + first * p.v_stride + kvh * kD;
+// The larger of each of two bf16 pairs, NaN if either is.
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+// NaN and infinities in V.  A weight is positive however small, so a row that
+// attends infinities of one sign is that infinity in their dim, and with both
+// signs or a NaN it is NaN.  The MMAs give that unless a weight, or the factor of a
+// rescale, is too small for fp32: 0 times infinity.  And they see zeros in place
+// of such values behind a tile's first position.  Where either may be, the epilogue
+// settles these dims from V itself: what a row is depends on no tile.
+struct NonFinite {
+    int plus[4], minus[4], nan[4];                      // first positions with each in dims 4 lane .. 4 lane + 3
+};
+
+// Over the first n positions of a sequence, by a warp; no further than to where every dim is NaN.
+__device__ __forceinline__ NonFinite find_nonfinite(const PromptParams& p, long long first, int kvh, int n) {
+    const int lane = threadIdx.x & 31;
+    constexpr int kNone = 0x7FFFFFFF, kTurn = 8;
+    NonFinite at;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) at.plus[e] = at.minus[e] = at.nan[e] = kNone;
+    const __nv_bfloat16* v = p.v + first * p.v_stride + kvh * kD + 4 * lane;
+    for (int j0 = 0; j0 < n; j0 += kTurn) {
+        uint2 x[kTurn];
+#pragma unroll
+        for (int i = 0; i < kTurn; ++i) x[i] = j0 + i < n ? *reinterpret_cast<const uint2*>(v + (j0 + i) * p.v_stride) : make_uint2(0, 0);
+        bool all_nan = true;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int i = 0; i < kTurn; ++i) {
+                const uint32_t y = ((e < 2 ? x[i].x : x[i].y) >> (16 * (e & 1))) & 0xFFFFu;
+                if (y == 0x7F80u) at.plus[e] = min(at.plus[e], j0 + i);
+                else if (y == 0xFF80u) at.minus[e] = min(at.minus[e], j0 + i);
+                else if ((y & 0x7F80u) == 0x7F80u) at.nan[e] = min(at.nan[e], j0 + i);
+            }
+            all_nan &= at.nan[e] != kNone;
+        }
+        if (__all_sync(0xffffffffu, all_nan)) break;
+    }
+    return at;
+}
+
+// Dim 4 c + e of the row at `pos`: bf16 bits of what it is, 0 where it attends numbers only; the whole warp comes here.
+__device__ __forceinline__ uint32_t settled(const NonFinite& at, int c, int e, int pos) {
+    const bool plus = __shfl_sync(0xffffffffu, at.plus[e], c) <= pos, minus = __shfl_sync(0xffffffffu, at.minus[e], c) <= pos;
+    const bool nan = __shfl_sync(0xffffffffu, at.nan[e], c) <= pos;
+    return nan || (plus && minus) ? 0x7FFFu : plus ? 0x7F80u : minus ? 0xFF80u : 0u;
+}
+
+// bf16 rows as they lie in shared memory (see the epilogue), one a lane; `sums`: the row's sum of weights is a number above 0.
+__device__ __noinline__ void settle_rows(const PromptParams& p, uint8_t* rows_sm, int i_row, long long first, int pos, int kvh,
+                                         bool sums) {
+    const NonFinite at = find_nonfinite(p, first, kvh, __reduce_max_sync(0xffffffffu, pos) + 1);
+    for (int c = 0; c < 32; ++c) {
+        uint16_t* x = reinterpret_cast<uint16_t*>(rows_sm + (c >> 4) * kQHalf + i_row * 128 + ((((c >> 1) ^ i_row) & 7) << 4) + (c & 1) * 8);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t y = settled(at, c, e, pos);
+            if (y && sums) x[e] = static_cast<uint16_t>(y);
+        }
+    }
+}
+
+// The e4m3 rows and their scales, from the output in TMEM.
+__device__ __noinline__ void settle_quantised(const PromptParams& p, uint32_t to, float inv, long long first, int pos, int kvh,
+                                              int head, bool sums, bool store) {
+    const NonFinite at = find_nonfinite(p, first, kvh, __reduce_max_sync(0xffffffffu, pos) + 1);
     const long long out_row = (first + pos) * p.nq + head;
     float amax = 0.0f;
-    for (int pass = 0; pass < (p.out_q ? 2 : 1); ++pass) {
+    for (int pass = 0; pass < 2; ++pass) {
         const float qi = amax > 0.0f ? 448.0f / amax : 0.0f;
-        for (int c = 0; c < 8; ++c) {
+        for (int b = 0; b < 8; ++b) {
             uint32_t o[16];
-            tmem_ld16(to + 16 * c, o);
+            __syncwarp();
+            tmem_ld16(to + 16 * b, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float x = __uint_as_float(o[e]) * inv;
-                for (int j = pos0 + 1; j <= pos; ++j) {
-                    const float y = __bfloat162float(vrow[j * p.v_stride + 16 * c + e]);
-                    if (!isfinite(y)) x += y;
+            for (int c = 0; c < 4; ++c) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t y = settled(at, 4 * b + c, e, pos);
+                    x[e] = y && sums ? __uint_as_float(y << 16) : __uint_as_float(o[4 * c + e]) * inv;
+                    amax = pass == 0 ? fmaxf(amax, fabsf(x[e])) : amax;
                 }
-                if (pass == 0) {
-                    amax = fmaxf(amax, fabsf(x));
-                    if (store) p.out[out_row * kD + 16 * c + e] = __float2bfloat16_rn(x);
-                } else if (store) {
-                    p.out_q[out_row * kD + 16 * c + e] = static_cast<uint8_t>(cvt_e4m3x2(x * qi, 0.0f));
-                }
+                if (pass == 1 && store)
+                    *reinterpret_cast<uint32_t*>(p.out_q + out_row * kD + 16 * b + 4 * c) =
+                        cvt_e4m3x2(x[0] * qi, x[1] * qi) | static_cast<uint32_t>(cvt_e4m3x2(x[2] * qi, x[3] * qi)) << 16;
             }
         }
     }
-    if (p.out_q && store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
+    if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
+}
+
+// The e4m3 rows and their scales.  The scale goes by the largest number; a NaN gets the code NaN, also where there is no
+// number or only zeros (qi = 0).
+__device__ __noinline__ void quantise_output(const PromptParams& p, uint32_t to, float inv, long long first, int pos, int kvh, int head,
+                                             bool sums, bool store, bool dirty) {
+    auto columns = [&](int c, float (&x)[32]) {         // 32 dims of the row
+        uint32_t o[32];
+        __syncwarp();
+        tmem_ld32(to + 32 * c, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(o[e]) * inv;
+    };
+    const long long out_row = (first + pos) * p.nq + head;
+    float amax = 0.0f, nan = 0.0f;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        float x[32];
+        columns(c, x);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) amax = fmaxf(amax, fabsf(x[e]));
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) nan = max3_nan(nan, x[e], x[e + 1]);
+    }
+    if (dirty || __any_sync(0xffffffffu, nan != nan && sums && store)) {
+        settle_quantised(p, to, inv, first, pos, kvh, head, sums, store);
+        return;
+    }
+    const float qi = amax > 0.0f ? 448.0f / amax : 0.0f;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        float x[32];
+        columns(c, x);
+        uint32_t wt[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            wt[e] = cvt_e4m3x2(x[4 * e] * qi, x[4 * e + 1] * qi) |
+                    static_cast<uint32_t>(cvt_e4m3x2(x[4 * e + 2] * qi, x[4 * e + 3] * qi)) << 16;
+        if (store) st_global_32(p.out_q + out_row * kD + 32 * c, wt);
+    }
+    if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
-prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-              const __grid_constant__ CUtensorMap vmap, const __grid_constant__ CUtensorMap omap) {
+prompt_kernel(const __grid_constant__ PromptParams p, const __grid_constant__ CUtensorMap qmap,
+              const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+              const __grid_constant__ CUtensorMap omap) {
     extern __shared__ uint8_t sm_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sm_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* q_s = sm;                                  // [2 slots][2 halves][256 rows][128 B]
@@ -480,7 +588,7 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
             auto chunk = [&](int i, int c) {
                 return reinterpret_cast<uint4*>(rows_sm + (c >> 3) * kQHalf + i * 128 + (((c ^ i) & 7) << 4));
             };
-            bool box = rows == tile_pos * p.G;
+            const bool box = rows == tile_pos * p.G;
 #pragma unroll 1
             for (int t = 0; t < mt; ++t) {
                 const int i_row = t * 128 + (threadIdx.x & 127);
@@ -488,52 +596,18 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                 if (!(ok = all(wait(&bars.o_full[t], (o_phase >> t) & 1)))) break;
                 o_phase ^= 1u << t;
                 tc_fence_after();
-                const float inv = 1.0f / l_s[i_row];
+                const float l = l_s[i_row], inv = 1.0f / l;
                 const bool dirty = *static_cast<volatile const int*>(&w.dirty) != 0;
                 const int at = group_div(min(i_row, rows - 1), g_inv);
                 const int pos = pos0 + at;
                 const int head = kvh * p.G + min(i_row, rows - 1) - at * p.G;
                 const bool store = i_row < rows;
-                const long long out_row = (first + pos) * p.nq + head;
-                if (dirty) {
-                    box = false;
-                    epilogue_dirty(p, to, inv, first, pos0, pos, kvh, head, store);
-                    tc_fence_before();
-                    mbar_arrive(&bars.o_free[t]);
-                    continue;
-                }
-                auto columns = [&](int c, float (&x)[32]) {     // 32 dims of the row
-                    uint32_t o[32];
-                    tmem_ld32(to + 32 * c, o);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(o[e]) * inv;
-                };
+                const bool sums = l > 0.0f;             // else the row is NaN, whatever V holds
                 if (p.out_q) {
-                    // The scale goes by the largest number; a NaN gets the code NaN, also where there is no number or only
-                    // zeros (qi = 0).
-                    float amax = 0.0f;
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        float x[32];
-                        columns(c, x);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) amax = fmaxf(amax, fabsf(x[e]));
-                    }
-                    const float qi = amax > 0.0f ? 448.0f / amax : 0.0f;
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        float x[32];
-                        columns(c, x);
-                        uint32_t wt[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            wt[e] = cvt_e4m3x2(x[4 * e] * qi, x[4 * e + 1] * qi) |
-                                    static_cast<uint32_t>(cvt_e4m3x2(x[4 * e + 2] * qi, x[4 * e + 3] * qi)) << 16;
-                        if (store) st_global_32(p.out_q + out_row * kD + 32 * c, wt);
-                    }
-                    if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
+                    quantise_output(p, to, inv, first, pos, kvh, head, sums, store, dirty);
+                    __syncwarp();
                 }
+                uint32_t nan = 0;
 #pragma unroll 1
                 for (int c = 0; c < 2; ++c) {
                     uint32_t o[64];
@@ -544,11 +618,17 @@ prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap qmap, co
                         tc_fence_before();
                         mbar_arrive(&bars.o_free[t]);   // the next tile may write its output
                     }
-                    auto pack = [&](int e) { return pack_bf16(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv); };
+                    auto pack = [&](int e) {
+                        const uint32_t x = pack_bf16(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+                        nan = max2_nan(nan, x);
+                        return x;
+                    };
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         *chunk(i_row, 8 * c + e) = make_uint4(pack(8 * e), pack(8 * e + 2), pack(8 * e + 4), pack(8 * e + 6));
                 }
+                const bool is_nan = (nan & 0x7FFFu) > 0x7F80u || (nan & 0x7FFF0000u) > 0x7F800000u;
+                if (dirty || __any_sync(0xffffffffu, is_nan && sums && store)) settle_rows(p, rows_sm, i_row, first, pos, kvh, sums);
                 if (box) continue;
                 __syncwarp();
                 const int row0 = t * 128 + (warp & 3) * 32;
