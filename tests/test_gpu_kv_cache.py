@@ -709,3 +709,25 @@ def test_decode_row_bits_do_not_depend_on_a_large_batch(gpu, nq, nkv, B, split):
     a = KV.kv4_decode(q, kd, vd, pt, short, 0.1, split_tokens=split, max_splits=1, quant=True)
     b = KV.kv4_decode(q, kd, vd, pt, short, 0.1, split_tokens=split, quant=True)
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and torch.equal(a[2][:, :B], b[2][:, :B])
+
+
+@pytest.mark.parametrize("split", [64, 16])
+def test_decode_quantised_rows_of_tiny_values(gpu, split):
+    """Rows whose 448 / max is past the fp32 range: zeros stay zeros, the rest within half an e4m3 step."""
+    rng = np.random.default_rng(15)
+    nq, n = 6, 50
+    for mag in (1e-36, 2.0 ** -125):
+        x = np.zeros((n, D), np.float32)
+        x[:, :64] = np.sign(rng.standard_normal((n, 64))) * mag
+        kc, vc = random_cache(rng, 4, 1)
+        for t, (codes, s) in enumerate(zip(*R.quantise(x))):
+            R.store(vc[t // PAGE, 0], "v", t % PAGE, codes, s)
+        q = normal_bf16(rng, 1, nq, D).to(gpu)
+        out, oq, os_ = KV.kv4_decode(q, torch.from_numpy(kc).to(gpu), torch.from_numpy(vc).to(gpu), i32([[0, 1, 2, 3]], gpu),
+                                     i32([n], gpu), 0.1, split_tokens=split, quant=True)
+        got = out.double()
+        held = oq.view(torch.float8_e4m3fn).double().reshape(1, nq, D) * os_[:, :1].double().t()[..., None]
+        # the scale is a subnormal number, half of 2^-149 off; the row's bf16 rounding may be of one, too
+        amax = got.abs().amax(dim=2, keepdim=True) * (1 + 2.0 ** -7) + 2.0 ** -134
+        tol = (2.0 ** -4 + 2.0 ** -7) * got.abs() + amax / 448 * 2.0 ** -10 * 1.01 + 448 * 2.0 ** -150 + 2.0 ** -134
+        assert not held[..., 64:].any() and ((held - got).abs() <= tol).all()

@@ -445,3 +445,19 @@ def test_an_infinity_does_not_depend_on_the_tile(gpu, G, scores):
     assert not torch.isfinite(held[hit]).any()
     rest = ~hit.any(dim=2)
     assert torch.equal(one[1].view(n, G, D)[rest], clean[1].view(n, G, D)[rest])
+
+
+def test_quantised_rows_of_tiny_values(gpu):
+    """Rows whose 448 / max is past the fp32 range: zeros stay zeros, the rest within half an e4m3 step."""
+    n, nq = 20, 12
+    rng = np.random.default_rng(14)
+    q, k = rows(rng, n, nq, D).to(gpu), rows(rng, n, 1, D).to(gpu)
+    for mag in (1e-36, 2.0 ** -125):
+        v = (rows(rng, n, 1, D).sign() * mag).to(torch.bfloat16).to(gpu)
+        v[..., 64:] = 0
+        out, oq, os_ = A.prompt_packed(q, k, v, cu_of([n], gpu), 0.1, quant=True)
+        got, held = out.double(), e4m3_rows(oq, os_, n, nq)
+        # the scale is a subnormal number, half of 2^-149 off; the row's bf16 rounding may be of one, too
+        amax = got.abs().amax(dim=2, keepdim=True) * (1 + 2.0 ** -7) + 2.0 ** -134
+        tol = (2.0 ** -4 + 2.0 ** -7) * got.abs() + amax / 448 * 2.0 ** -10 * 1.01 + 448 * 2.0 ** -150 + 2.0 ** -134
+        assert not held[..., 64:].any() and ((held - got).abs() <= tol).all()

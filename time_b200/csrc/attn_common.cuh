@@ -45,6 +45,23 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
+// ---------------------------------------------------------------- e4m3 rows
+
+// Codes of a row whose largest number is amax are e4m3(x * up * inv), values code
+// * scale.  The scale goes by the numbers: a NaN gets the code NaN, also where there
+// is no number or only zeros (inv = 0).  448 / amax is past the fp32 range below
+// 1.3e-36, so rows that small are taken 2^64 times their size.
+struct E4m3Row {
+    float up, inv, scale;
+};
+__device__ __forceinline__ E4m3Row e4m3_row(float amax) {
+    E4m3Row r;
+    r.up = amax < 7.8886090522101181e-31f ? 18446744073709551616.0f : 1.0f;      // 2^-100, 2^64
+    r.inv = amax > 0.0f ? 448.0f / (amax * r.up) : 0.0f;
+    r.scale = amax > 0.0f ? amax / 448.0f : 0.0f;
+    return r;
+}
+
 // ---------------------------------------------------------------- host
 
 inline moe_status_t launch_status() {

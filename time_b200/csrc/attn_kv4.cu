@@ -385,10 +385,9 @@ __device__ __forceinline__ void write_row(const Kv4Params& p, int b, int h, floa
         if ((d & 31) == 0) red[d >> 5] = a;
         named_bar_sync(1, kD);
         const float amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        // the largest number; a NaN gets the code NaN, also where there is no number or only zeros
-        const float qi = amax > 0.0f ? 448.0f / amax : 0.0f;
-        p.out_q[(static_cast<size_t>(b) * p.nq + h) * kD + d] = static_cast<uint8_t>(cvt_e4m3x2(v * qi, 0.0f) & 0xFFu);
-        if (d == 0) p.out_s[static_cast<size_t>(h) * p.out_ld + b] = amax > 0.0f ? amax / 448.0f : 0.0f;
+        const E4m3Row r = e4m3_row(amax);
+        p.out_q[(static_cast<size_t>(b) * p.nq + h) * kD + d] = static_cast<uint8_t>(cvt_e4m3x2(v * r.up * r.inv, 0.0f) & 0xFFu);
+        if (d == 0) p.out_s[static_cast<size_t>(h) * p.out_ld + b] = r.scale;
     }
 }
 

@@ -349,7 +349,7 @@ __device__ __noinline__ void settle_quantised(const PromptParams& p, uint32_t to
     const long long out_row = (first + pos) * p.nq + head;
     float amax = 0.0f;
     for (int pass = 0; pass < 2; ++pass) {
-        const float qi = amax > 0.0f ? 448.0f / amax : 0.0f;
+        const E4m3Row r = e4m3_row(amax);
         for (int b = 0; b < 8; ++b) {
             uint32_t o[16];
             __syncwarp();
@@ -366,15 +366,15 @@ __device__ __noinline__ void settle_quantised(const PromptParams& p, uint32_t to
                 }
                 if (pass == 1 && store)
                     *reinterpret_cast<uint32_t*>(p.out_q + out_row * kD + 16 * b + 4 * c) =
-                        cvt_e4m3x2(x[0] * qi, x[1] * qi) | static_cast<uint32_t>(cvt_e4m3x2(x[2] * qi, x[3] * qi)) << 16;
+                        cvt_e4m3x2(x[0] * r.up * r.inv, x[1] * r.up * r.inv) |
+                        static_cast<uint32_t>(cvt_e4m3x2(x[2] * r.up * r.inv, x[3] * r.up * r.inv)) << 16;
             }
         }
     }
-    if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
+    if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = e4m3_row(amax).scale;
 }
 
-// The e4m3 rows and their scales.  The scale goes by the largest number; a NaN gets the code NaN, also where there is no
-// number or only zeros (qi = 0).
+// The e4m3 rows and their scales.
 __device__ __noinline__ void quantise_output(const PromptParams& p, uint32_t to, float inv, long long first, int pos, int kvh, int head,
                                              bool sums, bool store, bool dirty) {
     auto columns = [&](int c, float (&x)[32]) {         // 32 dims of the row
@@ -400,7 +400,7 @@ __device__ __noinline__ void quantise_output(const PromptParams& p, uint32_t to,
         settle_quantised(p, to, inv, first, pos, kvh, head, sums, store);
         return;
     }
-    const float qi = amax > 0.0f ? 448.0f / amax : 0.0f;
+    const E4m3Row r = e4m3_row(amax);
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
         float x[32];
@@ -408,11 +408,11 @@ __device__ __noinline__ void quantise_output(const PromptParams& p, uint32_t to,
         uint32_t wt[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            wt[e] = cvt_e4m3x2(x[4 * e] * qi, x[4 * e + 1] * qi) |
-                    static_cast<uint32_t>(cvt_e4m3x2(x[4 * e + 2] * qi, x[4 * e + 3] * qi)) << 16;
+            wt[e] = cvt_e4m3x2(x[4 * e] * r.up * r.inv, x[4 * e + 1] * r.up * r.inv) |
+                    static_cast<uint32_t>(cvt_e4m3x2(x[4 * e + 2] * r.up * r.inv, x[4 * e + 3] * r.up * r.inv)) << 16;
         if (store) st_global_32(p.out_q + out_row * kD + 32 * c, wt);
     }
-    if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = amax > 0.0f ? amax / 448.0f : 0.0f;
+    if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = r.scale;
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
