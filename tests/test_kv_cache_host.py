@@ -187,6 +187,25 @@ def test_python_write_checks(change):
                           c, c, 4, 64, args["inv_freq"], seq_lens_out=args["seq_lens_out"], error_word=args["error_word"])
 
 
+@pytest.mark.parametrize("shape", [(8,), (2, 2, 2), ()])
+@pytest.mark.parametrize("rows", [False, True])
+def test_page_tables_have_two_dimensions(shape, rows):
+    import torch
+    i32 = lambda *n: torch.zeros(*n, dtype=torch.int32)
+    c = torch.zeros(4, 1, 1152, dtype=torch.uint8)
+    table, seq = torch.zeros(shape, dtype=torch.int32), i32(2) if rows else None
+    with pytest.raises(ValueError, match="page table"):
+        KV.kv4_rope_write(torch.zeros(2, 6 * 128, dtype=torch.bfloat16), i32(2), seq, table, c, c, 4, 64, torch.zeros(32))
+    with pytest.raises(ValueError, match="page table"):
+        KV.kv4_read_rows(c, c, i32(2), seq, table)
+    with pytest.raises(ValueError, match="page table"):
+        KV.kv4_decode(torch.zeros(2, 4, 128, dtype=torch.bfloat16), c, c, table, i32(2), 0.1, row_seq=seq)
+    with pytest.raises(ValueError, match="page table|page-table"):
+        KV.fork_pages(c[None], table, i32(2), i32(2))
+    with pytest.raises(ValueError, match="page table|page-table"):
+        KV.compact_pages(c[None], table, i32(2))
+
+
 # ---------------------------------------------------------------- the plain statements themselves
 
 def test_quantiser_by_hand():

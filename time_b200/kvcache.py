@@ -65,6 +65,14 @@ def _check_kv4(k_cache, v_cache):
         raise ValueError(f"k_cache and v_cache are contiguous uint8 tensors [pages][nkv][{PAGE4_BYTES}]")
 
 
+def _check_page_table(page_table, rows, row_seq):
+    """Two dimensions, and where rows map to themselves one row each."""
+    if page_table.dim() != 2:
+        raise ValueError("the page table is a tensor [sequences][pages]")
+    if row_seq is None and page_table.shape[0] < rows:
+        raise ValueError("the page table has a row per row of the call when row_seq is None")
+
+
 @functools.lru_cache(maxsize=1024)
 def _splits(B: int, nq: int, nkv: int, max_context: int, split_tokens: int | None, max_splits: int | None):
     """(tokens of a split, splits, workspace bytes)."""
@@ -96,8 +104,7 @@ def kv4_rope_write(qkv, positions, row_seq, page_table, k_cache, v_cache, nq: in
     if inv_freq is not None and (inv_freq.numel() < rot // 2 or inv_freq.dtype is not torch.float32 or
                                  not inv_freq.is_contiguous()):
         raise ValueError("inv_freq has rot / 2 contiguous float32 entries")
-    if row_seq is None and page_table.shape[0] < B:
-        raise ValueError("the page table has a row per row of qkv when row_seq is None")
+    _check_page_table(page_table, B, row_seq)
     return A.on_stream(qkv, stream, _rope_write, qkv, positions, row_seq, page_table, k_cache, v_cache, nq, rot, inv_freq,
                        keys, seq_lens_out, error_word)
 
@@ -121,8 +128,9 @@ def kv4_read_rows(k_cache, v_cache, positions, row_seq, page_table, error_word=N
     _check_kv4(k_cache, v_cache)
     A.check_i32(positions, row_seq, page_table, error_word)
     B = positions.numel()
-    if (B if row_seq is None else row_seq.numel()) != B or (row_seq is None and page_table.shape[0] < B):
+    if row_seq is not None and row_seq.numel() != B:
         raise ValueError("row_seq has one entry per position")
+    _check_page_table(page_table, B, row_seq)
     return A.on_stream(k_cache, stream, _read_rows, k_cache, v_cache, positions, row_seq, page_table, error_word)
 
 
@@ -152,8 +160,7 @@ def kv4_decode(q, k_cache, v_cache, page_table, seq_lens, scale: float, row_seq=
     B = q.shape[0]
     if seq_lens.numel() != B or (B if row_seq is None else row_seq.numel()) != B:
         raise ValueError("seq_lens and row_seq have one entry per row of q")
-    if row_seq is None and page_table.shape[0] < B:
-        raise ValueError("the page table has a row per row of q when row_seq is None")
+    _check_page_table(page_table, B, row_seq)
     return A.on_stream(q, stream, _decode, q, k_cache, v_cache, page_table, seq_lens, scale, row_seq, split_tokens,
                        max_splits, quant, workspace, error_word)
 
@@ -196,7 +203,7 @@ def _cache_args(caches):
 
 def _check_table(table, lens):
     if table.dim() != 2 or lens.numel() != table.shape[0]:
-        raise ValueError("lens has one entry per page-table row")
+        raise ValueError("the page table is a tensor [sequences][pages] and lens has one entry per row of it")
 
 
 def fork_pages(caches, table, lens, parents, reserve=None, workspace=None, error_word=None, stream=None):
