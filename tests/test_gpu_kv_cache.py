@@ -731,3 +731,22 @@ def test_decode_quantised_rows_of_tiny_values(gpu, split):
         amax = got.abs().amax(dim=2, keepdim=True) * (1 + 2.0 ** -7) + 2.0 ** -134
         tol = (2.0 ** -4 + 2.0 ** -7) * got.abs() + amax / 448 * 2.0 ** -10 * 1.01 + 448 * 2.0 ** -150 + 2.0 ** -134
         assert not held[..., 64:].any() and ((held - got).abs() <= tol).all()
+
+
+def test_streams_of_another_device_are_refused(gpu):
+    """Launches on another device's stream would run there on this one's tensors.  A stand-in has what is asked of a stream."""
+    other = type("Stream", (), {"device_index": 1, "cuda_stream": 0})()
+    c = KV.kv4_cache(4, 1, gpu)
+    z = lambda *n: torch.zeros(*n, dtype=torch.int32, device=gpu)
+    q = torch.zeros(2, 4, D, dtype=torch.bfloat16, device=gpu)
+    for call in (lambda s: KV.kv4_rope_write(torch.zeros(2, 6 * D, dtype=torch.bfloat16, device=gpu), z(2), z(2), z(2, 4), c, c, 4,
+                                             64, torch.zeros(32, device=gpu), stream=s),
+                 lambda s: KV.kv4_read_rows(c, c, z(2), z(2), z(2, 4), stream=s),
+                 lambda s: KV.kv4_decode(q, c, c, z(2, 4), z(2), 0.1, stream=s),
+                 lambda s: A.prompt_packed(q, q, q, z(2), 0.1, stream=s),
+                 lambda s: KV.fork_pages(c[None], z(2, 4), z(2), z(2), stream=s),
+                 lambda s: KV.compact_pages(c[None], z(2, 4), z(2), stream=s)):
+        with pytest.raises(ValueError, match="stream"):
+            call(other)
+        call(torch.cuda.Stream(gpu))
+    torch.cuda.synchronize()

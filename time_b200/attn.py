@@ -171,6 +171,8 @@ def on_stream(t, stream, call, *args):
     if stream is None:
         # the handle of torch.cuda.current_stream() without the object, which takes longer than the launch's arguments
         return call(torch._C._cuda_getCurrentRawStream(device), *args)
+    if stream.device_index != device:
+        raise ValueError(f"a stream of cuda:{stream.device_index} for tensors on {t.device}")
     with torch.cuda.stream(stream):
         return call(stream.cuda_stream, *args)
 
