@@ -206,6 +206,21 @@ def test_page_tables_have_two_dimensions(shape, rows):
         KV.compact_pages(c[None], table, i32(2))
 
 
+@pytest.mark.parametrize("shared", ["expanded", "strided"])
+def test_workspaces_are_contiguous(shared):
+    """A workspace of more elements than memory would be written past its end."""
+    import torch
+    i32 = lambda *n: torch.zeros(*n, dtype=torch.int32)
+    ws = torch.zeros(1, dtype=torch.uint8).expand(1 << 20) if shared == "expanded" else torch.zeros(1 << 20, dtype=torch.uint8)[::2]
+    c = torch.zeros(4, 1, 1152, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="workspace"):
+        KV.kv4_decode(torch.zeros(2, 4, 128, dtype=torch.bfloat16), c, c, i32(2, 4), i32(2), 0.1, workspace=ws)
+    with pytest.raises(ValueError, match="workspace"):
+        KV.fork_pages(c[None], i32(2, 4), i32(2), i32(2), workspace=ws)
+    with pytest.raises(ValueError, match="workspace"):
+        KV.compact_pages(c[None], i32(2, 4), i32(2), workspace=ws)
+
+
 # ---------------------------------------------------------------- the plain statements themselves
 
 def test_quantiser_by_hand():

@@ -73,6 +73,11 @@ def _check_page_table(page_table, rows, row_seq):
         raise ValueError("the page table has a row per row of the call when row_seq is None")
 
 
+def _check_workspace(workspace):
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("the workspace is contiguous")
+
+
 @functools.lru_cache(maxsize=1024)
 def _splits(B: int, nq: int, nkv: int, max_context: int, split_tokens: int | None, max_splits: int | None):
     """(tokens of a split, splits, workspace bytes)."""
@@ -161,6 +166,7 @@ def kv4_decode(q, k_cache, v_cache, page_table, seq_lens, scale: float, row_seq=
     if seq_lens.numel() != B or (B if row_seq is None else row_seq.numel()) != B:
         raise ValueError("seq_lens and row_seq have one entry per row of q")
     _check_page_table(page_table, B, row_seq)
+    _check_workspace(workspace)
     return A.on_stream(q, stream, _decode, q, k_cache, v_cache, page_table, seq_lens, scale, row_seq, split_tokens,
                        max_splits, quant, workspace, error_word)
 
@@ -212,6 +218,7 @@ def fork_pages(caches, table, lens, parents, reserve=None, workspace=None, error
     new tensors."""
     A.check_i32(table, lens, parents, reserve, error_word)
     _check_table(table, lens)
+    _check_workspace(workspace)
     if reserve is not None and reserve.numel() != parents.numel():
         raise ValueError("reserve has one entry per parent")
     return A.on_stream(caches, stream, _fork, caches, table, lens, parents, reserve, workspace, error_word)
@@ -237,6 +244,7 @@ def compact_pages(caches, table, lens, out=None, workspace=None, error_word=None
     be `table` itself."""
     A.check_i32(table, lens, out, error_word)
     _check_table(table, lens)
+    _check_workspace(workspace)
     if out is not None and out.shape != table.shape:
         raise ValueError("out has the page table's shape")
     return A.on_stream(caches, stream, _compact, caches, table, lens, out, workspace, error_word)
