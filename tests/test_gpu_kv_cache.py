@@ -750,3 +750,23 @@ def test_streams_of_another_device_are_refused(gpu):
             call(other)
         call(torch.cuda.Stream(gpu))
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("nq,nkv,lens", [(12, 1, [300, 1, 2000]), (16, 8, [700])])
+def test_decode_under_a_table_much_wider_than_the_contexts(gpu, nq, nkv, lens):
+    """Room for 131072 tokens a row, the split that goes by it, and what is behind a row's pages not looked at."""
+    rng = np.random.default_rng(nkv)
+    pool = sum(map(R.pages, lens)) + 3
+    kc, vc = random_cache(rng, pool, nkv)
+    pt = np.full((len(lens), 8192), 1 << 30, np.int32)
+    narrow = table_of(rng, lens, pool)
+    for b, n in enumerate(lens):
+        pt[b, :R.pages(n)] = narrow[b, :R.pages(n)]
+    q = normal_bf16(rng, len(lens), nq, D)
+    err = i32([0], gpu)
+    out = f64(KV.kv4_decode(q.to(gpu), torch.from_numpy(kc).to(gpu), torch.from_numpy(vc).to(gpu), i32(pt, gpu), i32(lens, gpu),
+                            D ** -0.5, error_word=err)[0])
+    assert int(err) == 0
+    for b, n in enumerate(lens):
+        ref, tol = R.attend(f64(q[b:b + 1]), seq_values(kc, "k", pt[b], n), seq_values(vc, "v", pt[b], n), [n], D ** -0.5)
+        assert (np.abs(out[b] - ref[0]) <= tol[0]).all()

@@ -461,3 +461,15 @@ def test_quantised_rows_of_tiny_values(gpu):
         amax = got.abs().amax(dim=2, keepdim=True) * (1 + 2.0 ** -7) + 2.0 ** -134
         tol = (2.0 ** -4 + 2.0 ** -7) * got.abs() + amax / 448 * 2.0 ** -10 * 1.01 + 448 * 2.0 ** -150 + 2.0 ** -134
         assert not held[..., 64:].any() and ((held - got).abs() <= tol).all()
+
+
+def test_a_long_prompt(gpu):
+    """16384 tokens, rows at the ends of steps and tiles and between, each against all the keys it attends."""
+    rng = np.random.default_rng(16)
+    n, nq = 16384, 12
+    q, k, v = rows(rng, n, nq, D).to(gpu), rows(rng, n, 1, D).to(gpu), rows(rng, n, 1, D).to(gpu)
+    err = torch.zeros(1, dtype=torch.int32, device=gpu)
+    out, _, _ = A.prompt_packed(q, k, v, cu_of([n], gpu), D ** -0.5, error_word=err)
+    at = [0, 20, 21, 63, 64, 1100, 4095, 8190, 8191, 12345, 16319, 16320, 16383]
+    ref, tol = R.attend(f64(q[at]), f64(k), f64(v), [t + 1 for t in at], D ** -0.5)
+    assert int(err) == 0 and (np.abs(f64(out[at]) - ref) <= tol).all()
