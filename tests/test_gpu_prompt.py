@@ -473,3 +473,38 @@ def test_a_long_prompt(gpu):
     at = [0, 20, 21, 63, 64, 1100, 4095, 8190, 8191, 12345, 16319, 16320, 16383]
     ref, tol = R.attend(f64(q[at]), f64(k), f64(v), [t + 1 for t in at], D ** -0.5)
     assert int(err) == 0 and (np.abs(f64(out[at]) - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("G,many", [(1, False), (5, False), (12, True), (16, False)])
+def test_infinities_and_nan_anywhere(gpu, G, many):
+    """Rows far behind them, in sequences of several lengths and two heads of keys: each dim is what the values that its row
+    attends make it; whole rows of NaN, from which on everything is."""
+    rng = np.random.default_rng(G)
+    lens = [1500, 3, 700, 64, 257]
+    T, nkv = sum(lens), 2
+    q, k, v = torch.zeros(T, nkv * G, D), torch.zeros(T, nkv, D), rows(rng, T, nkv, D)
+    q[..., 0] = 1.0
+    k[..., 0] = torch.from_numpy(rng.standard_normal((T, nkv)).astype(np.float32) - 300.0 * (rng.random((T, nkv)) < 0.3))
+    bad = rng.random((T, nkv, D)) < (0.02 if many else 0.0005)
+    kind = rng.choice([np.inf, -np.inf, np.nan], (T, nkv, D))
+    if not many:
+        bad[900], kind[900] = True, np.nan
+        bad[1600], kind[1600] = True, np.nan
+    bv = torch.where(torch.from_numpy(bad), torch.from_numpy(kind).to(torch.bfloat16), v)
+    q, k = q.to(torch.bfloat16).to(gpu), k.to(torch.bfloat16).to(gpu)
+    cu = cu_of(lens, gpu)
+    clean = A.prompt_packed(q, k, torch.where(torch.from_numpy(bad), torch.zeros_like(v), v).to(gpu), cu, 1.0)[0]
+    out, oq, os_ = A.prompt_packed(q, k, bv.to(gpu), cu, 1.0, quant=True)
+    assert same(out, A.prompt_packed(q, k, bv.to(gpu), cu, 1.0)[0])
+    want = clean.cpu()
+    at = 0
+    for n in lens:
+        s = slice(at, at + n)
+        plus, minus, nan = (np.maximum.accumulate(bad[s] & c, axis=0) for c in
+                            (kind[s] == np.inf, kind[s] == -np.inf, np.isnan(kind[s])))
+        for hit, x in ((plus, np.inf), (minus, -np.inf), (nan | (plus & minus), np.nan)):
+            want[s][torch.from_numpy(hit.repeat(G, axis=1))] = x
+        at += n
+    assert same(out.cpu(), want)
+    held = oq.view(torch.float8_e4m3fn).double().reshape(T, nkv * G, D).cpu()
+    assert torch.equal(torch.isnan(held * os_[:, :T].double().t()[..., None].cpu()).any(dim=2), (~torch.isfinite(want)).any(dim=2))

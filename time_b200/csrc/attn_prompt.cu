@@ -284,90 +284,140 @@ __device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
 
 // NaN and infinities in V.  A weight is positive however small, so a row that
 // attends infinities of one sign is that infinity in their dim, and with both
-// signs or a NaN it is NaN.  The MMAs give that unless a weight, or the factor of a
-// rescale, is too small for fp32: 0 times infinity.  And they see zeros in place
-// of such values behind a tile's first position.  Where either may be, the epilogue
-// settles these dims from V itself: what a row is depends on no tile.
-struct NonFinite {
-    int plus[4], minus[4], nan[4];                      // first positions with each in dims 4 lane .. 4 lane + 3
+// signs or a NaN it is NaN.  The MMAs give that but for two cases: a weight, or the
+// factor of a rescale, too small for fp32 makes NaN of an infinity, and V behind a
+// tile's first position has zeros in place of such values.  So where a row is NaN
+// although its sum of weights is a number, the epilogue looks for such values in
+// those dims of all of the sequence's V, and where V was cleaned, in all dims behind
+// the first position: what a row is depends on no tile.  (One NaN in V at the start
+// of a prompt of 16384 tokens: 954 us instead of 632; a whole row of them 1284.)
+struct Settled {
+    uint32_t over;                                      // chunks of 8 dims whose outcome stands in place of the row's value,
+                                                        // not beside it; alike in the warp
+    uint16_t dims[16];                                  // 2 bits a dim of this lane's row: 0 nothing, 1 inf, 2 -inf, 3 NaN
 };
+__device__ __forceinline__ float settle(float x, const Settled& s, int c, int e) {
+    const uint32_t k = s.dims[c] >> (2 * e) & 3u;
+    if (k == 0) return x;
+    const float y = __uint_as_float(k == 1 ? 0x7F800000u : k == 2 ? 0xFF800000u : 0x7FFFFFFFu);
+    return s.over >> c & 1 ? y : x + y;
+}
 
-// Over the first n positions of a sequence, by a warp; no further than to where every dim is NaN.
-__device__ __forceinline__ NonFinite find_nonfinite(const PromptParams& p, long long first, int kvh, int n) {
-    const int lane = threadIdx.x & 31;
-    constexpr int kNone = 0x7FFFFFFF, kTurn = 8;
-    NonFinite at;
+// By a warp, its lanes' rows at `pos`; `nan_chunks`: the chunks of this lane's row with a NaN to be settled.  A lane
+// looks at a row of V at a time, eight dims of it.
+__device__ __noinline__ void find_settled(const PromptParams& p, long long first, int pos0, int pos, int kvh, bool dirty,
+                                          uint32_t nan_chunks, Settled& out) {
+    constexpr int kNone = 0x7FFFFFFF, kBatch = 8;
+    const int lane = threadIdx.x & 31, n = __reduce_max_sync(0xffffffffu, pos) + 1;
+    out.over = __reduce_or_sync(0xffffffffu, nan_chunks);
+#pragma unroll 1
+    for (int c = 0; c < 16; ++c) {
+        const __nv_bfloat16* v = p.v + first * p.v_stride + kvh * kD + 8 * c;
+        int at[3][8];                                   // first position with inf, -inf, NaN
 #pragma unroll
-    for (int e = 0; e < 4; ++e) at.plus[e] = at.minus[e] = at.nan[e] = kNone;
-    const __nv_bfloat16* v = p.v + first * p.v_stride + kvh * kD + 4 * lane;
-    for (int j0 = 0; j0 < n; j0 += kTurn) {
-        uint2 x[kTurn];
+        for (int e = 0; e < 8; ++e) at[0][e] = at[1][e] = at[2][e] = kNone;
+        bool any = false;
+        for (int j0 = out.over >> c & 1 ? 0 : dirty ? pos0 + 1 : n; j0 < n; j0 += 32 * kBatch) {
+            uint4 x[kBatch];
 #pragma unroll
-        for (int i = 0; i < kTurn; ++i) x[i] = j0 + i < n ? *reinterpret_cast<const uint2*>(v + (j0 + i) * p.v_stride) : make_uint2(0, 0);
-        bool all_nan = true;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-#pragma unroll
-            for (int i = 0; i < kTurn; ++i) {
-                const uint32_t y = ((e < 2 ? x[i].x : x[i].y) >> (16 * (e & 1))) & 0xFFFFu;
-                if (y == 0x7F80u) at.plus[e] = min(at.plus[e], j0 + i);
-                else if (y == 0xFF80u) at.minus[e] = min(at.minus[e], j0 + i);
-                else if ((y & 0x7F80u) == 0x7F80u) at.nan[e] = min(at.nan[e], j0 + i);
+            for (int i = 0; i < kBatch; ++i) {
+                const int j = j0 + 32 * i + lane;
+                x[i] = j < n ? *reinterpret_cast<const uint4*>(v + j * p.v_stride) : make_uint4(0, 0, 0, 0);
             }
-            all_nan &= at.nan[e] != kNone;
-        }
-        if (__all_sync(0xffffffffu, all_nan)) break;
-    }
-    return at;
-}
-
-// Dim 4 c + e of the row at `pos`: bf16 bits of what it is, 0 where it attends numbers only; the whole warp comes here.
-__device__ __forceinline__ uint32_t settled(const NonFinite& at, int c, int e, int pos) {
-    const bool plus = __shfl_sync(0xffffffffu, at.plus[e], c) <= pos, minus = __shfl_sync(0xffffffffu, at.minus[e], c) <= pos;
-    const bool nan = __shfl_sync(0xffffffffu, at.nan[e], c) <= pos;
-    return nan || (plus && minus) ? 0x7FFFu : plus ? 0x7F80u : minus ? 0xFF80u : 0u;
-}
-
-// bf16 rows as they lie in shared memory (see the epilogue), one a lane; `sums`: the row's sum of weights is a number above 0.
-__device__ __noinline__ void settle_rows(const PromptParams& p, uint8_t* rows_sm, int i_row, long long first, int pos, int kvh,
-                                         bool sums) {
-    const NonFinite at = find_nonfinite(p, first, kvh, __reduce_max_sync(0xffffffffu, pos) + 1);
-    for (int c = 0; c < 32; ++c) {
-        uint16_t* x = reinterpret_cast<uint16_t*>(rows_sm + (c >> 4) * kQHalf + i_row * 128 + ((((c >> 1) ^ i_row) & 7) << 4) + (c & 1) * 8);
+            uint32_t found = 0;                         // an exponent of all ones carries into the sign's place
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t y = settled(at, c, e, pos);
-            if (y && sums) x[e] = static_cast<uint16_t>(y);
+            for (int i = 0; i < kBatch; ++i)
+                found |= ((x[i].x & 0x7F807F80u) + 0x00800080u) | ((x[i].y & 0x7F807F80u) + 0x00800080u) |
+                         ((x[i].z & 0x7F807F80u) + 0x00800080u) | ((x[i].w & 0x7F807F80u) + 0x00800080u);
+            if (!__any_sync(0xffffffffu, found & 0x80008000u)) continue;
+            any = true;
+            uint32_t nans = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const uint32_t w = e < 2 ? x[i].x : e < 4 ? x[i].y : e < 6 ? x[i].z : x[i].w;
+                    const uint32_t y = w >> (16 * (e & 1)) & 0xFFFFu;
+                    const int j = j0 + 32 * i + lane;
+                    if (y == 0x7F80u) at[0][e] = min(at[0][e], j);
+                    else if (y == 0xFF80u) at[1][e] = min(at[1][e], j);
+                    else if ((y & 0x7F80u) == 0x7F80u) at[2][e] = min(at[2][e], j);
+                }
+                nans |= static_cast<uint32_t>(at[2][e] != kNone) << e;
+            }
+            if (__reduce_or_sync(0xffffffffu, nans) == 0xFFu) break;       // NaN from there on whatever comes
         }
+        uint32_t dims = 0;
+        if (any) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool plus = __reduce_min_sync(0xffffffffu, at[0][e]) <= pos, minus = __reduce_min_sync(0xffffffffu, at[1][e]) <= pos;
+                const bool nan = __reduce_min_sync(0xffffffffu, at[2][e]) <= pos;
+                dims |= (nan ? 3u : static_cast<uint32_t>(plus) | static_cast<uint32_t>(minus) << 1) << (2 * e);
+            }
+        }
+        out.dims[c] = static_cast<uint16_t>(dims);
+    }
+}
+
+// 16-byte chunk c of output row i in shared memory (see the epilogue).
+__device__ __forceinline__ uint4* row_chunk(uint8_t* rows_sm, int i, int c) {
+    return reinterpret_cast<uint4*>(rows_sm + (c >> 3) * kQHalf + i * 128 + (((c ^ i) & 7) << 4));
+}
+
+// The bf16 rows in shared memory, one a lane; `sums`: the row's sum of weights is a number above 0.
+__device__ __noinline__ void settle_rows(const PromptParams& p, uint8_t* rows_sm, int i_row, long long first, int pos0, int pos, int kvh,
+                                         bool dirty, bool sums) {
+    uint32_t nan_chunks = 0;
+    for (int c = 0; c < 16; ++c) {
+        const uint4 x = *row_chunk(rows_sm, i_row, c);
+        const uint32_t m = max2_nan(max2_nan(x.x, x.y), max2_nan(x.z, x.w));
+        if (sums && ((m & 0x7FFFu) > 0x7F80u || (m & 0x7FFF0000u) > 0x7F800000u)) nan_chunks |= 1u << c;
+    }
+    Settled s;
+    find_settled(p, first, pos0, pos, kvh, dirty, nan_chunks, s);
+    if (!sums) return;
+    for (int c = 0; c < 16; ++c) {
+        if (!s.dims[c]) continue;
+        __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(row_chunk(rows_sm, i_row, c));
+        for (int e = 0; e < 8; ++e) x[e] = __float2bfloat16_rn(settle(__bfloat162float(x[e]), s, c, e));
     }
 }
 
 // The e4m3 rows and their scales, from the output in TMEM.
-__device__ __noinline__ void settle_quantised(const PromptParams& p, uint32_t to, float inv, long long first, int pos, int kvh,
-                                              int head, bool sums, bool store) {
-    const NonFinite at = find_nonfinite(p, first, kvh, __reduce_max_sync(0xffffffffu, pos) + 1);
+__device__ __noinline__ void settle_quantised(const PromptParams& p, uint32_t to, float inv, long long first, int pos0, int pos, int kvh,
+                                              int head, bool dirty, bool sums, bool store) {
+    auto columns = [&](int b, float (&x)[16]) {
+        uint32_t o[16];
+        __syncwarp();
+        tmem_ld16(to + 16 * b, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(o[e]) * inv;
+    };
+    float x[16];
+    uint32_t nan_chunks = 0;
+    for (int b = 0; b < 8; ++b) {
+        columns(b, x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            if (sums && store && x[e] != x[e]) nan_chunks |= 1u << (2 * b + e / 8);
+    }
+    Settled s;
+    find_settled(p, first, pos0, pos, kvh, dirty, nan_chunks, s);
+    if (!sums)
+        for (int c = 0; c < 16; ++c) s.dims[c] = 0;
     const long long out_row = (first + pos) * p.nq + head;
     float amax = 0.0f;
     for (int pass = 0; pass < 2; ++pass) {
         const E4m3Row r = e4m3_row(amax);
         for (int b = 0; b < 8; ++b) {
-            uint32_t o[16];
-            __syncwarp();
-            tmem_ld16(to + 16 * b, o);
-            tmem_wait_ld();
+            columns(b, x);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float x[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t y = settled(at, 4 * b + c, e, pos);
-                    x[e] = y && sums ? __uint_as_float(y << 16) : __uint_as_float(o[4 * c + e]) * inv;
-                    amax = pass == 0 ? fmaxf(amax, fabsf(x[e])) : amax;
-                }
-                if (pass == 1 && store)
-                    *reinterpret_cast<uint32_t*>(p.out_q + out_row * kD + 16 * b + 4 * c) =
-                        cvt_e4m3x2(x[0] * r.up * r.inv, x[1] * r.up * r.inv) |
-                        static_cast<uint32_t>(cvt_e4m3x2(x[2] * r.up * r.inv, x[3] * r.up * r.inv)) << 16;
+            for (int e = 0; e < 16; ++e) {
+                x[e] = settle(x[e], s, 2 * b + e / 8, e % 8);
+                if (pass == 0) amax = fmaxf(amax, fabsf(x[e]));
+                else if (store) p.out_q[out_row * kD + 16 * b + e] = static_cast<uint8_t>(cvt_e4m3x2(x[e] * r.up * r.inv, 0.0f));
             }
         }
     }
@@ -375,8 +425,8 @@ __device__ __noinline__ void settle_quantised(const PromptParams& p, uint32_t to
 }
 
 // The e4m3 rows and their scales.
-__device__ __noinline__ void quantise_output(const PromptParams& p, uint32_t to, float inv, long long first, int pos, int kvh, int head,
-                                             bool sums, bool store, bool dirty) {
+__device__ __noinline__ void quantise_output(const PromptParams& p, uint32_t to, float inv, long long first, int pos0, int pos, int kvh,
+                                             int head, bool dirty, bool sums, bool store) {
     auto columns = [&](int c, float (&x)[32]) {         // 32 dims of the row
         uint32_t o[32];
         __syncwarp();
@@ -397,7 +447,7 @@ __device__ __noinline__ void quantise_output(const PromptParams& p, uint32_t to,
         for (int e = 0; e < 32; e += 2) nan = max3_nan(nan, x[e], x[e + 1]);
     }
     if (dirty || __any_sync(0xffffffffu, nan != nan && sums && store)) {
-        settle_quantised(p, to, inv, first, pos, kvh, head, sums, store);
+        settle_quantised(p, to, inv, first, pos0, pos, kvh, head, dirty, sums, store);
         return;
     }
     const E4m3Row r = e4m3_row(amax);
@@ -584,10 +634,8 @@ prompt_kernel(const __grid_constant__ PromptParams p, const __grid_constant__ CU
             const long long first = w.first;
             // Rows go through shared memory in place of the queries, in their layout: a full tile leaves as one box, and of
             // one in part filled a store instruction covers two rows and not a sector of each of 32.
-            uint8_t* rows_sm = q_s + (n & 1) * kQBytes;             // 16-byte chunk c of row i
-            auto chunk = [&](int i, int c) {
-                return reinterpret_cast<uint4*>(rows_sm + (c >> 3) * kQHalf + i * 128 + (((c ^ i) & 7) << 4));
-            };
+            uint8_t* rows_sm = q_s + (n & 1) * kQBytes;
+            auto chunk = [&](int i, int c) { return row_chunk(rows_sm, i, c); };
             const bool box = rows == tile_pos * p.G;
 #pragma unroll 1
             for (int t = 0; t < mt; ++t) {
@@ -604,7 +652,7 @@ prompt_kernel(const __grid_constant__ PromptParams p, const __grid_constant__ CU
                 const bool store = i_row < rows;
                 const bool sums = l > 0.0f;             // else the row is NaN, whatever V holds
                 if (p.out_q) {
-                    quantise_output(p, to, inv, first, pos, kvh, head, sums, store, dirty);
+                    quantise_output(p, to, inv, first, pos0, pos, kvh, head, dirty, sums, store);
                     __syncwarp();
                 }
                 uint32_t nan = 0;
@@ -628,7 +676,8 @@ prompt_kernel(const __grid_constant__ PromptParams p, const __grid_constant__ CU
                         *chunk(i_row, 8 * c + e) = make_uint4(pack(8 * e), pack(8 * e + 2), pack(8 * e + 4), pack(8 * e + 6));
                 }
                 const bool is_nan = (nan & 0x7FFFu) > 0x7F80u || (nan & 0x7FFF0000u) > 0x7F800000u;
-                if (dirty || __any_sync(0xffffffffu, is_nan && sums && store)) settle_rows(p, rows_sm, i_row, first, pos, kvh, sums);
+                if (dirty || __any_sync(0xffffffffu, is_nan && sums && store))
+                    settle_rows(p, rows_sm, i_row, first, pos0, pos, kvh, dirty, sums && store);
                 if (box) continue;
                 __syncwarp();
                 const int row0 = t * 128 + (warp & 3) * 32;
