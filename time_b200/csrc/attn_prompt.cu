@@ -424,8 +424,9 @@ __device__ __noinline__ void settle_quantised(const PromptParams& p, uint32_t to
     if (store) p.out_s[static_cast<size_t>(head) * p.out_ld + first + pos] = e4m3_row(amax).scale;
 }
 
-// The e4m3 rows and their scales.
-__device__ __noinline__ void quantise_output(const PromptParams& p, uint32_t to, float inv, long long first, int pos0, int pos, int kvh,
+// The e4m3 rows and their scales.  (Not a call: the whole kernel comes out slower with one more, 97 us instead of 95 for
+// seven prompts of up to 1201 with 96 heads, 728 instead of 722 for one of 16384.)
+__device__ __forceinline__ void quantise_output(const PromptParams& p, uint32_t to, float inv, long long first, int pos0, int pos, int kvh,
                                              int head, bool dirty, bool sums, bool store) {
     auto columns = [&](int c, float (&x)[32]) {         // 32 dims of the row
         uint32_t o[32];
