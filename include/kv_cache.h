@@ -69,7 +69,9 @@ moe_status_t attn_kv4_read_rows(const void* k_cache, const void* v_cache, int nu
                                 void* k_out_bf16, void* v_out_bf16, int* error_word, cwStream_t stream);
 
 /* Context split for attn_kv4_decode_rows that fills the GPU at this batch and
- * longest context; max_splits = ceil(max_context / split). */
+ * longest context; max_splits = ceil(max_context / split).  max_context is best
+ * the longest context of the call, not what the page table has room for: the
+ * split grows with it, and the grid and the workspace with max_splits. */
 int attn_kv4_split_tokens(int B, int nkv, int max_context);
 /* Bytes of the split-partials workspace. */
 size_t attn_kv4_decode_workspace_bytes(int B, int nq, int max_splits);

@@ -296,16 +296,17 @@ kv4_read_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__
 // the file's head, S = Q K^T and O += P V on mma.sync with the group's query
 // heads as M, one online softmax whose maximum is left behind by up to 2^8.
 // mma.sync, because its B fragments are registers: a code goes from the ring to
-// the tensor core without a way back through shared memory, and a group's 16 rows
-// would leave seven eighths of a tcgen05 tile empty.
+// the tensor core without a way back through shared memory.  On tcgen05 the same
+// holds with the page's tokens and dims as M and the heads as N, the unpacked page
+// being the operand in TMEM; that form has not been built.
 //
 // Bound by what a page costs to unpack, not by its bytes: 366 instructions a page
 // and KV head, a third of them shifts and masks; the ALU pipe is 52 % busy, the
 // tensor pipe 38 %, and three CTAs (168 registers) leave a scheduler under three
 // warps.  Measured (B200, device time): 64 contexts of up to 16384, 64 heads on 8
-// KV heads, 189 us or 3.2 TB/s of pages; 64 of up to 32768, 12 heads, 56 us or
-// 2.4 TB/s, the merge and uneven lengths in it; 16 of up to 8191, 96
-// heads, 32 us; one of 32768, 10 us.  Slower: four CTAs of 128 registers, shifts as
+// KV heads, 169 us or 3.2 TB/s of pages; 64 of up to 32768, 12 heads, 53 us or
+// 2.5 TB/s, the merge and uneven lengths in it; 16 of up to 8191, 96
+// heads, 31 us; one of 32768, 10 us; the e4m3 rows add under 1 us.  Slower: four CTAs of 128 registers, shifts as
 // multiplications, scores of the next pair under this one's softmax.
 
 constexpr int kWarps = 4;
@@ -879,7 +880,8 @@ int attn_kv4_split_tokens(int B, int nkv, int max_context) {
     // One CTA's fixed cost is that of about 14 pages (4 us beside 0.27 us a page, 3 CTAs an SM).  One wave of the 444
     // CTAs at half the longest context, as long as that leaves splits of 256 to 1536 tokens; longer contexts go in two
     // waves or more, which even out uneven lengths (64 rows up to 32K: 2048 tokens 65 us, 1184 59 us).  A context that one
-    // split of 512 tokens holds needs no merge.
+    // split of 512 tokens holds needs no merge.  max_context is what a caller has room for: where its contexts are far
+    // shorter, few CTAs get the work (one row of 4096 tokens, 8 KV heads: 8.7 us, and 18.3 with max_context 131072).
     if (max_context <= 512) return (max_context + kPage - 1) / kPage * kPage;
     long long split = static_cast<long long>(B) * nkv * max_context / (2 * 444);
     if (split > 1536) split = split / 2 < 2048 ? split / 2 : 2048;

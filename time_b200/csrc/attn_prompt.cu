@@ -10,12 +10,13 @@
 //
 // Bound: the tensor pipe, 4 * 128 * nq * sum of L (L + 1) / 2 operations over
 // the lengths L.  Measured (B200, device time): one prompt of 16384 tokens, 12 query
-// heads on one KV head, 635-710 us or 1160-1290 TFLOP/s, where the power limit
-// sets the clock; one of 4096 with 96 heads on 8 KV heads, 351 us or 1175; four of
-// 1024, 120 us or 860; seven of up to 1201, 97 us or 780: a CTA has nine tiles
-// there, and first and last steps take longer than those between; 24 of up to 201,
-// 12 heads, 11.2 us: under one wave, launch, first loads, four steps and output in
-// a row.
+// heads on one KV head, 632 us or 1300 TFLOP/s in a short run and 722 us or 1140 in
+// a long one, where the power limit sets the clock; one of 4096 with 96 heads on 8
+// KV heads, 399 us or 1030, and four of 1024, 123-143 us, after those; seven of up to
+// 1201, 95 us or 800: a CTA has nine tiles there, and first and last steps take
+// longer than those between; 24 of up to 201, 12 heads, 9.8 us: under one wave,
+// launch, first loads, four steps and output in a row.  With the e4m3 rows 734, 110
+// and 10.8 us for the first, the seven and the 24.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -1028,9 +1029,9 @@ moe_status_t attn_prompt_packed(const void* q_bf16, long long q_stride, const vo
     // every sequence has at most one tile in part filled
     auto tiles_of = [&](int pos) { return ((T + pos - 1ll) / pos + num_seqs) * nkv; };
     // Where tiles of one M tile find an SM each, twice as many SMs run half as many rows (24 prompts of up to 201 tokens, 12
-    // heads: 11.2 us instead of 12.8; one of 128: 8.8 instead of 10.7).  A step of one M tile takes two thirds of one of
-    // two, so long prompts gain up to two tiles an SM (one of 2000: 31 instead of 35), while for short ones the second
-    // tile costs more (20 of 100: 13.5 instead of 12.0).  A row's bits are the same either way.
+    // heads: 9.8 us instead of 11.9; one of 128: 8.1 instead of 9.7).  A step of one M tile takes two thirds of one of
+    // two, so long prompts gain up to two tiles an SM (one of 2000: 29.9 instead of 34.5), while for short ones the second
+    // tile costs more (20 of 100: 12.2 instead of 11.0).  A row's bits are the same either way.
     const long long small = tiles_of(128 / p.G);
     p.tile_pos = small <= kSms || (small <= 2 * kSms && T >= 500ll * num_seqs) ? 128 / p.G : kRows / p.G;
     const long long tiles = tiles_of(p.tile_pos);

@@ -154,7 +154,9 @@ def _read_rows(stream, k_cache, v_cache, positions, row_seq, page_table, error_w
 def kv4_decode(q, k_cache, v_cache, page_table, seq_lens, scale: float, row_seq=None, split_tokens: int | None = None,
                max_splits: int | None = None, quant: bool = False, workspace=None, error_word=None, stream=None):
     """attn_kv4_decode_rows: attention of q bf16 [B][nq][128] over the first seq_lens[b] tokens of page-table row
-    row_seq[b] (None: b).  split_tokens None: the split that fills the GPU.  Returns (out bf16 [B][nq][128], out_q e4m3
+    row_seq[b] (None: b).  split_tokens None: the split that fills the GPU if contexts are as long as the page table is wide;
+    under a table much wider than they are, give split_tokens and max_splits (attn_kv4_split_tokens of the longest context
+    on hand).  Returns (out bf16 [B][nq][128], out_q e4m3
     [B][nq * 128] or None, out_s [nq][ld] or None)."""
     import torch
     _check_kv4(k_cache, v_cache)
