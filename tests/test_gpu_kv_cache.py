@@ -749,7 +749,7 @@ def test_streams_of_another_device_are_refused(gpu):
         with pytest.raises(ValueError, match="stream"):
             call(other)
         call(torch.cuda.Stream(gpu))
-    torch.cuda.synchronize()
+        torch.cuda.synchronize()                           # before the call's tensors go
 
 
 @pytest.mark.parametrize("nq,nkv,lens", [(12, 1, [300, 1, 2000]), (16, 8, [700])])
